@@ -2,7 +2,7 @@
  * slate_cuda.h -- C ABI of slate-b200: a Blackwell (sm_100a) CUDA backend for
  * eating-and-drinking/slate's LLaMA-style Q4_K continuous-batching decode.
  *
- * Three layers, all plain C types (no CUDA or torch types in signatures):
+ * Four layers, all plain C types (no CUDA or torch types in signatures):
  *
  *   1. The compute-backend vtable.  `slate_backend_t` is layout-identical to
  *      the reference's `struct slate_backend` (include/slate/backend.h:41-99)
@@ -10,13 +10,15 @@
  *      (src/backend/backend_cuda_stub.c:33).  `slate_backend_cuda_t` appends
  *      status-returning batched entries after the 13 reference members, so a
  *      `const slate_backend_t*` taken from it works with unchanged callers.
- *   2. The device-resident LLaMA batch engine (`slate_llama_batch_*`): the
+ *   2. Cache operators on a paged KV cache in f32, f16 or 8 bits: rotary append,
+ *      read-back, attention of token trees, acceptance of drafted trees.
+ *   3. The device-resident LLaMA batch engine (`slate_llama_batch_*`): the
  *      batched counterpart of slate_llama_decode_step
  *      (src/loader/llama_infer.c:134-206) with the continuous-batching shape of
  *      slate_infer_batch_step (src/infer/engine.c:543-642, include/slate/
  *      infer.h:168-187).  Weights live in HBM, KV is paged on the GPU, and
  *      slots / page tables / positions are maintained on the device.
- *   3. A micro-batching scheduler over the batch engine with the contract of
+ *   4. A micro-batching scheduler over the batch engine with the contract of
  *      slate_scheduler_* (src/server/scheduler.c, include/slate/scheduler.h:
  *      40-60), plus helpers (GGUF loading, synthetic model writer, Q4_K
  *      quantiser) used by tests and benchmarks.
@@ -68,6 +70,8 @@ typedef struct slate_backend {
 /* KV element types for the paged cache. */
 #define SLATE_KV_F32 0   /* the reference's dtype (llama_infer.c:225-226) */
 #define SLATE_KV_F16 1   /* IEEE binary16, round-to-nearest-even on append */
+#define SLATE_KV_Q8  2   /* 8 bits with one f32 scale for each (token, kv head), K
+                            and V apart; taken by the cache operators below */
 
 /* Appended entries.  All pointers are device pointers; work is enqueued on the
  * backend's stream (sync() waits for it).  Each returns 0 or <0. */
@@ -175,7 +179,135 @@ int slate_cuda_attention_paged_gqa_noalloc(float* out, const float* q, const int
                                            int kv_dtype, void* stream);
 
 /* ------------------------------------------------------------------------ */
-/* 2. Device-resident LLaMA batch engine                                     */
+/* 2. Cache operators: rotary append, read-back, tree attention, acceptance  */
+/* ------------------------------------------------------------------------ */
+/* They work on a paged cache described by slate_kv_cache_t, of the pool layout
+ * documented at slate_llama_batch_new_desc (pool[layer][page][K|V][kv_head]
+ * blocks of 16 tokens) in any of the three element types.  A SLATE_KV_Q8 block
+ * is 16 f32 scales followed by [16 tokens][head_dim] int8, 64 + 16 * head_dim
+ * bytes; an element stands for scale * int8.  The scale of a row x is
+ * amax(|x|) * (1/127) in f32 and its elements rint(x / scale); a row that holds
+ * an infinity or NaN reads back as NaN, a row of zeros as zeros.
+ *
+ * All pointers are device pointers unless noted, 16-byte aligned pools; work is
+ * enqueued on `stream` (a cudaStream_t, NULL = the legacy default stream)
+ * without synchronisation or allocation, so every call can be captured into a
+ * graph.  Each returns 0, -1 for bad arguments (before any launch; the message
+ * is in slate_cuda_last_error()) or -5 when a launch fails.  head_dim is a
+ * multiple of 4 from 4 to 256.  Table entries, slots and indexes are checked on
+ * the device: a token without a page is neither read nor written. */
+typedef struct slate_kv_cache {
+    void* pool;                  /* n_layers * n_pages * 2 * n_kv_heads blocks */
+    const int32_t* page_table;   /* [n_slots][max_pages], -1 = no page */
+    int64_t n_pages;
+    int n_slots, max_pages, n_layers, n_kv_heads, head_dim, kv_dtype;
+} slate_kv_cache_t;
+
+/* Bytes of a pool (0 for bad arguments). */
+size_t slate_kv_pool_bytes(int kv_dtype, int64_t n_pages, int n_layers, int n_kv_heads, int head_dim);
+
+/* Rotary positions: tables [n_pos][rot_dim / 2] of cos and sin (device), the
+ * rotated pairs (j, j + rot_dim/2) (SLATE_ROPE_HALF, the engine's layout) or
+ * (2j, 2j + 1) (SLATE_ROPE_INTERLEAVED) of the first rot_dim dims of a head;
+ * the other dims pass unchanged. */
+#define SLATE_ROPE_HALF        0
+#define SLATE_ROPE_INTERLEAVED 1
+typedef struct slate_rope {
+    const float* cos;
+    const float* sin;
+    int n_pos, rot_dim, layout;
+} slate_rope_t;
+
+/* Scalings of the frequencies for contexts beyond the trained length. */
+#define SLATE_ROPE_SCALE_NONE   0
+#define SLATE_ROPE_SCALE_LINEAR 1   /* positions divided by factor */
+#define SLATE_ROPE_SCALE_NTK    2   /* theta * factor^(rot_dim / (rot_dim - 2)) */
+#define SLATE_ROPE_SCALE_BANDS  3   /* by wavelength w against trained length T: divided by
+                                       factor where w > T / low, kept where w < T / high,
+                                       interpolated linearly in T / w between */
+typedef struct slate_rope_scaling {
+    int kind;
+    float factor;        /* >= 1 */
+    float low, high;     /* BANDS: 0 < low < high */
+    int trained;         /* BANDS: trained context length */
+    float magnitude;     /* cos and sin are multiplied by it (0 = 1) */
+} slate_rope_scaling_t;
+
+/* Fills HOST tables cos, sin [n_pos][rot_dim / 2] with the angles
+ * pos * theta^(-2j / rot_dim), scaled (scaling NULL = none), in f64 rounded
+ * once to f32.  Returns 0 or -1. */
+int slate_rope_tables(float* cos, float* sin, int n_pos, int rot_dim, float theta,
+                      const slate_rope_scaling_t* scaling);
+
+/* For each of `rows` tokens r: q_out[r] = q[r] (n_heads heads, f32, row strides
+ * ld_q / ld_q_out in floats) turned to position row_pos[r]; k[r] turned and
+ * v[r] (n_kv_heads heads) written to place row_index[r] of slot row_slot[r] in
+ * `layer`, rounded to f16 or quantised to 8 bits as they are written.  q_out
+ * may be q; q, k and v may be parts of one row (one ld).  A row with a negative
+ * row_index or a row_pos outside the tables is skipped; two rows of a call must
+ * not name the same place. */
+int slate_cuda_rope_append(const slate_kv_cache_t* cache, int layer, const slate_rope_t* rope,
+                           int rows, int n_heads, float* q_out, int ld_q_out, const float* q,
+                           int ld_q, const float* k, int ld_k, const float* v, int ld_v,
+                           const int32_t* row_slot, const int32_t* row_index,
+                           const int32_t* row_pos, void* stream);
+
+/* Reads the cache back: K, V [n_layers][rows][n_kv_heads * head_dim] (layers
+ * layer0 .. layer0 + n_layers - 1) of type out_dtype (SLATE_KV_F32 or _F16,
+ * rounded once) hold the rows at places (row_slot[r], row_index[r]), in any
+ * order; zeros for a place without a page. */
+int slate_cuda_kv_read(const slate_kv_cache_t* cache, int layer0, int n_layers, int rows,
+                       const int32_t* row_slot, const int32_t* row_index, void* K, void* V,
+                       int out_dtype, void* stream);
+
+/* The nodes of n_seq token trees (drafted tokens, or one token each for an
+ * ordinary decode step): sequence s has the rows row_off[s] .. row_off[s+1]-1
+ * (0 to SLATE_TREE_MAX_NODES nodes; a node after its ancestors), its cache is
+ * slot[s], which holds ctx[s] tokens of context followed by the nodes' own K/V
+ * (node i at place ctx[s] + i).  mask[row] bit j: the node sees node j of its
+ * sequence (a tree: its ancestors and itself). */
+#define SLATE_TREE_MAX_NODES 64
+typedef struct slate_tree {
+    int n_seq, rows;             /* rows = row_off[n_seq] */
+    int max_nodes;               /* of a sequence; picks the kernel, 1..64 */
+    const int32_t* row_off;      /* [n_seq + 1] */
+    const int32_t* slot;         /* [n_seq] */
+    const int32_t* ctx;          /* [n_seq] */
+    const uint64_t* mask;        /* [rows] */
+} slate_tree_t;
+
+/* Host helper: masks of n nodes (ancestors and itself) from their parents
+ * (parent[i] < i, -1 = follows the context).  Host arrays.  Returns 0 or -1. */
+int slate_tree_masks(uint64_t* mask, const int32_t* parent, int n);
+
+/* out[row] (n_heads heads of head_dim, f32, row stride ld_out) = attention of
+ * q[row] over the sequence's context and the nodes that its mask names, with
+ * grouped heads (n_heads % n_kv_heads == 0), scores scaled by `scale`.
+ * A row that sees nothing gets zeros; what a row does not see has no influence
+ * on it, whatever it holds.  ws: slate_cuda_attention_tree_workspace() bytes of
+ * device memory, 16-byte aligned, that calls which may overlap do not share. */
+size_t slate_cuda_attention_tree_workspace(const slate_kv_cache_t* cache, int n_heads, int n_seq,
+                                           int rows, int max_nodes);
+int slate_cuda_attention_tree(const slate_kv_cache_t* cache, int layer, const slate_tree_t* tree,
+                              int n_heads, float* out, int ld_out, const float* q, int ld_q,
+                              float scale, void* ws, size_t ws_bytes, void* stream);
+
+/* Greedy verification of drafted trees: token[row] is a node's token, target[row]
+ * the model's next token after it, parent[row] its parent's index in the
+ * sequence (-1: none, the node is taken as given).  A node is accepted when it
+ * and all nodes of its mask are given or equal their parents' target; the
+ * deepest accepted node (most mask bits; ties to the lowest index) ends the
+ * path.  For sequence s: out_count[s] = nodes of the path, out_node[s][64] their
+ * indexes and out_token[s][64] their targets (the new tokens), -1 beyond; the
+ * path's K/V rows of every layer are moved to places ctx[s], ctx[s] + 1, ...
+ * (ctx itself is not changed). */
+int slate_cuda_tree_accept(const slate_kv_cache_t* cache, const slate_tree_t* tree,
+                           const int32_t* parent, const int32_t* token, const int32_t* target,
+                           int32_t* out_count, int32_t* out_node, int32_t* out_token,
+                           void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* 3. Device-resident LLaMA batch engine                                     */
 /* ------------------------------------------------------------------------ */
 
 /* One transformer block's weights, member-for-member the reference's
@@ -373,7 +505,7 @@ int slate_llama_batch_profile(slate_llama_batch_t* b, int kernel, int n, int lay
                               float* ms);
 
 /* ------------------------------------------------------------------------ */
-/* 3. Scheduler (single decoder thread, scheduler.c:45-99 contract)          */
+/* 4. Scheduler (single decoder thread, scheduler.c:45-99 contract)          */
 /* ------------------------------------------------------------------------ */
 typedef struct slate_llama_scheduler slate_llama_scheduler_t;
 slate_llama_scheduler_t* slate_llama_scheduler_new(slate_llama_batch_t* b, int max_batch);

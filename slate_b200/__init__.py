@@ -18,6 +18,10 @@ LIB_PATH = os.path.join(HERE, "libslate_cuda.so")
 
 KV_F32 = 0
 KV_F16 = 1
+KV_Q8 = 2
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_NTK, ROPE_SCALE_BANDS = range(4)
+TREE_MAX_NODES = 64
 PROF_ATTENTION, PROF_QKV, PROF_WO, PROF_GATE_UP, PROF_DOWN, PROF_LM_HEAD, PROF_STEP, PROF_ALLREDUCE = \
     range(8)
 
@@ -72,6 +76,30 @@ def sampler_configs(n, temperature=1.0, top_k=0, top_p=0.0):
     return arr
 
 
+class KVCache(C.Structure):
+    """slate_kv_cache_t: a paged cache (device addresses and sizes)."""
+    _fields_ = [("pool", P), ("page_table", P), ("n_pages", c_int64)] + \
+               [(n, c_int) for n in ("n_slots", "max_pages", "n_layers", "n_kv_heads", "head_dim",
+                                     "kv_dtype")]
+
+
+class Rope(C.Structure):
+    """slate_rope_t: device tables [n_pos][rot_dim / 2] and the pairs' layout."""
+    _fields_ = [("cos", P), ("sin", P), ("n_pos", c_int), ("rot_dim", c_int), ("layout", c_int)]
+
+
+class RopeScaling(C.Structure):
+    """slate_rope_scaling_t."""
+    _fields_ = [("kind", c_int), ("factor", c_float), ("low", c_float), ("high", c_float),
+                ("trained", c_int), ("magnitude", c_float)]
+
+
+class TreeBatch(C.Structure):
+    """slate_tree_t: the nodes of a batch of token trees (device addresses)."""
+    _fields_ = [("n_seq", c_int), ("rows", c_int), ("max_nodes", c_int), ("row_off", P),
+                ("slot", P), ("ctx", P), ("mask", P)]
+
+
 class SynthConfig(C.Structure):
     _fields_ = [(n, c_int) for n in ("n_layers", "d_model", "ffn_hidden", "n_heads", "n_kv_heads",
                                      "vocab", "max_seq")] + [
@@ -110,6 +138,16 @@ EXPORTS = {
     "slate_cuda_sample_rows": (c_int, Pi32, P, c_int, c_int, c_int, P, C.POINTER(c_u64)),
     "slate_cuda_attention_paged_gqa_noalloc": (c_int, P, P, P, P, P, c_int, P, c_int64, c_int, c_int,
                                                c_int, c_int, c_int, c_int, P),
+    "slate_kv_pool_bytes": (c_size, c_int, c_int64, c_int, c_int, c_int),
+    "slate_rope_tables": (c_int, Pf32, Pf32, c_int, c_int, c_float, C.POINTER(RopeScaling)),
+    "slate_cuda_rope_append": (c_int, C.POINTER(KVCache), c_int, C.POINTER(Rope), c_int, c_int, P,
+                               c_int, P, c_int, P, c_int, P, c_int, P, P, P, P),
+    "slate_cuda_kv_read": (c_int, C.POINTER(KVCache), c_int, c_int, c_int, P, P, P, P, c_int, P),
+    "slate_tree_masks": (c_int, C.POINTER(c_u64), Pi32, c_int),
+    "slate_cuda_attention_tree_workspace": (c_size, C.POINTER(KVCache), c_int, c_int, c_int, c_int),
+    "slate_cuda_attention_tree": (c_int, C.POINTER(KVCache), c_int, C.POINTER(TreeBatch), c_int, P,
+                                  c_int, P, c_int, c_float, P, c_size, P),
+    "slate_cuda_tree_accept": (c_int, C.POINTER(KVCache), C.POINTER(TreeBatch), P, P, P, P, P, P, P),
     "slate_llama_batch_new_desc": (P, C.POINTER(LlamaDesc), C.POINTER(CudaOpts)),
     "slate_llama_batch_new_gguf": (P, C.c_char_p, C.POINTER(CudaOpts)),
     "slate_llama_batch_free": (None, P),
@@ -185,6 +223,64 @@ def sample_rows(d_logits, ld, B, V, cfg, rng):
     rc = F["slate_cuda_sample_rows"](_ptr(out, C.c_int32), d_logits, ld, B, V, C.byref(cfg),
                                      rng.ctypes.data_as(C.POINTER(c_u64)))
     return rc, out
+
+
+# -- cache operators (device addresses as ints; stream: a cudaStream_t as int) ----
+def _ok(rc, what):
+    if rc:
+        raise RuntimeError(f"{what} rc={rc}: {last_error()}")
+
+
+def kv_pool_bytes(kv_dtype, n_pages, n_layers, n_kv_heads, head_dim) -> int:
+    return F["slate_kv_pool_bytes"](kv_dtype, n_pages, n_layers, n_kv_heads, head_dim)
+
+
+def rope_tables(n_pos, rot_dim, theta, scaling: RopeScaling | None = None):
+    """Host cos and sin tables [n_pos, rot_dim / 2] (slate_rope_tables)."""
+    cos = np.empty((max(n_pos, 0), max(rot_dim, 0) // 2), np.float32)
+    sin = np.empty_like(cos)
+    rc = F["slate_rope_tables"](_ptr(cos), _ptr(sin), n_pos, rot_dim, theta, scaling)
+    if rc:
+        raise ValueError(f"slate_rope_tables rc={rc}: {last_error()}")
+    return cos, sin
+
+
+def tree_masks(parent) -> np.ndarray:
+    """uint64 masks (ancestors and itself) of nodes with these parents (-1 = none)."""
+    parent = np.ascontiguousarray(parent, np.int32)
+    mask = np.zeros(len(parent), np.uint64)
+    rc = F["slate_tree_masks"](_ptr(mask, c_u64), _ptr(parent, C.c_int32), len(parent))
+    if rc:
+        raise ValueError(f"slate_tree_masks rc={rc}: {last_error()}")
+    return mask
+
+
+def rope_append(cache, layer, rope, rows, n_heads, q_out, ld_q_out, q, ld_q, k, ld_k, v, ld_v,
+                row_slot, row_index, row_pos, stream=None):
+    _ok(F["slate_cuda_rope_append"](cache, layer, rope, rows, n_heads, q_out, ld_q_out, q, ld_q, k,
+                                    ld_k, v, ld_v, row_slot, row_index, row_pos, stream),
+        "rope_append")
+
+
+def kv_read(cache, layer0, n_layers, rows, row_slot, row_index, K, V, out_dtype=KV_F32,
+            stream=None):
+    _ok(F["slate_cuda_kv_read"](cache, layer0, n_layers, rows, row_slot, row_index, K, V, out_dtype,
+                                stream), "kv_read")
+
+
+def attention_tree_workspace(cache, n_heads, n_seq, rows, max_nodes) -> int:
+    return F["slate_cuda_attention_tree_workspace"](cache, n_heads, n_seq, rows, max_nodes)
+
+
+def attention_tree(cache, layer, tree, n_heads, out, ld_out, q, ld_q, scale, ws, ws_bytes,
+                   stream=None):
+    _ok(F["slate_cuda_attention_tree"](cache, layer, tree, n_heads, out, ld_out, q, ld_q, scale, ws,
+                                       ws_bytes, stream), "attention_tree")
+
+
+def tree_accept(cache, tree, parent, token, target, out_count, out_node, out_token, stream=None):
+    _ok(F["slate_cuda_tree_accept"](cache, tree, parent, token, target, out_count, out_node,
+                                    out_token, stream), "tree_accept")
 
 
 def tp_unique_id() -> bytes:
