@@ -4,6 +4,20 @@
 //   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i.k_j - max_j),
 // over j < ctx (the context) and the nodes j that bit j - ctx of the row's mask
 // names.
+//
+// The M = nodes * group rows that share a kv head are one matrix product with the
+// cache: attn_tree_mma (head_dim 64 and 128) reads the cache once for up to 32 of
+// them and multiplies on the tensor cores; attn_tree_rows takes any head_dim.
+//
+// f32-level products from 16-bit operands.  f16 and 8-bit cache: k and v are
+// exact in f16 (8 bits: the integer; its scale joins the score, or p).  q and p
+// are split into f16 hi + lo (x = hi + lo to ~22 bits), so two products carry
+// what f32 would.  To stay clear of f16's ends each q row is first divided by the
+// power of two below its largest element, and p (at most 1) multiplied by 2^15, so
+// that the lo half of a p of 2^-10 still has its bits.  f32 cache: tf32 hi + lo of
+// both sides, three products.  The running sums stay in f32 registers: every tile's
+// product is formed from zero and added by one FMA with the rescale, because a
+// tensor-core accumulator carried over thousands of tokens would truncate each time.
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -11,6 +25,7 @@
 #include "sb_internal.h"
 #include "sb_kernels.h"
 #include "sb_kv.h"
+#include "sb_pdl.h"
 
 namespace {
 
@@ -115,12 +130,794 @@ __global__ void __launch_bounds__(32 * NW) attn_tree_rows(
     }
 }
 
+// ---------------------------------------------------------------- shared plan
+// The cache's tokens are dealt out evenly: an item is one (sequence, kv head, tile
+// of MR rows), its work ceil(tokens / UNIT) units; the items' units in order are
+// cut into as many equal ranges as there are CTAs.  A CTA that holds the whole of
+// an item writes its output; of a cut item each CTA leaves a partial (max, sum, o)
+// for attn_tree_join.  Contexts of any lengths thereby load every SM alike.
+constexpr int UNIT = 64;
+
+struct Seq {
+    int s, r0, n, slot, ctx;      // rows r0 .. r0 + n - 1
+    int tiles, units;             // row tiles a head; units an item
+};
+__device__ __forceinline__ Seq seq_of(const slate_kv_cache_t& c, const slate_tree_t& tr, int s,
+                                      int G, int MR) {
+    Seq q;
+    q.s = s;
+    q.r0 = max(__ldg(tr.row_off + s), 0);
+    q.n = min(max(min(__ldg(tr.row_off + s + 1), tr.rows) - q.r0, 0), SLATE_TREE_MAX_NODES);
+    q.slot = __ldg(tr.slot + s);
+    q.ctx = min(max(__ldg(tr.ctx + s), 0), c.max_pages * SB_PAGE_TOKENS);
+    q.tiles = (q.n * G + MR - 1) / MR;
+    q.units = (q.ctx + q.n + UNIT - 1) / UNIT;
+    return q;
+}
+__device__ __forceinline__ int64_t seq_units(const Seq& q, int nkv) {
+    return (int64_t)q.tiles * nkv * q.units;
+}
+
+// Total units, and the sequence in which unit `at` lies with the units before it
+// (block-wide; every thread returns the same).  buf: one word a thread + 2.
+template <int NT>
+__device__ int64_t plan_total(const slate_kv_cache_t& c, const slate_tree_t& tr, int G, int MR,
+                              int64_t* buf, int64_t& before) {
+    const int per = (tr.n_seq + NT - 1) / NT, tid = threadIdx.x;
+    int64_t mine = 0;
+    for (int s = tid * per; s < min(tr.n_seq, (tid + 1) * per); ++s)
+        mine += seq_units(seq_of(c, tr, s, G, MR), c.n_kv_heads);
+    int64_t incl = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(FULL, incl, o);
+        if ((tid & 31) >= o) incl += x;
+    }
+    if ((tid & 31) == 31) buf[tid / 32] = incl;
+    __syncthreads();
+    int64_t base = 0, total = 0;
+    for (int w = 0; w < NT / 32; ++w) {
+        if (w < tid / 32) base += buf[w];
+        total += buf[w];
+    }
+    __syncthreads();
+    before = base + incl - mine;
+    return total;
+}
+// The sequence that holds unit `at`, given each thread's `before` and `total`.
+template <int NT>
+__device__ int plan_find(const slate_kv_cache_t& c, const slate_tree_t& tr, int G, int MR,
+                         int64_t* buf, int64_t before, int64_t at, int64_t& seq_before) {
+    const int per = (tr.n_seq + NT - 1) / NT, tid = threadIdx.x;
+    int64_t b = before;
+    for (int s = tid * per; s < min(tr.n_seq, (tid + 1) * per); ++s) {
+        const int64_t u = seq_units(seq_of(c, tr, s, G, MR), c.n_kv_heads);
+        if (at >= b && at < b + u) {
+            buf[0] = s;
+            buf[1] = b;
+        }
+        b += u;
+    }
+    __syncthreads();
+    const int s = (int)buf[0];
+    seq_before = buf[1];
+    __syncthreads();
+    return s;
+}
+// First unit of CTA i of the C that have work (at least a unit each).
+__device__ __forceinline__ int64_t cut(int64_t total, int C, int i) { return total * i / C; }
+
+// ------------------------------------------------------------ tensor-core path
+constexpr int MW = 4;                       // warps a CTA
+
+__device__ __forceinline__ uint32_t su32(const void* p) {
+    return (uint32_t)__cvta_generic_to_shared(p);
+}
+// 16 bytes global -> shared; 0 bytes read and zeros written where !ok.
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+                 "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 "
+                 "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x = hi + lo in f16 pairs / in tf32 (the low 13 bits cut off)
+__device__ __forceinline__ void split_f16(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x0, x1);
+    const float2 b = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x0 - b.x, x1 - b.y);
+    hi = *(const uint32_t*)&h;
+    lo = *(const uint32_t*)&l;
+}
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+    hi = __float_as_uint(x) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
+}
+// Two of the four int8 of w as exact f16: the byte with its sign bit turned is
+// u = x + 128; 0x6400 | u is the f16 1024 + u; minus 1152 leaves x.
+template <int SEL>
+__device__ __forceinline__ uint32_t i8_f16(uint32_t w) {
+    const uint32_t p = __byte_perm(w ^ 0x80808080u, 0x64646464u, SEL);
+    const __half2 h = __hsub2(*(const __half2*)&p, __floats2half2_rn(1152.f, 1152.f));
+    return *(const uint32_t*)&h;
+}
+
+// KT tokens of K and V a tile and warp, ~8 KB, in a ring of NS tiles for each warp
+// (the ring and q fit twice into an SM's shared memory).  A row's 16-byte chunks are
+// exchanged by XOR with a function of the row, so that neither ldmatrix (8 rows, one
+// chunk each) nor the f32 reads (4 or 8 rows) meet in a bank.
+template <int KV, int HD, int MODE>
+struct Shape {
+    static constexpr int RB = KV == SLATE_KV_F32 ? 4 * HD : KV == SLATE_KV_F16 ? 2 * HD : HD;
+    static constexpr int KT = RB == 512 ? 8 : RB == 256 ? 16 : 32;
+    static constexpr int CPR = RB / 16;
+    static constexpr int TB = 2 * KT * RB + (KV == SLATE_KV_Q8 ? 8 * KT : 0);
+    static constexpr int MT = MODE == 2 ? 2 : 1;
+    static constexpr int MR = MODE == 0 ? 8 : 16 * MT;              // rows a tile
+    static constexpr int KS = KV == SLATE_KV_F32 ? HD / 8 : HD / 16;    // k steps of a score
+    static constexpr int HL = MODE == 0 ? 1 : 2;                    // A operands a k step
+    static constexpr int QB = MT * KS * HL * 512;
+    static constexpr int NS0 = (112 * 1024 - QB) / (MW * TB);
+    static constexpr int NS = NS0 > 6 ? 6 : NS0;
+    static constexpr int MERGE = MW * MR * (HD + 2) * 4;
+    static constexpr int RING = MW * NS * TB > MERGE ? MW * NS * TB : MERGE;
+    static constexpr int SMEM = QB + RING + MR * 16;
+};
+template <int KV, int RB>
+__device__ __forceinline__ uint32_t swz(int row, int chunk) {
+    if (KV == SLATE_KV_F32)      // rows 0,2,4,6 (or 1,3,5,7) of one dim, rows 2i and 2i + 1 of 4 chunks
+        return row * RB + ((chunk ^ ((row & 6) ^ ((row & 1) << 2))) << 4);
+    if (RB == 64) {              // two rows a 128-byte line
+        const int line = row >> 1, pos = (row & 1) * 4 + chunk;
+        return line * 128 + ((pos ^ (line & 3)) << 4);
+    }
+    return row * RB + ((chunk ^ (row & 7)) << 4);
+}
+
+// Partial of one cut item: [MR][HD + 2]: (max in log2 units, sum, o) rows.
+template <int KV, int HD, int MODE>
+__global__ void __launch_bounds__(32 * MW, 2) attn_tree_mma(
+    const slate_kv_cache_t c, int layer, const slate_tree_t tr, int nq, float* __restrict__ out,
+    int ld_out, const float* __restrict__ q, int ld_q, float scale, float* __restrict__ ws) {
+    using S = Shape<KV, HD, MODE>;
+    constexpr int KT = S::KT, RB = S::RB, TB = S::TB, NS = S::NS, MT = S::MT, MR = S::MR, KS = S::KS;
+    constexpr int NTK = KT / 8;                       // 8-token score tiles
+    constexpr int NTD = HD / 8;                       // 8-dim output tiles
+    constexpr int RI = MODE == 0 ? 1 : 2 * MT;        // rows a lane
+    extern __shared__ __align__(128) unsigned char smem[];
+    uint4* sq = (uint4*)smem;                         // [MT][KS][HL][32 lanes] A fragments
+    unsigned char* ring = smem + S::QB;
+    float* rowscale = (float*)(smem + S::QB + S::RING);        // [MR]
+    uint64_t* rowmask = (uint64_t*)(rowscale + 2 * ((MR + 1) / 2));   // [MR]
+    __shared__ int64_t buf[MW + 2];
+    sb_grid_release();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+    const int nkv = c.n_kv_heads, G = nq / nkv;
+    int64_t before, seq_before;
+    const int64_t total = plan_total<32 * MW>(c, tr, G, MR, buf, before);
+    const int C = (int)min((int64_t)gridDim.x, total);
+    if ((int)blockIdx.x >= C) return;
+    int64_t at = cut(total, C, blockIdx.x);
+    const int64_t stop = cut(total, C, blockIdx.x + 1);
+    int s = plan_find<32 * MW>(c, tr, G, MR, buf, before, at, seq_before);
+    Seq sq_ = seq_of(c, tr, s, G, MR);
+    const size_t page_blk = sb_kv_block_bytes(KV, HD);
+    unsigned char* myring = ring + (size_t)warp * NS * TB;
+    const uint32_t myring_s = su32(myring);
+
+    for (int seg = 0; at < stop; ++seg) {
+        while (at >= seq_before + seq_units(sq_, nkv)) {
+            seq_before += seq_units(sq_, nkv);
+            sq_ = seq_of(c, tr, ++s, G, MR);
+        }
+        const int64_t rel = at - seq_before;
+        const int item = (int)(rel / sq_.units), u0 = (int)(rel % sq_.units);
+        const int u1 = (int)min((int64_t)sq_.units, u0 + (stop - at));
+        const int kvh = item / sq_.tiles, r_base = (item % sq_.tiles) * MR;
+        const int n_rows = min(MR, sq_.n * G - r_base);
+        const int end = sq_.ctx + sq_.n, tok0 = u0 * UNIT, tok1 = min(end, u1 * UNIT);
+        at += u1 - u0;
+
+        // ---- q as A fragments, each row divided by the power of two below its maximum
+        __syncthreads();                               // the last segment's merge is read
+        for (int r = warp; r < MR; r += MW) {
+            const int row = r_base + r, node = row / G;
+            const bool live = r < n_rows;
+            const float* x = q + (size_t)(sq_.r0 + (live ? node : 0)) * ld_q +
+                             (size_t)(kvh * G + (live ? row % G : 0)) * HD;
+            float v[HD / 32];
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i) {
+                v[i] = live ? x[lane * (HD / 32) + i] : 0.f;
+                top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+            }
+            top = __reduce_max_sync(FULL, top);
+            // exponent of the maximum, kept where 2^-e and 2^e are normal numbers
+            const int e = min(max((int)(top >> 23) - 127, -100), 100);
+            const float inv = __int_as_float((127 - e) << 23);
+            if (lane == 0) {
+                rowscale[r] = scale * 1.4426950408889634f * __int_as_float((127 + e) << 23);
+                rowmask[r] = live ? __ldg(tr.mask + sq_.r0 + node) : 0;
+            }
+            // element d of row r in the fragments: rows r % 16 < 8 in registers 0 and 2
+            const int mt = r / 16, rg = r & 7, up = MODE == 0 ? 0 : (r >> 3) & 1;
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i) {
+                const int d = lane * (HD / 32) + i;
+                const float y = v[i] * inv;
+                if (KV == SLATE_KV_F32) {
+                    // k steps 2j, 2j + 1 hold dims 16j + 4 t4 + {0, 1} and {2, 3}
+                    const int ks = 2 * (d / 16) + ((d & 3) >> 1), t = (d & 15) >> 2, reg = 2 * (d & 1) + up;
+                    uint32_t hi, lo;
+                    split_tf32(y, hi, lo);
+                    uint32_t* f = (uint32_t*)(sq + ((size_t)(mt * KS + ks) * S::HL) * 32 + rg * 4 + t);
+                    f[reg] = hi;
+                    f[MODE == 0 ? reg + 1 : 32 * 4 + reg] = lo;
+                } else {
+                    // f16: k = dim; 8 bits: dims 4 t4 + {0, 1} are k 2 t4 + {0, 1}, {2, 3} k + 8
+                    const int ks = d / 16, w = d & 15;
+                    const int t = KV == SLATE_KV_Q8 ? w >> 2 : (w & 7) >> 1;
+                    const int reg = 2 * (KV == SLATE_KV_Q8 ? (w & 3) >> 1 : w >> 3) + up;
+                    const __half hi = __float2half_rn(y), lo = __float2half_rn(y - __half2float(hi));
+                    __half* f = (__half*)(sq + ((size_t)(mt * KS + ks) * S::HL) * 32 + rg * 4 + t);
+                    f[2 * reg + (d & 1)] = hi;
+                    f[(MODE == 0 ? 2 * (reg + 1) : 32 * 8 + 2 * reg) + (d & 1)] = lo;
+                }
+            }
+        }
+        __syncthreads();
+
+        float o[MT][NTD][4], m[RI], l[RI], rs[RI];
+#pragma unroll
+        for (int a = 0; a < MT; ++a)
+#pragma unroll
+            for (int j = 0; j < NTD; ++j) o[a][j][0] = o[a][j][1] = o[a][j][2] = o[a][j][3] = 0.f;
+#pragma unroll
+        for (int i = 0; i < RI; ++i) {
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+            rs[i] = rowscale[8 * i + g];
+        }
+        float vref = 1.f;                              // Q8: o is in units of vref * 2^-15
+
+        // ---- the warp's tiles: KT tokens each, tiles warp, warp + MW, ...
+        const int tiles = (tok1 - tok0 + KT - 1) / KT;
+        const int mine = warp < tiles ? (tiles - 1 - warp) / MW + 1 : 0;
+        constexpr int PPT = KT > 16 ? KT / 16 : 1;     // pages a tile
+        int win[PPT];                                  // lane i: pages of the warp's tile (base + i)
+        uint32_t absent = 0;                           // bit (stage, page): the table has no such page
+        auto load_window = [&](int base) {
+#pragma unroll
+            for (int p = 0; p < PPT; ++p) {
+                const int t = tok0 + (warp + (base + lane) * MW) * KT + 16 * p;
+                win[p] = base + lane < mine && t < tok1 ? sb_kv_page(c, sq_.slot, t) : -1;
+            }
+        };
+        auto issue = [&](int i) {                      // the warp's i-th tile into stage i % NS
+            if (i < mine) {
+                if ((i & 31) == 0) load_window(i);
+                const int t0 = tok0 + (warp + i * MW) * KT;
+                const uint32_t st = myring_s + (i % NS) * TB;
+#pragma unroll
+                for (int p = 0; p < PPT; ++p) {
+                    const int page = __shfl_sync(FULL, win[p], i & 31);
+                    const uint32_t bit = 1u << ((i % NS) * PPT + p);
+                    absent = page < 0 ? absent | bit : absent & ~bit;
+                    const unsigned char* kb = sb_kv_block(c, layer, max(page, 0), 0, kvh);
+                    const unsigned char* vb = kb + (size_t)nkv * page_blk;
+                    constexpr int ROWS = KT < 16 ? KT : 16, HEAD = KV == SLATE_KV_Q8 ? SB_Q8_SCALES : 0;
+                    const int rsrc = KT < 16 ? t0 & 15 : 0;
+#pragma unroll
+                    for (int e = lane; e < ROWS * S::CPR; e += 32) {
+                        const int r = e / S::CPR, ch = e % S::CPR;
+                        const bool ok = page >= 0 && t0 + 16 * p + r < end;
+                        const size_t so = HEAD + (size_t)(rsrc + r) * RB + ch * 16;
+                        const uint32_t d = swz<KV, RB>(16 * p + r, ch);
+                        cp16(st + d, kb + so, ok);
+                        cp16(st + KT * RB + d, vb + so, ok);
+                    }
+                    if (KV == SLATE_KV_Q8 && lane < 8)
+                        cp16(st + 2 * KT * RB + (lane >= 4 ? 4 * KT : 0) + 64 * p + 16 * (lane & 3),
+                             (lane >= 4 ? vb : kb) + 16 * (lane & 3), page >= 0);
+                }
+            }
+            cp_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < NS - 1; ++i) issue(i);
+        for (int i = 0; i < mine; ++i) {
+            cp_wait<NS - 2>();
+            __syncwarp();
+            const int t0 = tok0 + (warp + i * MW) * KT;
+            const unsigned char* st = myring + (size_t)(i % NS) * TB;
+            const uint32_t ks_ = myring_s + (i % NS) * TB, vs_ = ks_ + KT * RB;
+            const float* ksc = (const float*)(st + 2 * KT * RB);
+            const float* vsc = ksc + KT;
+            float sc[MT][NTK][4];
+#pragma unroll
+            for (int a = 0; a < MT; ++a)
+#pragma unroll
+                for (int j = 0; j < NTK; ++j) sc[a][j][0] = sc[a][j][1] = sc[a][j][2] = sc[a][j][3] = 0.f;
+            // ---- scores
+            if constexpr (KV == SLATE_KV_F32) {
+#pragma unroll
+                for (int cc = 0; cc < HD / 16; ++cc) {
+                    uint4 A[MT][2][S::HL];
+#pragma unroll
+                    for (int a = 0; a < MT; ++a)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+#pragma unroll
+                            for (int h = 0; h < S::HL; ++h)
+                                A[a][k][h] = sq[((size_t)(a * KS + 2 * cc + k) * S::HL + h) * 32 + lane];
+#pragma unroll
+                    for (int j = 0; j < NTK; ++j) {
+                        const float4 x = *(const float4*)(st + swz<KV, RB>(8 * j + g, 4 * cc + t4));
+                        uint32_t bh[4], bl[4];
+                        split_tf32(x.x, bh[0], bl[0]);
+                        split_tf32(x.y, bh[1], bl[1]);
+                        split_tf32(x.z, bh[2], bl[2]);
+                        split_tf32(x.w, bh[3], bl[3]);
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+#pragma unroll
+                            for (int a = 0; a < MT; ++a) {
+                                const uint4 h4 = A[a][k][0], l4 = A[a][k][S::HL - 1];
+                                const uint32_t ah[4] = {h4.x, h4.y, h4.z, h4.w}, al[4] = {l4.x, l4.y, l4.z, l4.w};
+                                mma_tf32(sc[a][j], ah, bl[2 * k], bl[2 * k + 1]);
+                                if (MODE) mma_tf32(sc[a][j], al, bh[2 * k], bh[2 * k + 1]);
+                                mma_tf32(sc[a][j], ah, bh[2 * k], bh[2 * k + 1]);
+                            }
+                    }
+                }
+            } else {
+                // an ldmatrix.x4 brings two 8-token tiles: f16 of one k step, 8 bits of two
+                constexpr int KPL = KV == SLATE_KV_Q8 ? 2 : 1;
+#pragma unroll
+                for (int cc = 0; cc < KS / KPL; ++cc) {
+                    uint4 A[MT][KPL][S::HL];
+#pragma unroll
+                    for (int a = 0; a < MT; ++a)
+#pragma unroll
+                        for (int k = 0; k < KPL; ++k)
+#pragma unroll
+                            for (int h = 0; h < S::HL; ++h)
+                                A[a][k][h] = sq[((size_t)(a * KS + KPL * cc + k) * S::HL + h) * 32 + lane];
+#pragma unroll
+                    for (int jp = 0; jp < NTK / 2; ++jp) {
+                        uint32_t r[4];
+                        ldsm4(ks_ + swz<KV, RB>(16 * jp + (lane >> 4) * 8 + (lane & 7), 2 * cc + ((lane >> 3) & 1)), r);
+#pragma unroll
+                        for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+                            for (int k = 0; k < KPL; ++k) {
+                                const uint32_t b0 = KV == SLATE_KV_Q8 ? i8_f16<0x4140>(r[2 * jj + k]) : r[2 * jj];
+                                const uint32_t b1 = KV == SLATE_KV_Q8 ? i8_f16<0x4342>(r[2 * jj + k]) : r[2 * jj + 1];
+#pragma unroll
+                                for (int a = 0; a < MT; ++a)
+#pragma unroll
+                                    for (int h = S::HL - 1; h >= 0; --h) {
+                                        const uint4 x = A[a][k][h];
+                                        const uint32_t af[4] = {x.x, x.y, x.z, x.w};
+                                        mma_f16(sc[a][2 * jp + jj], af, b0, b1);
+                                    }
+                            }
+                    }
+                }
+            }
+            // ---- softmax over the tile: lane holds tokens 8 j + 2 t4 + e of rows 8 ri + g
+            const uint32_t gone = absent >> ((i % NS) * PPT) & ((1u << PPT) - 1);
+            const bool tail = t0 + KT > sq_.ctx || gone;
+            float p[RI][NTK][2], kf[NTK][2];
+#pragma unroll
+            for (int j = 0; j < NTK; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) kf[j][e] = KV == SLATE_KV_Q8 ? ksc[8 * j + 2 * t4 + e] : 1.f;
+            float corr[RI];
+#pragma unroll
+            for (int ri = 0; ri < RI; ++ri) {
+                float mx = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < NTK; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float d = MODE == 0 ? sc[0][j][e] + sc[0][j][2 + e] : sc[ri >> 1][j][2 * (ri & 1) + e];
+                        p[ri][j][e] = d * (KV == SLATE_KV_Q8 ? rs[ri] * kf[j][e] : rs[ri]);
+                    }
+                if (tail) {
+                    const uint64_t mk = rowmask[8 * ri + g];
+#pragma unroll
+                    for (int j = 0; j < NTK; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int x = t0 + 8 * j + 2 * t4 + e - sq_.ctx;
+                            if ((x >= 0 && (x >= sq_.n || !(mk >> x & 1))) || (gone >> (8 * j / 16) & 1))
+                                p[ri][j][e] = -INFINITY;
+                        }
+                }
+#pragma unroll
+                for (int j = 0; j < NTK; ++j) mx = fmaxf(mx, fmaxf(p[ri][j][0], p[ri][j][1]));
+                mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 2));
+                const float mn = fmaxf(m[ri], mx), base = mn == -INFINITY ? 0.f : mn;
+                corr[ri] = ex2(m[ri] - base);
+                m[ri] = mn;
+                l[ri] *= corr[ri];
+#pragma unroll
+                for (int j = 0; j < NTK; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        p[ri][j][e] = ex2(p[ri][j][e] - base);
+                        l[ri] += p[ri][j][e];
+                    }
+            }
+            // ---- weights of v: 8 bits: p vscale / vref (vref: a power of two not below any
+            // vscale met), so that they keep f16's range; 0 stays 0 whatever the scale
+            if (KV == SLATE_KV_Q8) {
+                float vf[NTK][2], vm = 0.f;
+#pragma unroll
+                for (int j = 0; j < NTK; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int t = 8 * j + 2 * t4 + e;
+                        vf[j][e] = vsc[t];
+                        if (t0 + t < end && vf[j][e] < INFINITY) vm = fmaxf(vm, vf[j][e]);
+                    }
+                vm = fmaxf(vm, __shfl_xor_sync(FULL, vm, 1));
+                vm = fmaxf(vm, __shfl_xor_sync(FULL, vm, 2));
+                if (i == 0 || vm > vref) {
+                    const int e = min(max((int)(__float_as_uint(vm) >> 23) - 126, -80), 126);
+                    const float nref = __int_as_float((127 + e) << 23), f = i ? vref / nref : 0.f;
+#pragma unroll
+                    for (int ri = 0; ri < RI; ++ri) corr[ri] *= f;        // o is rescaled once
+                    vref = nref;
+                }
+                const float vi = 32768.f / vref;
+#pragma unroll
+                for (int j = 0; j < NTK; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float f = vf[j][e] * vi;
+#pragma unroll
+                        for (int ri = 0; ri < RI; ++ri) p[ri][j][e] = p[ri][j][e] == 0.f ? 0.f : p[ri][j][e] * f;
+                    }
+            }
+            // An infinity or NaN in a v that only some rows see would reach the others as
+            // 0 * inf: such values are taken out of the tile and added for the rows that see them.
+            uint32_t odd = 0;
+            if (KV != SLATE_KV_Q8 && tail) {
+                for (int e = lane; e < KT * S::CPR; e += 32) {
+                    const int r = e / S::CPR;
+                    uint32_t* w = (uint32_t*)(st + KT * RB + swz<KV, RB>(r, e % S::CPR));
+                    if (t0 + r < sq_.ctx) continue;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t x = w[k];
+                        uint32_t keep = 0xffffffffu;
+                        if (KV == SLATE_KV_F32) {
+                            if ((x & 0x7f800000u) == 0x7f800000u) keep = 0;
+                        } else {
+                            if ((x & 0x7c00u) == 0x7c00u) keep &= 0xffff0000u;
+                            if ((x & 0x7c000000u) == 0x7c000000u) keep &= 0x0000ffffu;
+                        }
+                        if (keep != 0xffffffffu) {
+                            w[k] = x & keep;
+                            odd |= 1u << r;
+                        }
+                    }
+                }
+                odd = __reduce_or_sync(FULL, odd);
+            }
+            // ---- o = o corr + p v
+            if constexpr (KV == SLATE_KV_F32) {
+#pragma unroll
+                for (int jd = 0; jd < NTD; ++jd) {
+                    float d[MT][4];
+#pragma unroll
+                    for (int a = 0; a < MT; ++a) d[a][0] = d[a][1] = d[a][2] = d[a][3] = 0.f;
+#pragma unroll
+                    for (int j = 0; j < NTK; ++j) {
+                        // k = t4 is token 2 t4, k = t4 + 4 token 2 t4 + 1 of the 8
+                        const int r = 8 * j + 2 * t4, ch = 2 * jd + (g >> 2);
+                        uint32_t bh[2], bl[2];
+                        split_tf32(*(const float*)(st + KT * RB + swz<KV, RB>(r, ch) + 4 * (g & 3)), bh[0], bl[0]);
+                        split_tf32(*(const float*)(st + KT * RB + swz<KV, RB>(r + 1, ch) + 4 * (g & 3)), bh[1], bl[1]);
+#pragma unroll
+                        for (int a = 0; a < MT; ++a) {
+                            uint32_t ah[4], al[4];
+                            if (MODE == 0) {
+                                split_tf32(p[0][j][0], ah[0], ah[1]);
+                                split_tf32(p[0][j][1], ah[2], ah[3]);
+                            } else {
+                                split_tf32(p[(2 * a) % RI][j][0], ah[0], al[0]);
+                                split_tf32(p[(2 * a + 1) % RI][j][0], ah[1], al[1]);
+                                split_tf32(p[(2 * a) % RI][j][1], ah[2], al[2]);
+                                split_tf32(p[(2 * a + 1) % RI][j][1], ah[3], al[3]);
+                                mma_tf32(d[a], al, bh[0], bh[1]);
+                            }
+                            mma_tf32(d[a], ah, bl[0], bl[1]);
+                            mma_tf32(d[a], ah, bh[0], bh[1]);
+                        }
+                    }
+#pragma unroll
+                    for (int a = 0; a < MT; ++a)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            o[a][jd][e] = fmaf(o[a][jd][e], corr[MODE == 0 ? 0 : (2 * a + (e >> 1)) % RI], d[a][e]);
+                }
+            } else {
+                uint32_t P[MT][NTK / 2][S::HL][4];
+#pragma unroll
+                for (int a = 0; a < MT; ++a)
+#pragma unroll
+                    for (int k = 0; k < NTK / 2; ++k)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {          // tokens 16 k + 8 h + 2 t4 + {0, 1}
+                            const float f = KV == SLATE_KV_Q8 ? 1.f : 32768.f;
+                            const int j = 2 * k + h;
+                            if (MODE == 0) {
+                                split_f16(p[0][j][0] * f, p[0][j][1] * f, P[a][k][0][2 * h], P[a][k][0][2 * h + 1]);
+                            } else {
+                                split_f16(p[(2 * a) % RI][j][0] * f, p[(2 * a) % RI][j][1] * f, P[a][k][0][2 * h],
+                                          P[a][k][S::HL - 1][2 * h]);
+                                split_f16(p[(2 * a + 1) % RI][j][0] * f, p[(2 * a + 1) % RI][j][1] * f,
+                                          P[a][k][0][2 * h + 1], P[a][k][S::HL - 1][2 * h + 1]);
+                            }
+                        }
+                // 8 bits: one ldmatrix.x4.trans brings 16 dims of 32 tokens or 32 dims of 16; each
+                // word holds dims (2g, 2g + 1) of two tokens: even dims are one output tile, odd the next
+#pragma unroll
+                for (int jd = 0; jd < NTD; jd += 2) {
+                    float d[MT][2][4];
+#pragma unroll
+                    for (int a = 0; a < MT; ++a)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) d[a][x][0] = d[a][x][1] = d[a][x][2] = d[a][x][3] = 0.f;
+                    if constexpr (KV == SLATE_KV_Q8) {
+#pragma unroll
+                        for (int k2 = 0; k2 < NTK / 4; ++k2) {
+                            uint32_t r[4];
+                            ldsm4t(vs_ + swz<KV, RB>(32 * k2 + lane, jd / 2), r);
+#pragma unroll
+                            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                                for (int x = 0; x < 2; ++x) {
+                                    const uint32_t b0 = x ? i8_f16<0x4341>(r[2 * k]) : i8_f16<0x4240>(r[2 * k]);
+                                    const uint32_t b1 = x ? i8_f16<0x4341>(r[2 * k + 1]) : i8_f16<0x4240>(r[2 * k + 1]);
+#pragma unroll
+                                    for (int a = 0; a < MT; ++a)
+#pragma unroll
+                                        for (int h = S::HL - 1; h >= 0; --h)
+                                            mma_f16(d[a][x], P[a][2 * k2 + k][h], b0, b1);
+                                }
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < NTK / 2; ++k) {
+                            uint32_t r[4];
+                            ldsm4t(vs_ + swz<KV, RB>(16 * k + ((lane >> 3) & 1) * 8 + (lane & 7), jd + (lane >> 4)), r);
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                                for (int a = 0; a < MT; ++a)
+#pragma unroll
+                                    for (int h = S::HL - 1; h >= 0; --h)
+                                        mma_f16(d[a][x], P[a][k][h], r[2 * x], r[2 * x + 1]);
+                        }
+                    }
+#pragma unroll
+                    for (int a = 0; a < MT; ++a)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                o[a][jd + x][e] = fmaf(o[a][jd + x][e], corr[MODE == 0 ? 0 : (2 * a + (e >> 1)) % RI], d[a][x][e]);
+                }
+            }
+            if (KV != SLATE_KV_Q8 && odd) {
+                const float f = KV == SLATE_KV_F16 ? 32768.f : 1.f;
+#pragma unroll
+                for (int j = 0; j < NTK; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        for (int q4 = 0; q4 < 4; ++q4) {
+                            const int r = 8 * j + 2 * q4 + e;
+                            if (!(odd >> r & 1)) continue;
+                            const int page = sb_kv_page(c, sq_.slot, t0 + r);
+                            if (page < 0) continue;
+                            const unsigned char* v = sb_kv_block(c, layer, page, 1, kvh) + (size_t)((t0 + r) & 15) * RB;
+#pragma unroll
+                            for (int ri = 0; ri < RI; ++ri) {
+                                const float pv = __shfl_sync(FULL, p[ri][j][e], (lane & 28) | q4) * f;
+#pragma unroll
+                                for (int jd = 0; jd < NTD; ++jd)
+#pragma unroll
+                                    for (int x = 0; x < 2; ++x) {
+                                        const int d = 8 * jd + 2 * t4 + x;
+                                        const float y = KV == SLATE_KV_F32 ? ((const float*)v)[d] : __half2float(((const __half*)v)[d]);
+                                        if (pv != 0.f && !(fabsf(y) < INFINITY)) o[ri >> 1][jd][2 * (ri & 1) + x] += pv * y;
+                                    }
+                            }
+                        }
+            }
+            __syncwarp();                              // the stage is read: it may be filled again
+            issue(i + NS - 1);
+        }
+        cp_wait<0>();
+        __syncthreads();                               // every warp's ring is drained: reuse it
+
+        // ---- join the four warps: [MW][MR][HD + 2]
+        float* mg = (float*)ring;
+        const float of = KV == SLATE_KV_Q8 ? vref * 0x1p-15f : KV == SLATE_KV_F16 ? 0x1p-15f : 1.f;
+#pragma unroll
+        for (int ri = 0; ri < RI; ++ri) {
+            float* rec = mg + ((size_t)warp * MR + 8 * ri + g) * (HD + 2);
+            float ls = l[ri];
+            ls += __shfl_xor_sync(FULL, ls, 1);
+            ls += __shfl_xor_sync(FULL, ls, 2);
+            if (t4 == 0) {
+                rec[0] = m[ri];
+                rec[1] = ls;
+            }
+#pragma unroll
+            for (int jd = 0; jd < NTD; ++jd)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float x = MODE == 0 ? o[0][jd][e] + o[0][jd][2 + e] : o[ri >> 1][jd][2 * (ri & 1) + e];
+                    const int dd = KV == SLATE_KV_Q8 ? 16 * (jd / 2) + 2 * (2 * t4 + e) + (jd & 1) : 8 * jd + 2 * t4 + e;
+                    rec[2 + dd] = x * of;
+                }
+        }
+        __syncthreads();
+        const bool whole = u0 == 0 && u1 == sq_.units;
+        float* part = ws + (size_t)(2 * blockIdx.x + (seg ? 1 : 0)) * MR * (HD + 2);
+        for (int e = tid; e < n_rows * HD; e += 32 * MW) {
+            const int r = e / HD, d = e % HD;
+            float M = -INFINITY, L = 0.f, O = 0.f;
+#pragma unroll
+            for (int w = 0; w < MW; ++w) M = fmaxf(M, mg[((size_t)w * MR + r) * (HD + 2)]);
+#pragma unroll
+            for (int w = 0; w < MW; ++w) {
+                const float* rec = mg + ((size_t)w * MR + r) * (HD + 2);
+                // a part without a maximum holds zeros, or NaN if it saw one
+                const float f = rec[0] == -INFINITY ? 1.f : ex2(rec[0] - M);
+                L = fmaf(rec[1], f, L);
+                O = fmaf(rec[2 + d], f, O);
+            }
+            if (whole) {
+                const int row = r_base + r;
+                out[(size_t)(sq_.r0 + row / G) * ld_out + (size_t)(kvh * G + row % G) * HD + d] =
+                    L == 0.f ? 0.f : O / L;
+            } else {
+                float* rec = part + (size_t)r * (HD + 2);
+                if (d == 0) {
+                    rec[0] = M;
+                    rec[1] = L;
+                }
+                rec[2 + d] = O;
+            }
+        }
+    }
+}
+
+// Joins the partials of the cut items: one CTA an item, a warp a row in turn.
+template <int HD>
+__global__ void __launch_bounds__(128) attn_tree_join(const slate_kv_cache_t c, const slate_tree_t tr,
+                                                      int nq, int MR, int ctas, float* __restrict__ out,
+                                                      int ld_out, const float* __restrict__ ws) {
+    __shared__ int64_t buf[6];
+    const int nkv = c.n_kv_heads, G = nq / nkv, tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+    const int s = blockIdx.x, kvh = blockIdx.y;
+    int64_t before, first = 0;
+    const int64_t total = plan_total<128>(c, tr, G, MR, buf, before);
+    const Seq q = seq_of(c, tr, s, G, MR);
+    sb_grid_wait();        // the partials; before any return, so that the chain stays ordered
+    if ((int)blockIdx.z >= q.tiles) return;
+    const int C = (int)min((int64_t)ctas, total);
+    // units before this item: its sequence's, from the thread that counted it
+    const int per = (tr.n_seq + 127) / 128;
+    if (tid == s / per) {
+        for (int x = tid * per; x < s; ++x) before += seq_units(seq_of(c, tr, x, G, MR), nkv);
+        buf[4] = before;
+    }
+    __syncthreads();
+    first = buf[4] + (int64_t)(kvh * q.tiles + blockIdx.z) * q.units;
+    const int64_t last = first + q.units - 1;
+    // the CTA that holds unit x: the largest i with cut(i) <= x
+    auto owner = [&](int64_t x) {
+        int i = (int)((x * C) / total);
+        while (i + 1 < C && cut(total, C, i + 1) <= x) ++i;
+        while (i > 0 && cut(total, C, i) > x) --i;
+        return i;
+    };
+    const int c0 = owner(first), c1 = owner(last);
+    if (c0 == c1) return;                                // written by its CTA
+    const int r_base = blockIdx.z * MR, n_rows = min(MR, q.n * G - r_base);
+    for (int r = warp; r < n_rows; r += 4) {
+        float M = -INFINITY, L = 0.f, O[HD / 32];
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) O[i] = 0.f;
+        for (int i = c0 + lane; i <= c1; i += 32)
+            M = fmaxf(M, ws[((size_t)(2 * i + (cut(total, C, i) < first)) * MR + r) * (HD + 2)]);
+        for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(FULL, M, x));
+        for (int i = c0; i <= c1; ++i) {
+            // an item that begins inside the CTA's range is its later segment
+            const float* rec = ws + ((size_t)(2 * i + (cut(total, C, i) < first)) * MR + r) * (HD + 2);
+            const float f = rec[0] == -INFINITY ? 1.f : ex2(rec[0] - M);
+            L = fmaf(rec[1], f, L);
+#pragma unroll
+            for (int k = 0; k < HD / 32; ++k) O[k] = fmaf(rec[2 + lane + 32 * k], f, O[k]);
+        }
+        const int row = r_base + r;
+#pragma unroll
+        for (int k = 0; k < HD / 32; ++k)
+            out[(size_t)(q.r0 + row / G) * ld_out + (size_t)(kvh * G + row % G) * HD + lane + 32 * k] =
+                L == 0.f ? 0.f : O[k] / L;
+    }
+}
+
+constexpr int SMS = 148, CTAS = 2 * SMS;
+
+template <int KV, int HD, int MODE>
+int launch_mma(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq, float* out,
+               int ld_out, const float* q, int ld_q, float scale, float* ws, cudaStream_t st) {
+    using S = Shape<KV, HD, MODE>;
+    const auto k = attn_tree_mma<KV, HD, MODE>;
+    static const cudaError_t ready =
+        cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (ready != cudaSuccess) return sb_cuda_check(ready, "attention_tree shared memory");
+    k<<<CTAS, 32 * MW, S::SMEM, st>>>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws);
+    int rc = sb_cuda_check(cudaGetLastError(), "attention_tree");
+    if (rc) return rc;
+    const int tiles = (tr.max_nodes * (nq / c.n_kv_heads) + S::MR - 1) / S::MR;
+    return sb_cuda_check(sb_launch_pdl(attn_tree_join<HD>, dim3((unsigned)tr.n_seq, (unsigned)c.n_kv_heads, (unsigned)tiles),
+                                       dim3(128), 0, st, c, tr, nq, S::MR, CTAS, out, ld_out, (const float*)ws),
+                         "attention_tree join");
+}
+template <int KV, int HD>
+int launch_mode(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq, float* out,
+                int ld_out, const float* q, int ld_q, float scale, float* ws, cudaStream_t st) {
+    const int M = tr.max_nodes * (nq / c.n_kv_heads);
+    return M <= 8    ? launch_mma<KV, HD, 0>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st)
+           : M <= 16 ? launch_mma<KV, HD, 1>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st)
+                     : launch_mma<KV, HD, 2>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);
+}
+bool takes_mma(const slate_kv_cache_t* c) { return c->head_dim == 64 || c->head_dim == 128; }
+
 }  // namespace
 
 extern "C" size_t slate_cuda_attention_tree_workspace(const slate_kv_cache_t* cache, int n_heads,
                                                       int n_seq, int rows, int max_nodes) {
     if (!cache || n_heads < 1 || n_seq < 1 || rows < 0 || max_nodes < 1) return 0;
-    return 16;
+    // two partials of up to 32 rows for each CTA
+    return takes_mma(cache) ? (size_t)2 * CTAS * 32 * (cache->head_dim + 2) * 4 : 16;
 }
 
 extern "C" int slate_cuda_attention_tree(const slate_kv_cache_t* cache, int layer,
@@ -142,6 +939,16 @@ extern "C" int slate_cuda_attention_tree(const slate_kv_cache_t* cache, int laye
         return -1;
     }
     if (tree->rows == 0) return 0;
+    if (takes_mma(cache)) {
+        const auto f = hd == 64 ? cache->kv_dtype == SLATE_KV_F32   ? launch_mode<SLATE_KV_F32, 64>
+                                  : cache->kv_dtype == SLATE_KV_F16 ? launch_mode<SLATE_KV_F16, 64>
+                                                                    : launch_mode<SLATE_KV_Q8, 64>
+                       : cache->kv_dtype == SLATE_KV_F32   ? launch_mode<SLATE_KV_F32, 128>
+                       : cache->kv_dtype == SLATE_KV_F16 ? launch_mode<SLATE_KV_F16, 128>
+                                                         : launch_mode<SLATE_KV_Q8, 128>;
+        return f(*cache, layer, *tree, n_heads, out, ld_out, q, ld_q, scale, (float*)ws,
+                 (cudaStream_t)stream);
+    }
     attn_tree_rows<<<dim3((unsigned)tree->rows, (unsigned)n_heads), 32 * NW, 0,
                      (cudaStream_t)stream>>>(*cache, layer, *tree, n_heads, out, ld_out, q, ld_q, scale);
     return sb_cuda_check(cudaGetLastError(), "attention_tree");
