@@ -85,9 +85,189 @@ __global__ void __launch_bounds__(256) rope_append_kernel(
     }
 }
 
-// One warp per (layer, row, K|V, head).
-template <typename OT>
+// The same in 16-byte vectors, for head_dim up to 128 and rot_dim % 8 == 0 (every
+// common head): LPH lanes hold a head, four dims each, so a pair's other half is in the
+// same lane (interleaved) or rot_dim / 8 lanes away (one shuffle an element), and a
+// warp keeps RU * 32 / LPH heads in flight.  Bound by HBM: q is read and written, k
+// and v read, the cache written once; nothing else moves.
+constexpr int RU = 4;
+template <int LPH, int KV>
+__global__ void __launch_bounds__(256) rope_append_vec(
+    const slate_kv_cache_t c, int layer, const slate_rope_t rope, int rows, int nq,
+    float* q_out, int ld_qo, const float* q, int ld_q, const float* __restrict__ k, int ld_k,
+    const float* __restrict__ v, int ld_v, const int32_t* __restrict__ row_slot,
+    const int32_t* __restrict__ row_index, const int32_t* __restrict__ row_pos, int parts) {
+    constexpr int HPW = 32 / LPH;
+    const int lane = threadIdx.x & 31, sub = lane % LPH, hd = c.head_dim, nkv = c.n_kv_heads;
+    const int heads = nq + 2 * nkv, half = rope.rot_dim / 2, d = 4 * sub;
+    const unsigned w = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+    const unsigned r = w / parts;
+    if (r >= (unsigned)rows) return;
+    const int h0 = (int)(w % parts) * (RU * HPW) + lane / LPH;
+    const int index = row_index[r], pos = row_pos[r], slot = row_slot[r];
+    if (index < 0 || pos < 0 || pos >= rope.n_pos) return;
+    float4 x[RU];
+#pragma unroll
+    for (int u = 0; u < RU; ++u) {
+        const int h = h0 + u * HPW;
+        x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (h < heads && d < hd) {
+            const float* p = h < nq ? q + (size_t)r * ld_q + (size_t)h * hd
+                             : h < nq + nkv ? k + (size_t)r * ld_k + (size_t)(h - nq) * hd
+                                            : v + (size_t)r * ld_v + (size_t)(h - nq - nkv) * hd;
+            x[u] = *(const float4*)(p + d);
+        }
+    }
+    const bool inter = rope.layout == SLATE_ROPE_INTERLEAVED, second = d >= half;
+    float4 cs = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (d < rope.rot_dim) {
+        const size_t j = (size_t)pos * half + (inter ? d / 2 : second ? d - half : d);
+        if (inter) {
+            const float2 a = *(const float2*)(rope.cos + j), b = *(const float2*)(rope.sin + j);
+            cs = make_float4(a.x, a.x, a.y, a.y);
+            sn = make_float4(b.x, b.x, b.y, b.y);
+        } else {
+            cs = *(const float4*)(rope.cos + j);
+            sn = *(const float4*)(rope.sin + j);
+        }
+    }
+    const int from = inter ? lane : second ? lane - half / 4 : lane + half / 4;
+    const bool turn = d < rope.rot_dim;
+    const int page = sb_kv_page(c, slot, index), t = index % SB_PAGE_TOKENS;
+#pragma unroll
+    for (int u = 0; u < RU; ++u) {
+        const int h = h0 + u * HPW;
+        float4 y = x[u];
+        float4 o;
+        if (inter) {
+            o = make_float4(y.y, y.x, y.w, y.z);
+        } else {
+            o.x = __shfl_sync(FULL, y.x, from & 31);
+            o.y = __shfl_sync(FULL, y.y, from & 31);
+            o.z = __shfl_sync(FULL, y.z, from & 31);
+            o.w = __shfl_sync(FULL, y.w, from & 31);
+        }
+        if (turn && h < nq + nkv) {
+            // first of a pair: a c - b s; second: a s + b c
+            const auto one = [](float a, float b, float cs, float sn, bool sec) {
+                return sec ? __fadd_rn(__fmul_rn(b, sn), __fmul_rn(a, cs))
+                           : __fsub_rn(__fmul_rn(a, cs), __fmul_rn(b, sn));
+            };
+            y.x = one(x[u].x, o.x, cs.x, sn.x, inter ? false : second);
+            y.y = one(x[u].y, o.y, cs.y, sn.y, inter ? true : second);
+            y.z = one(x[u].z, o.z, cs.z, sn.z, inter ? false : second);
+            y.w = one(x[u].w, o.w, cs.w, sn.w, inter ? true : second);
+        }
+        uint32_t top = 0;
+        if (KV == SLATE_KV_Q8) {
+            const uint32_t m = 0x7fffffffu;
+            top = max(max(__float_as_uint(y.x) & m, __float_as_uint(y.y) & m),
+                      max(__float_as_uint(y.z) & m, __float_as_uint(y.w) & m));
+#pragma unroll
+            for (int z = LPH / 2; z; z >>= 1) top = max(top, __shfl_xor_sync(FULL, top, z));
+        }
+        if (h >= heads || d >= hd) continue;
+        if (h < nq) {
+            *(float4*)(q_out + (size_t)r * ld_qo + (size_t)h * hd + d) = y;
+            continue;
+        }
+        if (page < 0) continue;
+        const int hk = h - nq < nkv ? h - nq : h - nq - nkv;
+        unsigned char* blk = sb_kv_block(c, layer, page, h - nq < nkv ? 0 : 1, hk);
+        if (KV == SLATE_KV_F32) {
+            *(float4*)((float*)blk + t * hd + d) = y;
+        } else if (KV == SLATE_KV_F16) {
+            const __half2 a = __floats2half2_rn(y.x, y.y), b = __floats2half2_rn(y.z, y.w);
+            *(uint2*)((__half*)blk + t * hd + d) = make_uint2(*(const uint32_t*)&a, *(const uint32_t*)&b);
+        } else {
+            const float scale = __fmul_rn(__uint_as_float(top), (float)(1.0 / 127.0));
+            const bool plain = scale > 0.f && scale < INFINITY;
+            const auto q8 = [&](float a) {
+                return plain ? (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(a, scale)), -127.f), 127.f) & 255u : 0u;
+            };
+            if (sub == 0) ((float*)blk)[t] = scale;
+            *(uint32_t*)(blk + SB_Q8_SCALES + t * hd + d) =
+                q8(y.x) | q8(y.y) << 8 | q8(y.z) << 16 | q8(y.w) << 24;
+        }
+    }
+}
+
+// A warp per (layer, row), K and V: its n_kv_heads * head_dim / 4 vectors of four in
+// steps of 32, RV vectors of each in flight.  Consecutive lanes write consecutive 16
+// (f16: 8) bytes, and read 4, 8 or 16.  Bound by HBM, mostly by what it writes.
+constexpr int RV = 4;
+template <int KV>
+struct Vec4 {
+    using T = uint32_t;
+};
+template <>
+struct Vec4<SLATE_KV_F16> {
+    using T = uint2;
+};
+template <>
+struct Vec4<SLATE_KV_F32> {
+    using T = float4;
+};
+__device__ __forceinline__ float4 widen(float4 x, float) { return x; }
+__device__ __forceinline__ float4 widen(uint2 x, float) {
+    const float2 a = __half22float2(*(const __half2*)&x.x), b = __half22float2(*(const __half2*)&x.y);
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ float4 widen(uint32_t x, float s) {
+    return make_float4((float)(int8_t)x * s, (float)(int8_t)(x >> 8) * s, (float)(int8_t)(x >> 16) * s,
+                       (float)(int8_t)(x >> 24) * s);
+}
+__device__ __forceinline__ void put4(float* p, float4 x) { *(float4*)p = x; }
+__device__ __forceinline__ void put4(__half* p, float4 x) {
+    const __half2 a = __floats2half2_rn(x.x, x.y), b = __floats2half2_rn(x.z, x.w);
+    *(uint2*)p = make_uint2(*(const uint32_t*)&a, *(const uint32_t*)&b);
+}
+template <typename OT, int KV>
 __global__ void __launch_bounds__(256) kv_read_kernel(
+    const slate_kv_cache_t c, int layer0, int n_layers, int rows,
+    const int32_t* __restrict__ row_slot, const int32_t* __restrict__ row_index,
+    OT* __restrict__ K, OT* __restrict__ V) {
+    using T = typename Vec4<KV>::T;
+    const int lane = threadIdx.x & 31, hd4 = c.head_dim / 4, nv = c.n_kv_heads * hd4;
+    const int64_t w = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+    if (w >= (int64_t)n_layers * rows) return;
+    const int r = (int)(w % rows), layer = layer0 + (int)(w / rows);
+    const int index = row_index[r], page = sb_kv_page(c, row_slot[r], index), t = index % SB_PAGE_TOKENS;
+    const size_t bb = sb_kv_block_bytes(KV, c.head_dim);
+    const unsigned char* kb = page < 0 ? nullptr : sb_kv_block(c, layer, page, 0, 0);
+    const size_t head = KV == SLATE_KV_Q8 ? SB_Q8_SCALES : 0, vo = (size_t)c.n_kv_heads * bb;
+    for (int e0 = lane; e0 < nv; e0 += 32 * RV) {
+        T k[RV] = {}, v[RV] = {};
+        float ks[RV] = {}, vs[RV] = {};
+        if (kb) {
+#pragma unroll
+            for (int i = 0; i < RV; ++i) {
+                const int e = e0 + 32 * i;
+                if (e >= nv) break;
+                const int h = e / hd4;
+                const unsigned char* b = kb + h * bb;
+                const size_t at = head + ((size_t)t * hd4 + (e - h * hd4)) * sizeof(T);
+                k[i] = *(const T*)(b + at);
+                v[i] = *(const T*)(b + vo + at);
+                if (KV == SLATE_KV_Q8) {
+                    ks[i] = ((const float*)b)[t];
+                    vs[i] = ((const float*)(b + vo))[t];
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RV; ++i) {
+            const int e = e0 + 32 * i;
+            if (e >= nv) break;
+            put4(K + ((size_t)w * nv + e) * 4, widen(k[i], ks[i]));
+            put4(V + ((size_t)w * nv + e) * 4, widen(v[i], vs[i]));
+        }
+    }
+}
+
+// One warp per (layer, row, K|V, head): outputs that are not aligned to a vector.
+template <typename OT>
+__global__ void __launch_bounds__(256) kv_read_scalar(
     const slate_kv_cache_t c, int layer0, int n_layers, int rows,
     const int32_t* __restrict__ row_slot, const int32_t* __restrict__ row_index,
     OT* __restrict__ K, OT* __restrict__ V) {
@@ -118,21 +298,28 @@ __global__ void __launch_bounds__(256) kv_read_kernel(
 // (64 nodes, two warp votes), then each thread moves 16-byte (or 4-byte) columns
 // of the path's rows in order.  The path's indexes rise, so the k-th row's place
 // (k) never lies at or behind a later row's source (path[k'] >= k' > k): moving
-// in order never overwrites what is still to be read.
-constexpr int AT = 256;
+// in order never overwrites what is still to be read, nor does reading MU rows ahead.
+constexpr int AT = 256, MU = 8;
 template <typename U>
 __device__ void move_rows(const slate_kv_cache_t& c, int layer, int n, const int* src_page,
                           const int* src_t, const int* dst_page, const int* dst_t) {
     const int rb = sb_kv_row_bytes(c.kv_dtype, c.head_dim), cols = rb / (int)sizeof(U);
     const int head_off = c.kv_dtype == SLATE_KV_Q8 ? SB_Q8_SCALES : 0;
+    const int bb = sb_kv_block_bytes(c.kv_dtype, c.head_dim);
+    const size_t page_bytes = (size_t)2 * c.n_kv_heads * bb;
     for (int e = threadIdx.x; e < 2 * c.n_kv_heads * cols; e += AT) {
-        const int col = e % cols, hw = e / cols, which = hw / c.n_kv_heads, h = hw % c.n_kv_heads;
-        for (int k = 0; k < n; ++k) {
-            if (src_page[k] < 0 || dst_page[k] < 0) continue;
-            const U x = *(const U*)(sb_kv_block(c, layer, src_page[k], which, h) + head_off +
-                                    src_t[k] * rb + col * sizeof(U));
-            *(U*)(sb_kv_block(c, layer, dst_page[k], which, h) + head_off + dst_t[k] * rb +
-                  col * sizeof(U)) = x;
+        const int col = e % cols, hw = e / cols;
+        unsigned char* base = sb_kv_block(c, layer, 0, 0, 0) + hw * (size_t)bb + head_off + col * sizeof(U);
+        for (int k0 = 0; k0 < n; k0 += MU) {
+            U x[MU];
+#pragma unroll
+            for (int u = 0; u < MU; ++u)
+                if (k0 + u < n && src_page[k0 + u] >= 0 && dst_page[k0 + u] >= 0)
+                    x[u] = *(const U*)(base + src_page[k0 + u] * page_bytes + src_t[k0 + u] * rb);
+#pragma unroll
+            for (int u = 0; u < MU; ++u)
+                if (k0 + u < n && src_page[k0 + u] >= 0 && dst_page[k0 + u] >= 0)
+                    *(U*)(base + dst_page[k0 + u] * page_bytes + dst_t[k0 + u] * rb) = x[u];
         }
     }
 }
@@ -234,6 +421,26 @@ extern "C" int slate_cuda_rope_append(const slate_kv_cache_t* cache, int layer,
         sb_set_error("rope_append: %d rows are too many", rows);
         return -1;
     }
+    const auto al = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
+    // vectors need rows and tables on 16 bytes; other strides take the scalar kernel
+    if (hd <= 128 && rope->rot_dim % 8 == 0 && al(q) && al(q_out) && al(k) && al(v) && al(rope->cos) &&
+        al(rope->sin) && ld_q % 4 == 0 && ld_q_out % 4 == 0 && ld_k % 4 == 0 && ld_v % 4 == 0) {
+        const int lph = hd > 64 ? 32 : hd > 32 ? 16 : 8, at_once = RU * (32 / lph);
+        const int parts = (n_heads + 2 * nkv + at_once - 1) / at_once;
+        const int64_t n = (int64_t)rows * parts;
+        const auto go = [&](auto kernel) {
+            kernel<<<(unsigned)((n + 7) / 8), 256, 0, (cudaStream_t)stream>>>(
+                *cache, layer, *rope, rows, n_heads, q_out, ld_q_out, q, ld_q, k, ld_k, v, ld_v, row_slot,
+                row_index, row_pos, parts);
+        };
+        const auto by_type = [&](auto f32, auto f16, auto q8) {
+            cache->kv_dtype == SLATE_KV_F32 ? go(f32) : cache->kv_dtype == SLATE_KV_F16 ? go(f16) : go(q8);
+        };
+        if (lph == 32) by_type(rope_append_vec<32, SLATE_KV_F32>, rope_append_vec<32, SLATE_KV_F16>, rope_append_vec<32, SLATE_KV_Q8>);
+        else if (lph == 16) by_type(rope_append_vec<16, SLATE_KV_F32>, rope_append_vec<16, SLATE_KV_F16>, rope_append_vec<16, SLATE_KV_Q8>);
+        else by_type(rope_append_vec<8, SLATE_KV_F32>, rope_append_vec<8, SLATE_KV_F16>, rope_append_vec<8, SLATE_KV_Q8>);
+        return sb_cuda_check(cudaGetLastError(), "rope_append");
+    }
     rope_append_kernel<<<(unsigned)((warps + 7) / 8), 256, 0, (cudaStream_t)stream>>>(
         *cache, layer, *rope, rows, n_heads, q_out, ld_q_out, q, ld_q, k, ld_k, v, ld_v, row_slot,
         row_index, row_pos);
@@ -250,18 +457,31 @@ extern "C" int slate_cuda_kv_read(const slate_kv_cache_t* cache, int layer0, int
         return -1;
     }
     if (rows == 0) return 0;
-    const int64_t warps = (int64_t)n_layers * rows * 2 * cache->n_kv_heads;
+    const int64_t warps = (int64_t)n_layers * rows * 2 * cache->n_kv_heads;   // of the scalar kernel
     if ((warps + 7) / 8 > 0x7fffffff) {
         sb_set_error("kv_read: %d rows of %d layers are too many", rows, n_layers);
         return -1;
     }
-    const unsigned grid = (unsigned)((warps + 7) / 8);
+    const cudaStream_t st = (cudaStream_t)stream;
+    const uintptr_t mis = ((uintptr_t)K | (uintptr_t)V) & (out_dtype == SLATE_KV_F16 ? 7 : 15);
+    const auto go = [&](auto vec, auto scalar, auto* k, auto* v) {
+        if (mis)
+            scalar<<<(unsigned)((warps + 7) / 8), 256, 0, st>>>(*cache, layer0, n_layers, rows, row_slot, row_index, k, v);
+        else
+            vec<<<(unsigned)(((int64_t)n_layers * rows + 7) / 8), 256, 0, st>>>(*cache, layer0, n_layers, rows, row_slot,
+                                                                               row_index, k, v);
+    };
+    const int kt = cache->kv_dtype;
     if (out_dtype == SLATE_KV_F16)
-        kv_read_kernel<__half><<<grid, 256, 0, (cudaStream_t)stream>>>(
-            *cache, layer0, n_layers, rows, row_slot, row_index, (__half*)K, (__half*)V);
+        go(kt == SLATE_KV_F32   ? kv_read_kernel<__half, SLATE_KV_F32>
+           : kt == SLATE_KV_F16 ? kv_read_kernel<__half, SLATE_KV_F16>
+                                : kv_read_kernel<__half, SLATE_KV_Q8>,
+           kv_read_scalar<__half>, (__half*)K, (__half*)V);
     else
-        kv_read_kernel<float><<<grid, 256, 0, (cudaStream_t)stream>>>(
-            *cache, layer0, n_layers, rows, row_slot, row_index, (float*)K, (float*)V);
+        go(kt == SLATE_KV_F32   ? kv_read_kernel<float, SLATE_KV_F32>
+           : kt == SLATE_KV_F16 ? kv_read_kernel<float, SLATE_KV_F16>
+                                : kv_read_kernel<float, SLATE_KV_Q8>,
+           kv_read_scalar<float>, (float*)K, (float*)V);
     return sb_cuda_check(cudaGetLastError(), "kv_read");
 }
 
