@@ -26,10 +26,11 @@
 #include "sb_kernels.h"
 #include "sb_kv.h"
 #include "sb_pdl.h"
+#include "sb_tree.h"
+
+using namespace sb_tree;
 
 namespace {
-
-constexpr unsigned FULL = 0xffffffffu;
 
 __device__ __forceinline__ float element(const unsigned char* blk, int kv_dtype, int at) {
     return kv_dtype == SLATE_KV_F32   ? ((const float*)blk)[at]
@@ -130,103 +131,18 @@ __global__ void __launch_bounds__(32 * NW) attn_tree_rows(
     }
 }
 
-// ---------------------------------------------------------------- shared plan
-// The cache's tokens are dealt out evenly: an item is one (sequence, kv head, tile
-// of MR rows), its work ceil(tokens / UNIT) units; the items' units in order are
-// cut into as many equal ranges as there are CTAs.  A CTA that holds the whole of
-// an item writes its output; of a cut item each CTA leaves a partial (max, sum, o)
-// for attn_tree_join.  Contexts of any lengths thereby load every SM alike.
-constexpr int UNIT = 64;
-
-struct Seq {
-    int s, r0, n, slot, ctx;      // rows r0 .. r0 + n - 1
-    int tiles, units;             // row tiles a head; units an item
-};
-__device__ __forceinline__ Seq seq_of(const slate_kv_cache_t& c, const slate_tree_t& tr, int s,
-                                      int G, int MR) {
-    Seq q;
-    q.s = s;
-    q.r0 = max(__ldg(tr.row_off + s), 0);
-    q.n = min(max(min(__ldg(tr.row_off + s + 1), tr.rows) - q.r0, 0), SLATE_TREE_MAX_NODES);
-    q.slot = __ldg(tr.slot + s);
-    q.ctx = min(max(__ldg(tr.ctx + s), 0), c.max_pages * SB_PAGE_TOKENS);
-    q.tiles = (q.n * G + MR - 1) / MR;
-    q.units = (q.ctx + q.n + UNIT - 1) / UNIT;
-    return q;
-}
-__device__ __forceinline__ int64_t seq_units(const Seq& q, int nkv) {
-    return (int64_t)q.tiles * nkv * q.units;
-}
-
-// Total units, and the sequence in which unit `at` lies with the units before it
-// (block-wide; every thread returns the same).  buf: one word a thread + 2.
-template <int NT>
-__device__ int64_t plan_total(const slate_kv_cache_t& c, const slate_tree_t& tr, int G, int MR,
-                              int64_t* buf, int64_t& before) {
-    const int per = (tr.n_seq + NT - 1) / NT, tid = threadIdx.x;
-    int64_t mine = 0;
-    for (int s = tid * per; s < min(tr.n_seq, (tid + 1) * per); ++s)
-        mine += seq_units(seq_of(c, tr, s, G, MR), c.n_kv_heads);
-    int64_t incl = mine;
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(FULL, incl, o);
-        if ((tid & 31) >= o) incl += x;
-    }
-    if ((tid & 31) == 31) buf[tid / 32] = incl;
-    __syncthreads();
-    int64_t base = 0, total = 0;
-    for (int w = 0; w < NT / 32; ++w) {
-        if (w < tid / 32) base += buf[w];
-        total += buf[w];
-    }
-    __syncthreads();
-    before = base + incl - mine;
-    return total;
-}
-// The sequence that holds unit `at`, given each thread's `before` and `total`.
-template <int NT>
-__device__ int plan_find(const slate_kv_cache_t& c, const slate_tree_t& tr, int G, int MR,
-                         int64_t* buf, int64_t before, int64_t at, int64_t& seq_before) {
-    const int per = (tr.n_seq + NT - 1) / NT, tid = threadIdx.x;
-    int64_t b = before;
-    for (int s = tid * per; s < min(tr.n_seq, (tid + 1) * per); ++s) {
-        const int64_t u = seq_units(seq_of(c, tr, s, G, MR), c.n_kv_heads);
-        if (at >= b && at < b + u) {
-            buf[0] = s;
-            buf[1] = b;
-        }
-        b += u;
-    }
-    __syncthreads();
-    const int s = (int)buf[0];
-    seq_before = buf[1];
-    __syncthreads();
-    return s;
-}
-// First unit of CTA i of the C that have work (at least a unit each).
-__device__ __forceinline__ int64_t cut(int64_t total, int C, int i) { return total * i / C; }
-
 // ------------------------------------------------------------ tensor-core path
+#ifndef SB_TC_MIN
+#define SB_TC_MIN 32
+#endif
+#ifndef SB_T0
+#define SB_T0 3
+#endif
+constexpr int MAXC = 4 * SMS;               // CTAs at most (join)
+constexpr int UNIT = 64;
+static_assert(MAXC * 32 <= SMS * TC_ROWS, "workspace");
 constexpr int MW = 4;                       // warps a CTA
 
-__device__ __forceinline__ uint32_t su32(const void* p) {
-    return (uint32_t)__cvta_generic_to_shared(p);
-}
-// 16 bytes global -> shared; 0 bytes read and zeros written where !ok.
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0)
-                 : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
@@ -247,27 +163,11 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x = hi + lo in f16 pairs / in tf32 (the low 13 bits cut off)
-__device__ __forceinline__ void split_f16(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x0, x1);
-    const float2 b = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x0 - b.x, x1 - b.y);
-    hi = *(const uint32_t*)&h;
-    lo = *(const uint32_t*)&l;
-}
+// x = hi + lo in tf32 (the low 13 bits cut off)
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
     hi = __float_as_uint(x) & 0xffffe000u;
     lo = __float_as_uint(x - __uint_as_float(hi));
 }
-// Two of the four int8 of w as exact f16: the byte with its sign bit turned is
-// u = x + 128; 0x6400 | u is the f16 1024 + u; minus 1152 leaves x.
-template <int SEL>
-__device__ __forceinline__ uint32_t i8_f16(uint32_t w) {
-    const uint32_t p = __byte_perm(w ^ 0x80808080u, 0x64646464u, SEL);
-    const __half2 h = __hsub2(*(const __half2*)&p, __floats2half2_rn(1152.f, 1152.f));
-    return *(const uint32_t*)&h;
-}
-
 // KT tokens of K and V a tile and warp, ~8 KB, in a ring of NS tiles for each warp
 // (the ring and q fit twice into an SM's shared memory).  A row's 16-byte chunks are
 // exchanged by XOR with a function of the row, so that neither ldmatrix (8 rows, one
@@ -283,7 +183,8 @@ struct Shape {
     static constexpr int KS = KV == SLATE_KV_F32 ? HD / 8 : HD / 16;    // k steps of a score
     static constexpr int HL = MODE == 0 ? 1 : 2;                    // A operands a k step
     static constexpr int QB = MT * KS * HL * 512;
-    static constexpr int NS0 = (112 * 1024 - QB) / (MW * TB);
+    static constexpr int CPS = MODE == 0 ? SB_T0 : 2;                // CTAs an SM
+    static constexpr int NS0 = ((CPS == 2 ? 112 : CPS == 3 ? 74 : 55) * 1024 - QB) / (MW * TB);
     static constexpr int NS = NS0 > 6 ? 6 : NS0;
     static constexpr int MERGE = MW * MR * (HD + 2) * 4;
     static constexpr int RING = MW * NS * TB > MERGE ? MW * NS * TB : MERGE;
@@ -302,7 +203,7 @@ __device__ __forceinline__ uint32_t swz(int row, int chunk) {
 
 // Partial of one cut item: [MR][HD + 2]: (max in log2 units, sum, o) rows.
 template <int KV, int HD, int MODE>
-__global__ void __launch_bounds__(32 * MW, 2) attn_tree_mma(
+__global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_mma(
     const slate_kv_cache_t c, int layer, const slate_tree_t tr, int nq, float* __restrict__ out,
     int ld_out, const float* __restrict__ q, int ld_q, float scale, float* __restrict__ ws) {
     using S = Shape<KV, HD, MODE>;
@@ -315,18 +216,18 @@ __global__ void __launch_bounds__(32 * MW, 2) attn_tree_mma(
     unsigned char* ring = smem + S::QB;
     float* rowscale = (float*)(smem + S::QB + S::RING);        // [MR]
     uint64_t* rowmask = (uint64_t*)(rowscale + 2 * ((MR + 1) / 2));   // [MR]
-    __shared__ int64_t buf[MW + 2];
+    __shared__ PlanBuf buf;
     sb_grid_release();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     const int nkv = c.n_kv_heads, G = nq / nkv;
     int64_t before, seq_before;
-    const int64_t total = plan_total<32 * MW>(c, tr, G, MR, buf, before);
-    const int C = (int)min((int64_t)gridDim.x, total);
-    if ((int)blockIdx.x >= C) return;
-    int64_t at = cut(total, C, blockIdx.x);
-    const int64_t stop = cut(total, C, blockIdx.x + 1);
-    int s = plan_find<32 * MW>(c, tr, G, MR, buf, before, at, seq_before);
-    Seq sq_ = seq_of(c, tr, s, G, MR);
+    const int64_t total = plan_total(c, tr, G, MR, UNIT, buf, before);
+    const Cut cut(total, gridDim.x);
+    if ((int)blockIdx.x >= cut.C) return;
+    int64_t at = cut.first(blockIdx.x);
+    const int64_t stop = cut.first(blockIdx.x + 1);
+    int s = plan_find(c, tr, G, MR, UNIT, buf, before, at, seq_before);
+    Seq sq_ = seq_of(c, tr, s, G, MR, UNIT);
     const size_t page_blk = sb_kv_block_bytes(KV, HD);
     unsigned char* myring = ring + (size_t)warp * NS * TB;
     const uint32_t myring_s = su32(myring);
@@ -334,10 +235,10 @@ __global__ void __launch_bounds__(32 * MW, 2) attn_tree_mma(
     for (int seg = 0; at < stop; ++seg) {
         while (at >= seq_before + seq_units(sq_, nkv)) {
             seq_before += seq_units(sq_, nkv);
-            sq_ = seq_of(c, tr, ++s, G, MR);
+            sq_ = seq_of(c, tr, ++s, G, MR, UNIT);
         }
-        const int64_t rel = at - seq_before;
-        const int item = (int)(rel / sq_.units), u0 = (int)(rel % sq_.units);
+        const uint32_t rel = (uint32_t)(at - seq_before);     // < 2^31: 2^24 tokens of 64 rows a head at most
+        const int item = (int)(rel / (uint32_t)sq_.units), u0 = (int)(rel % (uint32_t)sq_.units);
         const int u1 = (int)min((int64_t)sq_.units, u0 + (stop - at));
         const int kvh = item / sq_.tiles, r_base = (item % sq_.tiles) * MR;
         const int n_rows = min(MR, sq_.n * G - r_base);
@@ -827,64 +728,75 @@ __global__ void __launch_bounds__(32 * MW, 2) attn_tree_mma(
     }
 }
 
-// Joins the partials of the cut items: one CTA an item, a warp a row in turn.
+// Joins the partials of the cut items: one CTA of 128 threads a (sequence, kv head,
+// row).  The records' weights are formed once, then each thread sums its dim over the
+// records (head_dim 64: two halves of the records), several loads in flight.
 template <int HD>
 __global__ void __launch_bounds__(128) attn_tree_join(const slate_kv_cache_t c, const slate_tree_t tr,
-                                                      int nq, int MR, int ctas, float* __restrict__ out,
+                                                      int nq, int MR, int unit, int ctas, float* __restrict__ out,
                                                       int ld_out, const float* __restrict__ ws) {
-    __shared__ int64_t buf[6];
-    const int nkv = c.n_kv_heads, G = nq / nkv, tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
-    const int s = blockIdx.x, kvh = blockIdx.y;
-    int64_t before, first = 0;
-    const int64_t total = plan_total<128>(c, tr, G, MR, buf, before);
-    const Seq q = seq_of(c, tr, s, G, MR);
-    sb_grid_wait();        // the partials; before any return, so that the chain stays ordered
-    if ((int)blockIdx.z >= q.tiles) return;
-    const int C = (int)min((int64_t)ctas, total);
-    // units before this item: its sequence's, from the thread that counted it
+    constexpr int HALVES = 128 / HD;
+    __shared__ PlanBuf buf;
+    __shared__ float wt[MAXC], top[4], so[HALVES - 1 ? 128 : 1], sl[4];
+    const int nkv = c.n_kv_heads, G = nq / nkv, tid = threadIdx.x;
+    const int R = tr.max_nodes * G, s = blockIdx.x / R, row = blockIdx.x % R, kvh = blockIdx.y;
+    int64_t before;
+    const int64_t total = plan_total(c, tr, G, MR, unit, buf, before);
+    const Seq q = seq_of(c, tr, s, G, MR, unit);
     const int per = (tr.n_seq + 127) / 128;
-    if (tid == s / per) {
-        for (int x = tid * per; x < s; ++x) before += seq_units(seq_of(c, tr, x, G, MR), nkv);
-        buf[4] = before;
+    if (tid == s / per) {          // units before this sequence, from the thread that counted them
+        for (int x = tid * per; x < s; ++x) before += seq_units(seq_of(c, tr, x, G, MR, unit), nkv);
+        buf.before = before;
     }
     __syncthreads();
-    first = buf[4] + (int64_t)(kvh * q.tiles + blockIdx.z) * q.units;
-    const int64_t last = first + q.units - 1;
-    // the CTA that holds unit x: the largest i with cut(i) <= x
-    auto owner = [&](int64_t x) {
-        int i = (int)((x * C) / total);
-        while (i + 1 < C && cut(total, C, i + 1) <= x) ++i;
-        while (i > 0 && cut(total, C, i) > x) --i;
-        return i;
-    };
-    const int c0 = owner(first), c1 = owner(last);
-    if (c0 == c1) return;                                // written by its CTA
-    const int r_base = blockIdx.z * MR, n_rows = min(MR, q.n * G - r_base);
-    for (int r = warp; r < n_rows; r += 4) {
-        float M = -INFINITY, L = 0.f, O[HD / 32];
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i) O[i] = 0.f;
-        for (int i = c0 + lane; i <= c1; i += 32)
-            M = fmaxf(M, ws[((size_t)(2 * i + (cut(total, C, i) < first)) * MR + r) * (HD + 2)]);
-        for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(FULL, M, x));
-        for (int i = c0; i <= c1; ++i) {
-            // an item that begins inside the CTA's range is its later segment
-            const float* rec = ws + ((size_t)(2 * i + (cut(total, C, i) < first)) * MR + r) * (HD + 2);
-            const float f = rec[0] == -INFINITY ? 1.f : ex2(rec[0] - M);
-            L = fmaf(rec[1], f, L);
-#pragma unroll
-            for (int k = 0; k < HD / 32; ++k) O[k] = fmaf(rec[2 + lane + 32 * k], f, O[k]);
-        }
-        const int row = r_base + r;
-#pragma unroll
-        for (int k = 0; k < HD / 32; ++k)
-            out[(size_t)(q.r0 + row / G) * ld_out + (size_t)(kvh * G + row % G) * HD + lane + 32 * k] =
-                L == 0.f ? 0.f : O[k] / L;
+    sb_grid_wait();        // the partials; before any return, so that the chain stays ordered
+    if (row >= q.n * G) return;
+    const Cut cut(total, ctas);
+    const int64_t first = buf.before + (int64_t)(kvh * q.tiles + row / MR) * q.units;
+    const int c0 = cut.owner(first), n = cut.owner(first + q.units - 1) - c0 + 1;
+    if (n == 1) return;                                  // written by its CTA
+    // an item that begins inside its first CTA's range is that CTA's later segment
+    const size_t rec = (size_t)MR * (HD + 2);
+    const float* base = ws + (size_t)2 * c0 * rec + (size_t)(row % MR) * (HD + 2);
+    const auto at = [&](int i) { return base + (size_t)2 * i * rec + (i == 0 && cut.first(c0) < first ? rec : 0); };
+    float M = -INFINITY;
+    for (int i = tid; i < n; i += 128) M = fmaxf(M, wt[i] = at(i)[0]);
+    for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(FULL, M, x));
+    if ((tid & 31) == 0) top[tid / 32] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+    float L = 0.f;
+    for (int i = tid; i < n; i += 128) {
+        const float f = wt[i] == -INFINITY ? 1.f : ex2(wt[i] - M);
+        wt[i] = f;
+        L = fmaf(at(i)[1], f, L);
     }
+    for (int x = 16; x; x >>= 1) L += __shfl_xor_sync(FULL, L, x);
+    if ((tid & 31) == 0) sl[tid / 32] = L;
+    __syncthreads();
+    L = sl[0] + sl[1] + sl[2] + sl[3];
+    const int d = tid % HD;
+    float O = 0.f;
+#pragma unroll 8
+    for (int i = tid / HD; i < n; i += HALVES) O = fmaf(at(i)[2 + d], wt[i], O);
+    if (HALVES > 1) {
+        if (tid >= HD) so[tid] = O;
+        __syncthreads();
+        if (tid >= HD) return;
+        O += so[tid + HD];
+    }
+    out[(size_t)(q.r0 + row / G) * ld_out + (size_t)(kvh * G + row % G) * HD + d] = L == 0.f ? 0.f : O / L;
 }
 
-constexpr int SMS = 148, CTAS = 2 * SMS;
 
+
+template <int HD>
+int join(const slate_kv_cache_t& c, const slate_tree_t& tr, int nq, int MR, int unit, int ctas, float* out, int ld_out,
+         const float* ws, cudaStream_t st) {
+    const dim3 grid((unsigned)(tr.n_seq * tr.max_nodes * (nq / c.n_kv_heads)), (unsigned)c.n_kv_heads);
+    return sb_cuda_check(sb_launch_pdl(attn_tree_join<HD>, grid, dim3(128), 0, st, c, tr, nq, MR, unit, ctas, out, ld_out, ws),
+                         "attention_tree join");
+}
 template <int KV, int HD, int MODE>
 int launch_mma(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq, float* out,
                int ld_out, const float* q, int ld_q, float scale, float* ws, cudaStream_t st) {
@@ -893,18 +805,18 @@ int launch_mma(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int
     static const cudaError_t ready =
         cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (ready != cudaSuccess) return sb_cuda_check(ready, "attention_tree shared memory");
-    k<<<CTAS, 32 * MW, S::SMEM, st>>>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws);
-    int rc = sb_cuda_check(cudaGetLastError(), "attention_tree");
-    if (rc) return rc;
-    const int tiles = (tr.max_nodes * (nq / c.n_kv_heads) + S::MR - 1) / S::MR;
-    return sb_cuda_check(sb_launch_pdl(attn_tree_join<HD>, dim3((unsigned)tr.n_seq, (unsigned)c.n_kv_heads, (unsigned)tiles),
-                                       dim3(128), 0, st, c, tr, nq, S::MR, CTAS, out, ld_out, (const float*)ws),
-                         "attention_tree join");
+    k<<<S::CPS * SMS, 32 * MW, S::SMEM, st>>>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws);
+    const int rc = sb_cuda_check(cudaGetLastError(), "attention_tree");
+    return rc ? rc : join<HD>(c, tr, nq, S::MR, UNIT, S::CPS * SMS, out, ld_out, ws, st);
 }
 template <int KV, int HD>
 int launch_mode(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq, float* out,
                 int ld_out, const float* q, int ld_q, float scale, float* ws, cudaStream_t st) {
     const int M = tr.max_nodes * (nq / c.n_kv_heads);
+    if (KV != SLATE_KV_F32 && M > SB_TC_MIN) {
+        const int rc = attend_tc(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);
+        return rc ? rc : join<HD>(c, tr, nq, TC_ROWS, TC_UNIT, SMS, out, ld_out, ws, st);
+    }
     return M <= 8    ? launch_mma<KV, HD, 0>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st)
            : M <= 16 ? launch_mma<KV, HD, 1>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st)
                      : launch_mma<KV, HD, 2>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);
@@ -916,8 +828,8 @@ bool takes_mma(const slate_kv_cache_t* c) { return c->head_dim == 64 || c->head_
 extern "C" size_t slate_cuda_attention_tree_workspace(const slate_kv_cache_t* cache, int n_heads,
                                                       int n_seq, int rows, int max_nodes) {
     if (!cache || n_heads < 1 || n_seq < 1 || rows < 0 || max_nodes < 1) return 0;
-    // two partials of up to 32 rows for each CTA
-    return takes_mma(cache) ? (size_t)2 * CTAS * 32 * (cache->head_dim + 2) * 4 : 16;
+    // two partials for each CTA: 148 of 128 rows, up to 4 * 148 of 32
+    return takes_mma(cache) ? (size_t)2 * SMS * TC_ROWS * (cache->head_dim + 2) * 4 : 16;
 }
 
 extern "C" int slate_cuda_attention_tree(const slate_kv_cache_t* cache, int layer,
@@ -927,7 +839,7 @@ extern "C" int slate_cuda_attention_tree(const slate_kv_cache_t* cache, int laye
     if (sb_kv_check(cache, "attention_tree") || sb_tree_check(tree, "attention_tree")) return -1;
     const int hd = cache->head_dim;
     if (layer < 0 || layer >= cache->n_layers || n_heads < 1 || n_heads % cache->n_kv_heads ||
-        n_heads > 65535 || !out || !q || ld_out < n_heads * hd || ld_q < n_heads * hd ||
+        n_heads > 65535 || (int64_t)tree->n_seq * tree->max_nodes * n_heads > 0x7fffffff || !out || !q || ld_out < n_heads * hd || ld_q < n_heads * hd ||
         !(fabsf(scale) < INFINITY)) {
         sb_set_error("attention_tree: bad arguments");
         return -1;

@@ -1,0 +1,157 @@
+/*
+ * sb_tree.h -- what the tree-attention kernels share (attn_tree.cu,
+ * attn_tree_tc.cu; internal, CUDA C++ only): the cut of the work over the CTAs
+ * and the splitting of operands.
+ */
+#ifndef SB_TREE_H
+#define SB_TREE_H
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "sb_kernels.h"
+#include "sb_kv.h"
+
+namespace sb_tree {
+
+constexpr unsigned FULL = 0xffffffffu;
+constexpr int SMS = 148;
+
+// ---------------------------------------------------------------- shared plan
+// The cache's tokens are dealt out evenly: an item is one (sequence, kv head, tile
+// of MR rows), its work ceil(tokens / unit) units; the items' units in order are
+// cut into as many equal ranges as there are CTAs.  A CTA that holds the whole of
+// an item writes its output; of a cut item each CTA leaves a partial (max, sum, o)
+// for attn_tree_join.  Contexts of any lengths thereby load every SM alike.
+struct Seq {
+    int s, r0, n, slot, ctx;      // rows r0 .. r0 + n - 1
+    int tiles, units;             // row tiles a head; units an item
+};
+__device__ __forceinline__ Seq seq_of(const slate_kv_cache_t& c, const slate_tree_t& tr, int s,
+                                      int G, int MR, int unit) {
+    Seq q;
+    q.s = s;
+    q.r0 = max(__ldg(tr.row_off + s), 0);
+    q.n = min(max(min(__ldg(tr.row_off + s + 1), tr.rows) - q.r0, 0), SLATE_TREE_MAX_NODES);
+    q.slot = __ldg(tr.slot + s);
+    q.ctx = min(max(__ldg(tr.ctx + s), 0), c.max_pages * SB_PAGE_TOKENS);
+    q.tiles = (q.n * G + MR - 1) / MR;
+    q.units = (q.ctx + q.n + unit - 1) / unit;
+    return q;
+}
+__device__ __forceinline__ int64_t seq_units(const Seq& q, int nkv) {
+    return (int64_t)q.tiles * nkv * q.units;
+}
+
+// Block-wide: the units of all sequences, those before this thread's sequences
+// (`per` consecutive ones a thread, the first 128 threads).
+struct PlanBuf {
+    int64_t sum[4];
+    int64_t before;
+    int s;
+};
+__device__ __forceinline__ int64_t plan_total(const slate_kv_cache_t& c, const slate_tree_t& tr, int G, int MR, int unit,
+                                              PlanBuf& buf, int64_t& before) {
+    const int per = (tr.n_seq + 127) / 128, tid = threadIdx.x;
+    int64_t mine = 0;
+    for (int s = tid * per; s < min(tr.n_seq, (tid + 1) * per); ++s)
+        mine += seq_units(seq_of(c, tr, s, G, MR, unit), c.n_kv_heads);
+    int64_t incl = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(FULL, incl, o);
+        if ((tid & 31) >= o) incl += x;
+    }
+    if ((tid & 31) == 31 && tid < 128) buf.sum[tid / 32] = incl;
+    __syncthreads();
+    int64_t base = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (w < tid / 32) base += buf.sum[w];
+        total += buf.sum[w];
+    }
+    before = base + incl - mine;
+    return total;
+}
+// The sequence that holds unit `at` and the units before it.
+__device__ __forceinline__ int plan_find(const slate_kv_cache_t& c, const slate_tree_t& tr, int G, int MR, int unit,
+                                         PlanBuf& buf, int64_t before, int64_t at, int64_t& seq_before) {
+    const int per = (tr.n_seq + 127) / 128, tid = threadIdx.x;
+    int64_t b = before;
+    for (int s = tid * per; s < min(tr.n_seq, (tid + 1) * per) && b <= at; ++s) {
+        const int64_t u = seq_units(seq_of(c, tr, s, G, MR, unit), c.n_kv_heads);
+        if (at < b + u) {
+            buf.s = s;
+            buf.before = b;
+        }
+        b += u;
+    }
+    __syncthreads();
+    seq_before = buf.before;
+    return buf.s;
+}
+// The cut of `total` units over the C CTAs that have work: the first `more` hold
+// `each` + 1 units, the others `each`.
+struct Cut {
+    int C, more;
+    int64_t each;
+    __device__ Cut(int64_t total, int ctas) {
+        C = (int)min((int64_t)ctas, total);
+        // 32-bit division where it does (the usual case): a 64-bit one takes a microsecond
+        each = total < 0x7fffffff ? (int64_t)((uint32_t)total / (uint32_t)max(C, 1)) : total / max(C, 1);
+        more = (int)(total - each * C);
+    }
+    __device__ int64_t first(int i) const { return each * i + min(i, more); }
+    __device__ int owner(int64_t x) const {
+        const int64_t big = (each + 1) * more;
+        if (x < big) return (int)(x < 0x7fffffff ? (uint32_t)x / (uint32_t)(each + 1) : x / (each + 1));
+        x -= big;
+        return more + (int)(x < 0x7fffffff ? (uint32_t)x / (uint32_t)each : x / each);
+    }
+};
+
+__device__ __forceinline__ uint32_t su32(const void* p) {
+    return (uint32_t)__cvta_generic_to_shared(p);
+}
+// 16 bytes global -> shared; 0 bytes read and zeros written where !ok.
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Two values as f16 pairs: x = hi + lo
+__device__ __forceinline__ void split_f16(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x0, x1);
+    const float2 b = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x0 - b.x, x1 - b.y);
+    hi = *(const uint32_t*)&h;
+    lo = *(const uint32_t*)&l;
+}
+// Two of the four int8 of w as exact f16: the byte with its sign bit turned is
+// u = x + 128; 0x6400 | u is the f16 1024 + u; minus 1152 leaves x.
+template <int SEL>
+__device__ __forceinline__ uint32_t i8_f16(uint32_t w) {
+    const uint32_t p = __byte_perm(w ^ 0x80808080u, 0x64646464u, SEL);
+    const __half2 h = __hsub2(*(const __half2*)&p, __floats2half2_rn(1152.f, 1152.f));
+    return *(const uint32_t*)&h;
+}
+
+// attn_tree_tc.cu: rows in tiles of TC_ROWS, units of TC_UNIT tokens, SMS CTAs; two
+// partials of TC_ROWS x (head_dim + 2) floats for each in ws.
+constexpr int TC_ROWS = 128, TC_UNIT = 128;
+int attend_tc(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq, float* out, int ld_out,
+              const float* q, int ld_q, float scale, float* ws, cudaStream_t st);
+
+}  // namespace sb_tree
+
+#endif
