@@ -68,9 +68,10 @@ __device__ __forceinline__ void bar_arrive(uint64_t* b) {
 }
 __device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity) {
     uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+    // the thread may sleep up to 2 us in the instruction: a spin would take the softmax's issue slots
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
                  "selp.u32 %0, 1, 0, p;\n\t}\n"
-                 : "=r"(ok) : "r"(su32(b)), "r"(parity) : "memory");
+                 : "=r"(ok) : "r"(su32(b)), "r"(parity), "r"(2000) : "memory");
     return ok != 0;
 }
 // Bounded: false, and the CTA's fail word set, after WAIT_NS or once another warp failed.
@@ -150,7 +151,8 @@ __device__ __forceinline__ uint32_t op_at(int r, int ch) {
     return (uint32_t)((ch >> 3) * 16384 + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
 }
 
-// The CTA's segments: each a run of tiles of one item.
+// The CTA's segments: each a run of tiles of one item.  In shared memory, advanced by one
+// thread: the roles have no registers to spare for it.
 struct Segs {
     int64_t at, stop, seq_before;
     int s, seg;
@@ -193,6 +195,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
     unsigned char* skv = sq + 2 * S::QB;                        // [K0, K1, V0, V1]
     float* ssc = (float*)(skv + 4 * S::TB);                      // [SCB][K, V][KT]
     __shared__ Bars bars;
+    __shared__ Segs sg;
+    __shared__ int more_s;
     __shared__ PlanBuf buf;
     __shared__ uint32_t tmem_s;
     __shared__ __align__(8) uint8_t gone_s[SCB][8];                // per page: the table has none
@@ -207,10 +211,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
     const int64_t total = plan_total(c, tr, G, MR, KT, buf, before);
     const Cut cut(total, gridDim.x);
     if ((int)blockIdx.x >= cut.C) return;
-    Segs sg;
-    sg.at = cut.first(blockIdx.x);
-    sg.stop = cut.first(blockIdx.x + 1);
-    sg.seg = -1;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             bar_init(&bars.kfull[i], 8);          // pages
@@ -222,6 +222,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
             bar_init(&bars.dfull[i], 1);
         }
         fail_s = 0;
+        sg.at = cut.first(blockIdx.x);
+        sg.stop = cut.first(blockIdx.x + 1);
+        sg.seg = -1;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 15) {
@@ -229,23 +232,36 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         tc_before();
     }
-    sg.s = plan_find(c, tr, G, MR, KT, buf, before, sg.at, sg.seq_before);     // a barrier
+    int64_t seq_before;
+    const int s0 = plan_find(c, tr, G, MR, KT, buf, before, cut.first(blockIdx.x), seq_before);     // a barrier
     tc_after();
     const uint32_t tmem = tmem_s;
-    sg.sq = seq_of(c, tr, sg.s, G, MR, KT);
+    if (tid == 0) {
+        sg.s = s0;
+        sg.seq_before = seq_before;
+        sg.sq = seq_of(c, tr, s0, G, MR, KT);
+    }
+    // Every role walks the same segments; four barriers of the CTA a segment: the last one has
+    // left the buffers, the next is known, q is there, every product is done and the half rows'
+    // sums are there.
+    const auto next_segment = [&]() {
+        __syncthreads();
+        if (tid == 0) more_s = sg.next(c, tr, G);
+        __syncthreads();
+        return more_s != 0;
+    };
     const auto sS = [&](int b) { return tmem + 128u * b; };
     const auto sD = [&](int b) { return tmem + 256u + 128u * b; };
     uint32_t nuse[2] = {0, 0};                  // tiles done in each buffer by this role: barrier phases
     volatile int* fail = &fail_s;
 
-    // Every role walks the same segments; three barriers of the CTA a segment: its buffers
-    // are free, q is there, every product is done and the half rows' sums are there.
     if (warp < 8) {
-        while (sg.next(c, tr, G)) {
+        // no spills: with 227 KB of shared memory the first-level cache is too small to hold them
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+        while (next_segment()) {
             const Seq& sq_ = sg.sq;
             const int nt = sg.nt, kvh = sg.kvh, r_base = sg.r_base, n_rows = sg.n_rows, tok0 = sg.tok0;
         // ---- q, each row divided by the power of two below its maximum; scale's sign joins q
-            __syncthreads();                           // the last segment has left the buffers
         for (int r = warp; r < MR; r += 8) {
             const int row = r_base + r;
             const bool live = r < n_rows;
@@ -385,19 +401,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                         uint32_t x[16], pk[16];                        // pk: hi of 8 pairs, then lo
                         tmem_ld(sp + 16 * cc, x);
                         const uint32_t v = all.value ? 0xffffffffu : seen(16 * cc & ~31) >> (16 * cc & 31);
-                        float4 k4[4], v4[4];
-                        if (Q8)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                k4[i] = *(const float4*)(ks + 16 * cc + 4 * i);
-                                v4[i] = *(const float4*)(vs + 16 * cc + 4 * i);
-                            }
                         tmem_ld_wait();
 #pragma unroll
                         for (int i = 0; i < 16; i += 2) {
                             float2 y = make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-                            const float4 kk = k4[i / 4], vv = v4[i / 4];
-                            if (Q8) y = __fmul2_rn(y, i & 2 ? make_float2(kk.z, kk.w) : make_float2(kk.x, kk.y));
+                            if (Q8) y = __fmul2_rn(y, *(const float2*)(ks + 16 * cc + i));
                             y = __ffma2_rn(y, rs2, nb2);
                             float2 p = make_float2(ex2(y.x), ex2(y.y));
                             if (!all.value) {
@@ -406,7 +414,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                             }
                             sum = __fadd2_rn(sum, p);
                             if (Q8) {
-                                p = __fmul2_rn(p, i & 2 ? make_float2(vv.z, vv.w) : make_float2(vv.x, vv.y));
+                                p = __fmul2_rn(p, *(const float2*)(vs + 16 * cc + i));
                                 if (!all.value) {                      // 0 stays 0 whatever the scale
                                     if (!(v >> i & 1)) p.x = 0.f;
                                     if (!(v >> (i + 1) & 1)) p.y = 0.f;
@@ -478,13 +486,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
             }
             if (*fail) break;
         }
-    } else if (warp == 15) {
+    } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (warp == 15) {
         // ================= products: f32 accumulate, M = 128, N = 128 (scores) or HD (p v);
         // V is MN-major (bit 16)
         constexpr uint32_t idq = 1u << 4 | (uint32_t)(KT >> 3) << 17 | (uint32_t)(MR >> 4) << 24;
         constexpr uint32_t idv = 1u << 4 | 1u << 16 | (uint32_t)(HD >> 3) << 17 | (uint32_t)(MR >> 4) << 24;
-        while (sg.next(c, tr, G)) {
-            __syncthreads();
+        while (next_segment()) {
             __syncthreads();
             if (lane == 0) {
                 bool ok = true;
@@ -533,15 +542,19 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
         // warp 8 + w takes jobs w, w + 7, ...
         const int w = warp - 8;
         uint32_t used[2] = {0, 0};                     // tiles before this segment, in each buffer
-        while (sg.next(c, tr, G)) {
+        while (next_segment()) {
             const int nt = sg.nt, kvh = sg.kvh, tok0 = sg.tok0, end = sg.end, ctx = sg.sq.ctx, slot = sg.sq.slot;
-            __syncthreads();
             __syncthreads();
             bool ok = true;
             const int njobs = 16 * nt;
+            const size_t kv_step = (size_t)nkv * sb_kv_block_bytes(KV, HD), page_step = 2 * kv_step;
+            const unsigned char* pool = sb_kv_block(c, layer, 0, 0, kvh);
+            const int32_t* pages = c.page_table + (size_t)max(slot, 0) * c.max_pages;
+            const int n_pages = (int)c.n_pages, last = slot >= 0 && slot < c.n_slots ? min(c.max_pages, (end + 15) / 16) : 0;
             const auto page_of = [&](int n) {
-                const int t = tok0 + (n >> 4) * KT + 16 * (n & 7);
-                return n < njobs && t < end ? sb_kv_page(c, slot, t) : -1;
+                const int i = (tok0 + (n >> 4) * KT) / 16 + (n & 7);
+                const int p = n < njobs && i < last ? __ldg(pages + i) : -1;
+                return p < n_pages ? p : -1;
             };
             // the operand buffer is free once the product two tiles back has read it
             const auto wait_free = [&](int n) {
@@ -556,16 +569,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                 if (lane == 0) bar_arrive(n & 8 ? &bars.vfull[(n >> 4) & 1] : &bars.kfull[(n >> 4) & 1]);
             };
             if constexpr (Q8) {
-                // 16 dims lane % U of every (32 / U)-th token, widened to two chunks; the second 64
-                // dims write theirs in the other order, so that a bank is met once
+                // Lane: 16 dims k of token t (and every TS-th after it), widened to chunks 2 k and 2 k + 1.
+                // Eight lanes in turn hold four k of two tokens: their chunks differ by the tokens' low
+                // bit, so that a store meets no bank twice.
                 constexpr int U = HD / 16, TS = 32 / U, NP = 16 / TS;
-                const bool sw = HD > 64 && lane % U >= 4;
-                uint32_t to[2][2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    to[i][0] = op_at(lane / U + TS * i, 2 * (lane % U) + (sw ? 1 : 0)) - TS * i * 128;
-                    to[i][1] = op_at(lane / U + TS * i, 2 * (lane % U) + (sw ? 0 : 1)) - TS * i * 128;
-                }
+                const int lt = lane / 4 % TS, lk = lane % 4 + 4 * (lane / 4 / TS);
+                const uint32_t to[2] = {op_at(lt, 2 * lk), op_at(lt + TS, 2 * lk) - TS * 128};
                 struct Raw {
                     uint4 x[NP];
                     float4 ks, vs;                     // K jobs, lanes 0-3: both scales of 4 tokens
@@ -574,14 +583,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                 const auto fetch = [&](Raw& r, int n) {
                     const int page = r.page = page_of(n);
                     r.ks = r.vs = make_float4(0.f, 0.f, 0.f, 0.f);
-                    const unsigned char* blk = sb_kv_block(c, layer, max(page, 0), (n >> 3) & 1, kvh);
+                    const unsigned char* blk = pool + max(page, 0) * page_step + ((n & 8) ? kv_step : 0);
 #pragma unroll
                     for (int i = 0; i < NP; ++i)
                         r.x[i] = page < 0 ? make_uint4(0, 0, 0, 0)
-                                          : __ldg((const uint4*)(blk + SB_Q8_SCALES) + 32 * i + lane);
+                                          : __ldg((const uint4*)(blk + SB_Q8_SCALES) + (lt + TS * i) * U + lk);
                     if (page >= 0 && !(n & 8) && lane < 4) {
                         r.ks = __ldg((const float4*)blk + lane);
-                        r.vs = __ldg((const float4*)(blk + (size_t)nkv * sb_kv_block_bytes(KV, HD)) + lane);
+                        r.vs = __ldg((const float4*)(blk + kv_step) + lane);
                     }
                 };
                 const auto put = [&](const Raw& r, int n) {
@@ -594,8 +603,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                         const uint4 v = r.x[i];
                         const uint4 a = make_uint4(i8_f16<0x4140>(v.x), i8_f16<0x4342>(v.x), i8_f16<0x4140>(v.y), i8_f16<0x4342>(v.y));
                         const uint4 z = make_uint4(i8_f16<0x4140>(v.z), i8_f16<0x4342>(v.z), i8_f16<0x4140>(v.w), i8_f16<0x4342>(v.w));
-                        *(uint4*)(dst + to[i & 1][0] + TS * i * 128) = sw ? z : a;
-                        *(uint4*)(dst + to[i & 1][1] + TS * i * 128) = sw ? a : z;
+                        *(uint4*)(dst + to[i & 1] + TS * i * 128) = a;
+                        *(uint4*)(dst + (to[i & 1] ^ 16) + TS * i * 128) = z;
                     }
                     if (!(n & 8)) {                    // before kfull: the softmax reads them after the scores
                         float vm = 0.f;
@@ -665,7 +674,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                     wait_free(n);
                     if (!ok) break;
                     const uint32_t dst = su32(skv) + (((n & 8) ? 2 : 0) + (j & 1)) * S::TB + pg * 2048;
-                    const unsigned char* src = sb_kv_block(c, layer, max(page, 0), (n >> 3) & 1, kvh) + 16 * lane;
+                    const unsigned char* src = pool + max(page, 0) * page_step + ((n & 8) ? kv_step : 0) + 16 * lane;
 #pragma unroll
                     for (int i = 0; i < NP; ++i)
                         cp16(dst + op_at(lane / CPT + TS * i, lane % CPT), src + 512 * i,
@@ -694,12 +703,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
             if (*fail) break;
         }
     }
+    }
     __syncthreads();
     if (*fail) {
         // products and copies in flight end before the CTA does; then, what this CTA owed and
         // did not do: NaN, whole or in part
         for (const uint64_t t0 = gtimer(); gtimer() - t0 < WAIT_NS / 100;) {}
-        while (sg.next(c, tr, G)) {
+        while (next_segment()) {
             for (int e = tid; e < sg.n_rows * (HD + 2); e += NTHREADS) {
                 const int r = e / (HD + 2), d = e % (HD + 2), row = sg.r_base + r;
                 if (!sg.whole) ws[((size_t)(2 * blockIdx.x + 1) * MR + r) * (HD + 2) + d] = NAN;

@@ -133,7 +133,8 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ void split_f16(float x0, float x1, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __floats2half2_rn(x0, x1);
     const float2 b = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x0 - b.x, x1 - b.y);
+    const float2 r = __fadd2_rn(make_float2(x0, x1), make_float2(-b.x, -b.y));
+    const __half2 l = __floats2half2_rn(r.x, r.y);
     hi = *(const uint32_t*)&h;
     lo = *(const uint32_t*)&l;
 }
