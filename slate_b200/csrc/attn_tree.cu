@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(32 * NW) attn_tree_rows(
 #ifndef SB_T0
 #define SB_T0 3
 #endif
-constexpr int MAXC = 4 * SMS;               // CTAs at most (join)
+constexpr int MAXC = 4 * SMS;               // CTAs at most
 constexpr int UNIT = 64;
 static_assert(MAXC * 32 <= SMS * TC_ROWS, "workspace");
 constexpr int MW = 4;                       // warps a CTA
@@ -728,18 +728,18 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
     }
 }
 
-// Joins the partials of the cut items: one CTA of 128 threads a (sequence, kv head,
-// row).  The records' weights are formed once, then each thread sums its dim over the
-// records (head_dim 64: two halves of the records), several loads in flight.
+// Joins the partials of the cut items: one CTA a (sequence, kv head, `rpc` rows), a warp a
+// row: lane i forms the weight of record i, then the lanes sum their dims over the records,
+// eight loads in flight.
 template <int HD>
 __global__ void __launch_bounds__(128) attn_tree_join(const slate_kv_cache_t c, const slate_tree_t tr,
-                                                      int nq, int MR, int unit, int ctas, float* __restrict__ out,
-                                                      int ld_out, const float* __restrict__ ws) {
-    constexpr int HALVES = 128 / HD;
+                                                      int nq, int MR, int unit, int ctas, int rpc,
+                                                      float* __restrict__ out, int ld_out,
+                                                      const float* __restrict__ ws) {
+    constexpr int E = HD / 32;                           // dims a lane: 2 or 4
     __shared__ PlanBuf buf;
-    __shared__ float wt[MAXC], top[4], so[HALVES - 1 ? 128 : 1], sl[4];
-    const int nkv = c.n_kv_heads, G = nq / nkv, tid = threadIdx.x;
-    const int R = tr.max_nodes * G, s = blockIdx.x / R, row = blockIdx.x % R, kvh = blockIdx.y;
+    const int nkv = c.n_kv_heads, G = nq / nkv, tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+    const int chunks = (tr.max_nodes * G + rpc - 1) / rpc, s = blockIdx.x / chunks, kvh = blockIdx.y;
     int64_t before;
     const int64_t total = plan_total(c, tr, G, MR, unit, buf, before);
     const Seq q = seq_of(c, tr, s, G, MR, unit);
@@ -749,52 +749,54 @@ __global__ void __launch_bounds__(128) attn_tree_join(const slate_kv_cache_t c, 
         buf.before = before;
     }
     __syncthreads();
-    sb_grid_wait();        // the partials; before any return, so that the chain stays ordered
-    if (row >= q.n * G) return;
     const Cut cut(total, ctas);
-    const int64_t first = buf.before + (int64_t)(kvh * q.tiles + row / MR) * q.units;
-    const int c0 = cut.owner(first), n = cut.owner(first + q.units - 1) - c0 + 1;
-    if (n == 1) return;                                  // written by its CTA
-    // an item that begins inside its first CTA's range is that CTA's later segment
-    const size_t rec = (size_t)MR * (HD + 2);
-    const float* base = ws + (size_t)2 * c0 * rec + (size_t)(row % MR) * (HD + 2);
-    const auto at = [&](int i) { return base + (size_t)2 * i * rec + (i == 0 && cut.first(c0) < first ? rec : 0); };
-    float M = -INFINITY;
-    for (int i = tid; i < n; i += 128) M = fmaxf(M, wt[i] = at(i)[0]);
-    for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(FULL, M, x));
-    if ((tid & 31) == 0) top[tid / 32] = M;
-    __syncthreads();
-    M = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-    float L = 0.f;
-    for (int i = tid; i < n; i += 128) {
-        const float f = wt[i] == -INFINITY ? 1.f : ex2(wt[i] - M);
-        wt[i] = f;
-        L = fmaf(at(i)[1], f, L);
-    }
-    for (int x = 16; x; x >>= 1) L += __shfl_xor_sync(FULL, L, x);
-    if ((tid & 31) == 0) sl[tid / 32] = L;
-    __syncthreads();
-    L = sl[0] + sl[1] + sl[2] + sl[3];
-    const int d = tid % HD;
-    float O = 0.f;
+    sb_grid_wait();        // the partials; before any return, so that the chain stays ordered
+    const int row0 = blockIdx.x % chunks * rpc;
+    for (int row = row0 + warp; row < min(row0 + rpc, q.n * G); row += 4) {
+        const int64_t first = buf.before + (int64_t)(kvh * q.tiles + row / MR) * q.units;
+        const int c0 = cut.owner(first), n = cut.owner(first + q.units - 1) - c0 + 1;
+        if (n == 1) continue;                            // written by its CTA
+        // an item that begins inside its first CTA's range is that CTA's later segment
+        const size_t rec = (size_t)MR * (HD + 2);
+        const float* base = ws + (size_t)2 * c0 * rec + (size_t)(row % MR) * (HD + 2);
+        const size_t late = cut.first(c0) < first ? rec : 0;
+        float M = -INFINITY, L = 0.f, O[E];
+        for (int i = lane; i < n; i += 32) M = fmaxf(M, base[2 * i * rec + (i ? 0 : late)]);
+        for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(FULL, M, x));
+#pragma unroll
+        for (int k = 0; k < E; ++k) O[k] = 0.f;
+        for (int i0 = 0; i0 < n; i0 += 32) {
+            float f = 0.f;
+            if (i0 + lane < n) {
+                const float2 ml = *(const float2*)(base + 2 * (i0 + lane) * rec + (i0 + lane ? 0 : late));
+                f = ml.x == -INFINITY ? 1.f : ex2(ml.x - M);
+                L = fmaf(ml.y, f, L);
+            }
 #pragma unroll 8
-    for (int i = tid / HD; i < n; i += HALVES) O = fmaf(at(i)[2 + d], wt[i], O);
-    if (HALVES > 1) {
-        if (tid >= HD) so[tid] = O;
-        __syncthreads();
-        if (tid >= HD) return;
-        O += so[tid + HD];
+            for (int i = 0; i < min(n - i0, 32); ++i) {
+                const float w = __shfl_sync(FULL, f, i);
+                const float* o = base + 2 * (i0 + i) * rec + (i0 + i ? 0 : late) + 2 + E * lane;
+#pragma unroll
+                for (int k = 0; k < E; k += 2) {
+                    const float2 y = *(const float2*)(o + k);
+                    O[k] = fmaf(y.x, w, O[k]);
+                    O[k + 1] = fmaf(y.y, w, O[k + 1]);
+                }
+            }
+        }
+        for (int x = 16; x; x >>= 1) L += __shfl_xor_sync(FULL, L, x);
+        float* o = out + (size_t)(q.r0 + row / G) * ld_out + (size_t)(kvh * G + row % G) * HD + E * lane;
+#pragma unroll
+        for (int k = 0; k < E; ++k) o[k] = L == 0.f ? 0.f : O[k] / L;
     }
-    out[(size_t)(q.r0 + row / G) * ld_out + (size_t)(kvh * G + row % G) * HD + d] = L == 0.f ? 0.f : O / L;
 }
-
-
 
 template <int HD>
 int join(const slate_kv_cache_t& c, const slate_tree_t& tr, int nq, int MR, int unit, int ctas, float* out, int ld_out,
          const float* ws, cudaStream_t st) {
-    const dim3 grid((unsigned)(tr.n_seq * tr.max_nodes * (nq / c.n_kv_heads)), (unsigned)c.n_kv_heads);
-    return sb_cuda_check(sb_launch_pdl(attn_tree_join<HD>, grid, dim3(128), 0, st, c, tr, nq, MR, unit, ctas, out, ld_out, ws),
+    const int R = tr.max_nodes * (nq / c.n_kv_heads), rpc = R >= 128 ? 16 : 4;
+    const dim3 grid((unsigned)(tr.n_seq * ((R + rpc - 1) / rpc)), (unsigned)c.n_kv_heads);
+    return sb_cuda_check(sb_launch_pdl(attn_tree_join<HD>, grid, dim3(128), 0, st, c, tr, nq, MR, unit, ctas, rpc, out, ld_out, ws),
                          "attention_tree join");
 }
 template <int KV, int HD, int MODE>
