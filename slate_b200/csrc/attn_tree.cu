@@ -132,9 +132,6 @@ __global__ void __launch_bounds__(32 * NW) attn_tree_rows(
 }
 
 // ------------------------------------------------------------ tensor-core path
-#ifndef SB_TC_MIN
-#define SB_TC_MIN 32
-#endif
 #ifndef SB_T0
 #define SB_T0 3
 #endif
@@ -217,17 +214,16 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
     float* rowscale = (float*)(smem + S::QB + S::RING);        // [MR]
     uint64_t* rowmask = (uint64_t*)(rowscale + 2 * ((MR + 1) / 2));   // [MR]
     __shared__ PlanBuf buf;
+    sb_grid_wait();
     sb_grid_release();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     const int nkv = c.n_kv_heads, G = nq / nkv;
-    int64_t before, seq_before;
-    const int64_t total = plan_total(c, tr, G, MR, UNIT, buf, before);
-    const Cut cut(total, gridDim.x);
-    if ((int)blockIdx.x >= cut.C) return;
-    int64_t at = cut.first(blockIdx.x);
-    const int64_t stop = cut.first(blockIdx.x + 1);
-    int s = plan_find(c, tr, G, MR, UNIT, buf, before, at, seq_before);
-    Seq sq_ = seq_of(c, tr, s, G, MR, UNIT);
+    Start st_;
+    if (!plan_start(c, tr, G, MR, UNIT, gridDim.x, buf, st_)) return;
+    int64_t at = st_.at, seq_before = st_.seq_before;
+    const int64_t stop = st_.stop;
+    Seq sq_ = st_.sq;
+    int s = sq_.s;
     const size_t page_blk = sb_kv_block_bytes(KV, HD);
     unsigned char* myring = ring + (size_t)warp * NS * TB;
     const uint32_t myring_s = su32(myring);
@@ -247,26 +243,29 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
 
         // ---- q as A fragments, each row divided by the power of two below its maximum
         __syncthreads();                               // the last segment's merge is read
-        for (int r = warp; r < MR; r += MW) {
-            const int row = r_base + r, node = row / G;
-            const bool live = r < n_rows;
-            const float* x = q + (size_t)(sq_.r0 + (live ? node : 0)) * ld_q +
-                             (size_t)(kvh * G + (live ? row % G : 0)) * HD;
-            float v[HD / 32];
+        if (tid < MR) rowmask[tid] = tid < n_rows ? __ldg(tr.mask + sq_.r0 + (r_base + tid) / G) : 0;
+        float qv[MR / MW][HD / 32];                    // all of the warp's rows before any is used
+#pragma unroll
+        for (int k = 0; k < MR / MW; ++k) {
+            const int row = r_base + min(warp + k * MW, n_rows - 1);
+            const float* x = q + (size_t)(sq_.r0 + row / G) * ld_q + (size_t)(kvh * G + row % G) * HD + lane * (HD / 32);
+#pragma unroll
+            for (int i = 0; i < HD / 32; ++i) qv[k][i] = x[i];
+        }
+#pragma unroll
+        for (int k = 0; k < MR / MW; ++k) {
+            const int r = warp + k * MW;
+            float(&v)[HD / 32] = qv[k];
             uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < HD / 32; ++i) {
-                v[i] = live ? x[lane * (HD / 32) + i] : 0.f;
                 top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
             }
             top = __reduce_max_sync(FULL, top);
             // exponent of the maximum, kept where 2^-e and 2^e are normal numbers
             const int e = min(max((int)(top >> 23) - 127, -100), 100);
             const float inv = __int_as_float((127 - e) << 23);
-            if (lane == 0) {
-                rowscale[r] = scale * 1.4426950408889634f * __int_as_float((127 + e) << 23);
-                rowmask[r] = live ? __ldg(tr.mask + sq_.r0 + node) : 0;
-            }
+            if (lane == 0) rowscale[r] = scale * 1.4426950408889634f * __int_as_float((127 + e) << 23);
             // element d of row r in the fragments: rows r % 16 < 8 in registers 0 and 2
             const int mt = r / 16, rg = r & 7, up = MODE == 0 ? 0 : (r >> 3) & 1;
 #pragma unroll
@@ -740,20 +739,15 @@ __global__ void __launch_bounds__(128) attn_tree_join(const slate_kv_cache_t c, 
     __shared__ PlanBuf buf;
     const int nkv = c.n_kv_heads, G = nq / nkv, tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
     const int chunks = (tr.max_nodes * G + rpc - 1) / rpc, s = blockIdx.x / chunks, kvh = blockIdx.y;
+    // no early release: the next call's CTAs have to find the SMs empty, all of them at once
+    Seq q;
     int64_t before;
-    const int64_t total = plan_total(c, tr, G, MR, unit, buf, before);
-    const Seq q = seq_of(c, tr, s, G, MR, unit);
-    const int per = (tr.n_seq + 127) / 128;
-    if (tid == s / per) {          // units before this sequence, from the thread that counted them
-        for (int x = tid * per; x < s; ++x) before += seq_units(seq_of(c, tr, x, G, MR, unit), nkv);
-        buf.before = before;
-    }
-    __syncthreads();
+    const int64_t total = plan_of(c, tr, G, MR, unit, s, buf, q, before);
     const Cut cut(total, ctas);
     sb_grid_wait();        // the partials; before any return, so that the chain stays ordered
     const int row0 = blockIdx.x % chunks * rpc;
     for (int row = row0 + warp; row < min(row0 + rpc, q.n * G); row += 4) {
-        const int64_t first = buf.before + (int64_t)(kvh * q.tiles + row / MR) * q.units;
+        const int64_t first = before + (int64_t)(kvh * q.tiles + row / MR) * q.units;
         const int c0 = cut.owner(first), n = cut.owner(first + q.units - 1) - c0 + 1;
         if (n == 1) continue;                            // written by its CTA
         // an item that begins inside its first CTA's range is that CTA's later segment
@@ -807,15 +801,16 @@ int launch_mma(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int
     static const cudaError_t ready =
         cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (ready != cudaSuccess) return sb_cuda_check(ready, "attention_tree shared memory");
-    k<<<S::CPS * SMS, 32 * MW, S::SMEM, st>>>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws);
-    const int rc = sb_cuda_check(cudaGetLastError(), "attention_tree");
+    const int rc = sb_cuda_check(sb_launch_pdl(k, dim3(S::CPS * SMS), dim3(32 * MW), S::SMEM, st, c, layer, tr, nq, out, ld_out, q,
+                                               ld_q, scale, ws),
+                                 "attention_tree");
     return rc ? rc : join<HD>(c, tr, nq, S::MR, UNIT, S::CPS * SMS, out, ld_out, ws, st);
 }
 template <int KV, int HD>
 int launch_mode(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq, float* out,
                 int ld_out, const float* q, int ld_q, float scale, float* ws, cudaStream_t st) {
     const int M = tr.max_nodes * (nq / c.n_kv_heads);
-    if (KV != SLATE_KV_F32 && M > SB_TC_MIN) {
+    if (KV == SLATE_KV_F16 ? M > 16 : KV == SLATE_KV_Q8 && M > 32) {
         const int rc = attend_tc(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);
         return rc ? rc : join<HD>(c, tr, nq, TC_ROWS, TC_UNIT, SMS, out, ld_out, ws, st);
     }

@@ -137,6 +137,7 @@ __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void softmax_sync() {
+    __syncwarp();
     asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
 }
 // Byte of 16-byte chunk ch (8 f16) of row r in an operand of 128 rows: 64 columns a
@@ -197,13 +198,12 @@ __global__ void __launch_bounds__(TcShape<KV, HD>::NTHREADS, 1) attn_tree_tc(
     __shared__ __align__(16) float vmax_s[SCB][8];                 // per page: largest v scale
     __shared__ float part_max[2][PARTS][MR];      // [tile parity][part][row]
     __shared__ int fail_s;
+    sb_grid_wait();
     sb_grid_release();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int nkv = c.n_kv_heads, G = nq / nkv;
-    int64_t before;
-    const int64_t total = plan_total(c, tr, G, MR, KT, buf, before);
-    const Cut cut(total, gridDim.x);
-    if ((int)blockIdx.x >= cut.C) return;
+    Start st_;
+    if (!plan_start(c, tr, G, MR, KT, gridDim.x, buf, st_)) return;
     if (tid == 0) {
         for (int i = 0; i < NB; ++i) {
             bar_init(&bars.kfull[i], 8);          // pages
@@ -218,9 +218,12 @@ __global__ void __launch_bounds__(TcShape<KV, HD>::NTHREADS, 1) attn_tree_tc(
         bar_init(&bars.dfull, 1);
         bar_init(&bars.dfree, 32 * NSW);
         fail_s = 0;
-        sg.at = cut.first(blockIdx.x);
-        sg.stop = cut.first(blockIdx.x + 1);
+        sg.at = st_.at;
+        sg.stop = st_.stop;
         sg.seg = -1;
+        sg.s = st_.sq.s;
+        sg.seq_before = st_.seq_before;
+        sg.sq = st_.sq;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == NSW + NPW) {
@@ -228,15 +231,9 @@ __global__ void __launch_bounds__(TcShape<KV, HD>::NTHREADS, 1) attn_tree_tc(
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         tc_before();
     }
-    int64_t seq_before;
-    const int s0 = plan_find(c, tr, G, MR, KT, buf, before, cut.first(blockIdx.x), seq_before);     // a barrier
+    __syncthreads();
     tc_after();
     const uint32_t tmem = tmem_s;
-    if (tid == 0) {
-        sg.s = s0;
-        sg.seq_before = seq_before;
-        sg.sq = seq_of(c, tr, s0, G, MR, KT);
-    }
     // Every role walks the same segments; four barriers of the CTA a segment: the last one has
     // left the buffers, the next is known, q is there, every product is done and the quarter rows'
     // sums are there.
@@ -521,6 +518,7 @@ __global__ void __launch_bounds__(TcShape<KV, HD>::NTHREADS, 1) attn_tree_tc(
                     ok = ok && bar_wait(&bars.vfull[vb_], phaseN(t), fail) && bar_wait(&bars.pfull[b], phase2(t), fail) &&
                          (t == 0 || bar_wait(&bars.dfree, (t - 1) & 1, fail));
                     if (!ok) return;
+                    fence_async();
                     tc_after();
                     const uint32_t vb = su32(skv) + (NB + vb_) * S::TB;
 #pragma unroll
@@ -537,6 +535,10 @@ __global__ void __launch_bounds__(TcShape<KV, HD>::NTHREADS, 1) attn_tree_tc(
                     const int b = t & 1, kb_ = t % NB;
                     ok = bar_wait(&bars.kfull[kb_], phaseN(t), fail);
                     if (!ok) break;
+                    // K was written through the generic proxy and is read through the async one.  The
+                    // fence stands here, behind the barrier: in the producers it would wait for the loads
+                    // that they keep in flight.
+                    fence_async();
                     tc_after();
                     const uint32_t kb = su32(skv) + kb_ * S::TB;
 #pragma unroll
@@ -581,8 +583,7 @@ __global__ void __launch_bounds__(TcShape<KV, HD>::NTHREADS, 1) attn_tree_tc(
                 if (ok && t >= NB)
                     ok = __all_sync(FULL, bar_wait(n & 8 ? &bars.vfree[t % NB] : &bars.kfree[t % NB], phaseN(t - NB), fail));
             };
-            const auto arrive = [&](int n) {
-                fence_async();
+            const auto arrive = [&](int n) {           // the proxy fence is the product warp's
                 __syncwarp();
                 const uint32_t b = (tb + (n >> 4)) % NB;
                 if (lane == 0) bar_arrive(n & 8 ? &bars.vfull[b] : &bars.kfull[b]);
@@ -750,8 +751,9 @@ int launch(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq,
     static const cudaError_t ready =
         cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, TcShape<KV, HD>::SMEM);
     if (ready != cudaSuccess) return sb_cuda_check(ready, "attention_tree shared memory");
-    k<<<SMS, TcShape<KV, HD>::NTHREADS, TcShape<KV, HD>::SMEM, st>>>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws);
-    return sb_cuda_check(cudaGetLastError(), "attention_tree");
+    return sb_cuda_check(sb_launch_pdl(k, dim3(SMS), dim3(TcShape<KV, HD>::NTHREADS), TcShape<KV, HD>::SMEM, st, c, layer, tr, nq,
+                                       out, ld_out, q, ld_q, scale, ws),
+                         "attention_tree");
 }
 
 }  // namespace

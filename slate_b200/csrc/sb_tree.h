@@ -111,6 +111,86 @@ struct Cut {
     }
 };
 
+// Where a CTA begins: its units [at, stop), the sequence that holds `at`, the units before
+// that sequence.  False for a CTA without work.  Up to 32 sequences (the calls where the
+// microsecond counts) every warp finds it alone, a lane a sequence, without a barrier.
+struct Start {
+    int64_t at, stop, seq_before;
+    Seq sq;
+};
+__device__ __forceinline__ Seq seq_from(const Seq& q, int lane) {
+    Seq r;
+    r.s = lane;
+    r.r0 = __shfl_sync(FULL, q.r0, lane);
+    r.n = __shfl_sync(FULL, q.n, lane);
+    r.slot = __shfl_sync(FULL, q.slot, lane);
+    r.ctx = __shfl_sync(FULL, q.ctx, lane);
+    r.tiles = __shfl_sync(FULL, q.tiles, lane);
+    r.units = __shfl_sync(FULL, q.units, lane);
+    return r;
+}
+__device__ __forceinline__ int64_t plan_warp(const slate_kv_cache_t& c, const slate_tree_t& tr, int G, int MR,
+                                             int unit, Seq& q, int64_t& before) {
+    const int lane = threadIdx.x & 31;
+    q = seq_of(c, tr, min(lane, tr.n_seq - 1), G, MR, unit);
+    const int64_t mine = lane < tr.n_seq ? seq_units(q, c.n_kv_heads) : 0;
+    int64_t incl = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(FULL, incl, o);
+        if (lane >= o) incl += x;
+    }
+    before = incl - mine;
+    return __shfl_sync(FULL, incl, 31);
+}
+__device__ __forceinline__ bool plan_start(const slate_kv_cache_t& c, const slate_tree_t& tr, int G, int MR, int unit,
+                                           int ctas, PlanBuf& buf, Start& st) {
+    int64_t before;
+    if (tr.n_seq <= 32) {
+        Seq q;
+        const int64_t total = plan_warp(c, tr, G, MR, unit, q, before);
+        const Cut cut(total, ctas);
+        if ((int)blockIdx.x >= cut.C) return false;
+        st.at = cut.first(blockIdx.x);
+        st.stop = cut.first(blockIdx.x + 1);
+        // the last sequence that begins at or before `at` and has units
+        const unsigned hit = __ballot_sync(FULL, (int)(threadIdx.x & 31) < tr.n_seq && before <= st.at && seq_units(q, c.n_kv_heads) > 0);
+        const int s = 31 - __clz(hit);
+        st.seq_before = __shfl_sync(FULL, before, s);
+        st.sq = seq_from(q, s);
+        return true;
+    }
+    const int64_t total = plan_total(c, tr, G, MR, unit, buf, before);
+    const Cut cut(total, ctas);
+    if ((int)blockIdx.x >= cut.C) return false;
+    st.at = cut.first(blockIdx.x);
+    st.stop = cut.first(blockIdx.x + 1);
+    const int s = plan_find(c, tr, G, MR, unit, buf, before, st.at, st.seq_before);
+    st.sq = seq_of(c, tr, s, G, MR, unit);
+    return true;
+}
+// Sequence s, the units before it, and the total.
+__device__ __forceinline__ int64_t plan_of(const slate_kv_cache_t& c, const slate_tree_t& tr, int G, int MR, int unit,
+                                           int s, PlanBuf& buf, Seq& sq, int64_t& before) {
+    if (tr.n_seq <= 32) {
+        Seq q;
+        int64_t b;
+        const int64_t total = plan_warp(c, tr, G, MR, unit, q, b);
+        sq = seq_from(q, s);
+        before = __shfl_sync(FULL, b, s);
+        return total;
+    }
+    const int64_t total = plan_total(c, tr, G, MR, unit, buf, before);
+    const int per = (tr.n_seq + 127) / 128, tid = threadIdx.x;
+    if (tid == s / per) {          // from the thread that counted them
+        for (int x = tid * per; x < s; ++x) before += seq_units(seq_of(c, tr, x, G, MR, unit), c.n_kv_heads);
+        buf.before = before;
+    }
+    __syncthreads();
+    before = buf.before;
+    sq = seq_of(c, tr, s, G, MR, unit);
+    return total;
+}
+
 __device__ __forceinline__ uint32_t su32(const void* p) {
     return (uint32_t)__cvta_generic_to_shared(p);
 }
