@@ -133,12 +133,13 @@ __global__ void __launch_bounds__(32 * NW) attn_tree_rows(
 
 // ------------------------------------------------------------ tensor-core path
 #ifndef SB_T0
-#define SB_T0 3
+#define SB_T0 2
 #endif
 constexpr int MAXC = 4 * SMS;               // CTAs at most
 constexpr int UNIT = 64;
 static_assert(MAXC * 32 <= SMS * TC_ROWS, "workspace");
 constexpr int MW = 4;                       // warps a CTA
+constexpr float DIG = 127.f * 65536.f;      // three digits to base 256 stay within 8 bits each
 
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -152,6 +153,12 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
                  "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_i8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 "
+                 "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -177,8 +184,10 @@ struct Shape {
     static constexpr int TB = 2 * KT * RB + (KV == SLATE_KV_Q8 ? 8 * KT : 0);
     static constexpr int MT = MODE == 2 ? 2 : 1;
     static constexpr int MR = MODE == 0 ? 8 : 16 * MT;              // rows a tile
-    static constexpr int KS = KV == SLATE_KV_F32 ? HD / 8 : HD / 16;    // k steps of a score
-    static constexpr int HL = MODE == 0 ? 1 : 2;                    // A operands a k step
+    // 8 bits and up to 16 rows: scores from integer products, q in three 8-bit digits
+    static constexpr bool I8 = KV == SLATE_KV_Q8 && MODE < 2;
+    static constexpr int KS = I8 ? HD / 32 : KV == SLATE_KV_F32 ? HD / 8 : HD / 16;    // k steps of a score
+    static constexpr int HL = I8 ? MODE + 2 : MODE == 0 ? 1 : 2;    // A operands a k step
     static constexpr int QB = MT * KS * HL * 512;
     static constexpr int CPS = MODE == 0 ? SB_T0 : 2;                // CTAs an SM
     static constexpr int NS0 = ((CPS == 2 ? 112 : CPS == 3 ? 74 : 55) * 1024 - QB) / (MW * TB);
@@ -266,6 +275,32 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
             const int e = min(max((int)(top >> 23) - 127, -100), 100);
             const float inv = __int_as_float((127 - e) << 23);
             if (lane == 0) rowscale[r] = scale * 1.4426950408889634f * __int_as_float((127 + e) << 23);
+            if constexpr (S::I8) {
+                // q / 2^(e + 1) (below 1) times DIG as an integer of three digits to base 256, each in
+                // -128 .. 127.  Dims 32 ks + 16 hi + 4 t + b are byte b of register 2 hi (+ 1: row + 8)
+                // of lane (row % 8, t).  Up to 8 rows: operand 0 holds the top digit in its rows 0-7 and
+                // the middle one in rows 8-15, operand 1 the low digit; else an operand a digit.
+                const float f = inv * (0.5f * DIG);
+                if (lane == 0) rowscale[r] = top < 0x7f800000u ? rowscale[r] * (2.f / DIG) : NAN;
+#pragma unroll
+                for (int i = 0; i < HD / 32; ++i) {
+                    const int d = lane * (HD / 32) + i, v0 = __float2int_rn(v[i] * f);
+                    const int d0 = (int8_t)v0, v1 = (v0 - d0) >> 8, d1 = (int8_t)v1, d2 = (v1 - d1) >> 8;
+                    const int reg = (d >> 4 & 1) * 2, at = ((r & 7) * 4 + (d >> 2 & 3)) * 16 + (d & 3);
+                    int8_t* f8 = (int8_t*)(sq + (size_t)(d / 32) * S::HL * 32);
+                    if (MODE == 0) {
+                        f8[at + 4 * reg] = (int8_t)d2;
+                        f8[at + 4 * (reg + 1)] = (int8_t)d1;
+                        f8[512 + at + 4 * reg] = (int8_t)d0;
+                        f8[512 + at + 4 * (reg + 1)] = 0;
+                    } else {
+                        const int up8 = r >> 3 & 1;
+                        f8[at + 4 * (reg + up8)] = (int8_t)d2;
+                        f8[512 + at + 4 * (reg + up8)] = (int8_t)d1;
+                        f8[1024 + at + 4 * (reg + up8)] = (int8_t)d0;
+                    }
+                }
+            } else {
             // element d of row r in the fragments: rows r % 16 < 8 in registers 0 and 2
             const int mt = r / 16, rg = r & 7, up = MODE == 0 ? 0 : (r >> 3) & 1;
 #pragma unroll
@@ -291,6 +326,7 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
                     f[(MODE == 0 ? 2 * (reg + 1) : 32 * 8 + 2 * reg) + (d & 1)] = lo;
                 }
             }
+            }
         }
         __syncthreads();
 
@@ -311,18 +347,27 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
         const int tiles = (tok1 - tok0 + KT - 1) / KT;
         const int mine = warp < tiles ? (tiles - 1 - warp) / MW + 1 : 0;
         constexpr int PPT = KT > 16 ? KT / 16 : 1;     // pages a tile
-        int win[PPT];                                  // lane i: pages of the warp's tile (base + i)
+        // lane i: pages of the warp's tile (base + i), of these 32 tiles and the next
+        int win[PPT], nwin[PPT];
         uint32_t absent = 0;                           // bit (stage, page): the table has no such page
-        auto load_window = [&](int base) {
+        auto load_window = [&](int base, int (&w)[PPT]) {
 #pragma unroll
             for (int p = 0; p < PPT; ++p) {
                 const int t = tok0 + (warp + (base + lane) * MW) * KT + 16 * p;
-                win[p] = base + lane < mine && t < tok1 ? sb_kv_page(c, sq_.slot, t) : -1;
+                w[p] = base + lane < mine && t < tok1 ? sb_kv_page(c, sq_.slot, t) : -1;
             }
         };
+        load_window(0, win);
+        load_window(32, nwin);
+        const size_t kv_step = (size_t)nkv * page_blk, page_step = 2 * kv_step;
+        const unsigned char* pool = sb_kv_block(c, layer, 0, 0, kvh);
         auto issue = [&](int i) {                      // the warp's i-th tile into stage i % NS
             if (i < mine) {
-                if ((i & 31) == 0) load_window(i);
+                if (i > 0 && (i & 31) == 0) {
+#pragma unroll
+                    for (int p = 0; p < PPT; ++p) win[p] = nwin[p];
+                    load_window(i + 32, nwin);
+                }
                 const int t0 = tok0 + (warp + i * MW) * KT;
                 const uint32_t st = myring_s + (i % NS) * TB;
 #pragma unroll
@@ -330,8 +375,8 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
                     const int page = __shfl_sync(FULL, win[p], i & 31);
                     const uint32_t bit = 1u << ((i % NS) * PPT + p);
                     absent = page < 0 ? absent | bit : absent & ~bit;
-                    const unsigned char* kb = sb_kv_block(c, layer, max(page, 0), 0, kvh);
-                    const unsigned char* vb = kb + (size_t)nkv * page_blk;
+                    const unsigned char* kb = pool + max(page, 0) * page_step;
+                    const unsigned char* vb = kb + kv_step;
                     constexpr int ROWS = KT < 16 ? KT : 16, HEAD = KV == SLATE_KV_Q8 ? SB_Q8_SCALES : 0;
                     const int rsrc = KT < 16 ? t0 & 15 : 0;
 #pragma unroll
@@ -397,6 +442,44 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
                             }
                     }
                 }
+            } else if constexpr (S::I8) {
+                // exact: |sum| <= 128 * 127 * 128 < 2^21.  The sums start at the bits of 1.5 * 2^23, so that
+                // the result read as a float is 1.5 * 2^23 + sum
+                constexpr float BIAS = 12582912.f;
+                int acc[S::HL][NTK][4];
+#pragma unroll
+                for (int h = 0; h < S::HL; ++h)
+#pragma unroll
+                    for (int j = 0; j < NTK; ++j)
+                        acc[h][j][0] = acc[h][j][1] = acc[h][j][2] = acc[h][j][3] = 0x4b400000;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    uint32_t A[S::HL][4];
+#pragma unroll
+                    for (int h = 0; h < S::HL; ++h) {
+                        const uint4 x = sq[(k * S::HL + h) * 32 + lane];
+                        A[h][0] = x.x, A[h][1] = x.y, A[h][2] = x.z, A[h][3] = x.w;
+                    }
+#pragma unroll
+                    for (int jp = 0; jp < NTK / 2; ++jp) {
+                        uint32_t r[4];
+                        ldsm4(ks_ + swz<KV, RB>(16 * jp + (lane >> 4) * 8 + (lane & 7), 2 * k + ((lane >> 3) & 1)), r);
+#pragma unroll
+                        for (int h = 0; h < S::HL; ++h) {
+                            mma_i8(acc[h][2 * jp], A[h], r[0], r[1]);
+                            mma_i8(acc[h][2 * jp + 1], A[h], r[2], r[3]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < NTK; ++j)
+#pragma unroll
+                    for (int e = 0; e < (MODE == 0 ? 2 : 4); ++e) {
+                        const float d2 = __int_as_float(acc[0][j][e]) - BIAS;
+                        const float d1 = __int_as_float(acc[MODE == 0 ? 0 : 1][j][MODE == 0 ? 2 + e : e]) - BIAS;
+                        const float d0 = __int_as_float(acc[S::HL - 1][j][e]) - BIAS;
+                        sc[0][j][e] = fmaf(fmaf(d2, 256.f, d1), 256.f, d0);
+                    }
             } else {
                 // an ldmatrix.x4 brings two 8-token tiles: f16 of one k step, 8 bits of two
                 constexpr int KPL = KV == SLATE_KV_Q8 ? 2 : 1;
@@ -439,7 +522,13 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
 #pragma unroll
             for (int j = 0; j < NTK; ++j)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) kf[j][e] = KV == SLATE_KV_Q8 ? ksc[8 * j + 2 * t4 + e] : 1.f;
+                for (int e = 0; e < 2; ++e) kf[j][e] = 1.f;
+            if (KV == SLATE_KV_Q8)
+#pragma unroll
+                for (int j = 0; j < NTK; ++j) {
+                    const float2 x = *(const float2*)(ksc + 8 * j + 2 * t4);
+                    kf[j][0] = x.x, kf[j][1] = x.y;
+                }
             float corr[RI];
 #pragma unroll
             for (int ri = 0; ri < RI; ++ri) {
@@ -448,7 +537,9 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
                 for (int j = 0; j < NTK; ++j)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float d = MODE == 0 ? sc[0][j][e] + sc[0][j][2 + e] : sc[ri >> 1][j][2 * (ri & 1) + e];
+                        const float d = S::I8 && MODE == 0 ? sc[0][j][e]
+                                        : MODE == 0    ? sc[0][j][e] + sc[0][j][2 + e]
+                                                       : sc[ri >> 1][j][2 * (ri & 1) + e];
                         p[ri][j][e] = d * (KV == SLATE_KV_Q8 ? rs[ri] * kf[j][e] : rs[ri]);
                     }
                 if (tail) {
@@ -481,17 +572,15 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
             // ---- weights of v: 8 bits: p vscale / vref (vref: a power of two not below any
             // vscale met), so that they keep f16's range; 0 stays 0 whatever the scale
             if (KV == SLATE_KV_Q8) {
-                float vf[NTK][2], vm = 0.f;
+                float vf[NTK][2];
 #pragma unroll
-                for (int j = 0; j < NTK; ++j)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int t = 8 * j + 2 * t4 + e;
-                        vf[j][e] = vsc[t];
-                        if (t0 + t < end && vf[j][e] < INFINITY) vm = fmaxf(vm, vf[j][e]);
-                    }
-                vm = fmaxf(vm, __shfl_xor_sync(FULL, vm, 1));
-                vm = fmaxf(vm, __shfl_xor_sync(FULL, vm, 2));
+                for (int j = 0; j < NTK; ++j) {
+                    const float2 x = *(const float2*)(vsc + 8 * j + 2 * t4);
+                    vf[j][0] = x.x, vf[j][1] = x.y;
+                }
+                // the tile's largest: lane = token, as bits
+                const float v1 = vsc[lane];
+                const float vm = __uint_as_float(__reduce_max_sync(FULL, t0 + lane < end && v1 > 0.f && v1 < INFINITY ? __float_as_uint(v1) : 0u));
                 if (i == 0 || vm > vref) {
                     const int e = min(max((int)(__float_as_uint(vm) >> 23) - 126, -80), 126);
                     const float nref = __int_as_float((127 + e) << 23), f = i ? vref / nref : 0.f;
@@ -506,7 +595,8 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
                     for (int e = 0; e < 2; ++e) {
                         const float f = vf[j][e] * vi;
 #pragma unroll
-                        for (int ri = 0; ri < RI; ++ri) p[ri][j][e] = p[ri][j][e] == 0.f ? 0.f : p[ri][j][e] * f;
+                        for (int ri = 0; ri < RI; ++ri)
+                            p[ri][j][e] = tail && p[ri][j][e] == 0.f ? 0.f : p[ri][j][e] * f;
                     }
             }
             // An infinity or NaN in a v that only some rows see would reach the others as
@@ -573,7 +663,8 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
                             o[a][jd][e] = fmaf(o[a][jd][e], corr[MODE == 0 ? 0 : (2 * a + (e >> 1)) % RI], d[a][e]);
                 }
             } else {
-                uint32_t P[MT][NTK / 2][S::HL][4];
+                constexpr int PH = MODE == 0 ? 1 : 2;
+                uint32_t P[MT][NTK / 2][PH][4];
 #pragma unroll
                 for (int a = 0; a < MT; ++a)
 #pragma unroll
@@ -586,9 +677,9 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
                                 split_f16(p[0][j][0] * f, p[0][j][1] * f, P[a][k][0][2 * h], P[a][k][0][2 * h + 1]);
                             } else {
                                 split_f16(p[(2 * a) % RI][j][0] * f, p[(2 * a) % RI][j][1] * f, P[a][k][0][2 * h],
-                                          P[a][k][S::HL - 1][2 * h]);
+                                          P[a][k][PH - 1][2 * h]);
                                 split_f16(p[(2 * a + 1) % RI][j][0] * f, p[(2 * a + 1) % RI][j][1] * f,
-                                          P[a][k][0][2 * h + 1], P[a][k][S::HL - 1][2 * h + 1]);
+                                          P[a][k][0][2 * h + 1], P[a][k][PH - 1][2 * h + 1]);
                             }
                         }
                 // 8 bits: one ldmatrix.x4.trans brings 16 dims of 32 tokens or 32 dims of 16; each
@@ -614,7 +705,7 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
 #pragma unroll
                                     for (int a = 0; a < MT; ++a)
 #pragma unroll
-                                        for (int h = S::HL - 1; h >= 0; --h)
+                                        for (int h = PH - 1; h >= 0; --h)
                                             mma_f16(d[a][x], P[a][2 * k2 + k][h], b0, b1);
                                 }
                         }
@@ -628,7 +719,7 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
 #pragma unroll
                                 for (int a = 0; a < MT; ++a)
 #pragma unroll
-                                    for (int h = S::HL - 1; h >= 0; --h)
+                                    for (int h = PH - 1; h >= 0; --h)
                                         mma_f16(d[a][x], P[a][k][h], r[2 * x], r[2 * x + 1]);
                         }
                     }
@@ -810,7 +901,9 @@ template <int KV, int HD>
 int launch_mode(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq, float* out,
                 int ld_out, const float* q, int ld_q, float scale, float* ws, cudaStream_t st) {
     const int M = tr.max_nodes * (nq / c.n_kv_heads);
-    if (KV == SLATE_KV_F16 ? M > 16 : KV == SLATE_KV_Q8 && M > 32) {
+    // attn_tree_mma with 32 rows against attn_tree_tc, 16 sequences of 8 nodes x 4 heads over 8000
+    // tokens: f16 at head_dim 128 113 and 93 us, at 64 62 and 79, 8 bits at 128 103 and 129
+    if (KV != SLATE_KV_F32 && M > (KV == SLATE_KV_F16 && HD == 128 ? 16 : 32)) {
         const int rc = attend_tc(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);
         return rc ? rc : join<HD>(c, tr, nq, TC_ROWS, TC_UNIT, SMS, out, ld_out, ws, st);
     }
