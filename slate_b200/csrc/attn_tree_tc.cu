@@ -7,7 +7,7 @@
 //   S = Qhi K^T + Qlo K^T           128 x 128, in tensor memory, f32
 //   P = exp(S - max), hi and lo     written over S, the next product's A operand
 //   D = Phi V + Plo V               128 x head_dim, in tensor memory
-//   O = O corr + D                  in registers, one FMA an element
+//   O += D                          in registers, every RUN tiles
 // S has two buffers: while the softmax warps work on tile j, the tensor cores run P V of
 // tile j - 1 and Q K^T of tile j + 1.  D is drained every tile because an
 // accumulator carried over a long context in the tensor cores would truncate at every step.
@@ -15,7 +15,7 @@
 // (they exchange the row's maximum) and of O's dims: the work is mostly latency, and four
 // warps a scheduler hide it where two with twice the row did not.  Warps 16-22 bring K and V
 // page by page in turn into the operands' swizzled layout (f16: 16-byte asynchronous copies;
-// 8 bits: through registers, three pages ahead, widened to f16 on the way).  Warp 23 issues the
+// 8 bits: through registers, two pages ahead, widened to f16 on the way).  Warp 23 issues the
 // products.
 // What bounds it: the tensor cores, 2 x the plain formula's products for the two
 // halves, from 64 rows up; the exponentials and splits take nearly as many issue slots.
@@ -29,23 +29,32 @@
 #include "sb_pdl.h"
 #include "sb_tree.h"
 
+#ifndef SB_RUN
+#define SB_RUN 8
+#endif
+
 using namespace sb_tree;
 
 namespace {
 
-constexpr int MR = 128, KT = 128, NPW = 7;
-constexpr int NB = 3;                         // K and V tiles in shared memory, of each
-#ifndef SB_PARTS
-#define SB_PARTS (KV == SLATE_KV_Q8 ? 2 : 4)
-#endif
+constexpr int MR = 128, KT = 128;
+constexpr int PARTS = 2;                      // threads that share a row
+constexpr int NSW = 4 * PARTS, NPW = 7, NTHREADS = 32 * (NSW + NPW + 1);
 constexpr uint64_t WAIT_NS = 2000000000ull;
-constexpr int SCB = 8;                        // tiles whose scales and flags are kept: NB + 2 are in use
+constexpr int SCB = 8;                        // tiles whose scales and flags are kept: NB + 3 are in use
+// The maximum that p is taken against may lag behind the true one by 2^LAG: only then are O and
+// the sum rescaled.  p carries 2^(15 - LAG), so that it stays below f16's end all the same.
+constexpr int LAG = 8;
+// Tiles that D may add up before it is drained (a power of two).  The tensor cores cut each
+// step's sum off: 8 tiles, 128 steps, cost 1e-6 of the output at worst, one tile 1e-7.
+constexpr int RUN = SB_RUN;
 
-// PARTS threads share a row.
 template <int KV, int HD>
 struct TcShape {
-    static constexpr int PARTS = SB_PARTS;
-    static constexpr int NSW = 4 * PARTS, NTHREADS = 32 * (NSW + NPW + 1);
+    // K and V tiles in shared memory, of each: the 8-bit producers go through registers and
+    // the first-level cache, which a third pair would leave little of (490 against 550 us at 256
+    // rows over 32000 tokens); f16 keeps more copies in flight with three (76 against 66 us, 64 rows)
+    static constexpr int NB = KV == SLATE_KV_Q8 ? 2 : 3;
     static constexpr int TB = KT * HD * 2;                 // a K or V tile in f16
     static constexpr int SC = SCB * 2 * KT * 4;
     static constexpr int SMEM = 2 * NB * TB + SC + 1024;
@@ -58,8 +67,9 @@ struct No {
     static constexpr bool value = false;
 };
 
+template <int NB>
 struct Bars {
-    uint64_t kfull[NB], kfree[NB], vfull[NB], vfree[NB], sfull[2], pfull[2], dfull, dfree;
+    uint64_t kfull[NB], kfree[NB], vfull[NB], vfree[NB], sfull[2], pfull[2], dfull[2];
 };
 
 __device__ __forceinline__ uint64_t gtimer() {
@@ -135,10 +145,9 @@ __device__ __forceinline__ void tmem_st(uint32_t a, const uint32_t (&r)[16]) {
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-template <int N>
 __device__ __forceinline__ void softmax_sync() {
     __syncwarp();
-    asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * NSW) : "memory");
 }
 // Byte of 16-byte chunk ch (8 f16) of row r in an operand of 128 rows: 64 columns a
 // 16 KB block, rows of 128 bytes, chunks exchanged by the row's low bits.
@@ -177,18 +186,18 @@ struct Segs {
 };
 
 template <int KV, int HD>
-__global__ void __launch_bounds__(TcShape<KV, HD>::NTHREADS, 1) attn_tree_tc(
+__global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
     const slate_kv_cache_t c, int layer, const slate_tree_t tr, int nq, float* __restrict__ out,
     int ld_out, const float* __restrict__ q, int ld_q, float scale, float* __restrict__ ws) {
     using S = TcShape<KV, HD>;
     constexpr bool Q8 = KV == SLATE_KV_Q8;
-    constexpr int KS = HD / 16, PARTS = S::PARTS, NSW = S::NSW, NTHREADS = S::NTHREADS;
+    constexpr int KS = HD / 16, NB = S::NB;
     extern __shared__ unsigned char smem_raw[];
     // by an offset, so that the compiler still knows it for shared memory
     unsigned char* smem = smem_raw + ((1024u - (su32(smem_raw) & 1023u)) & 1023u);
     unsigned char* skv = smem;                                  // NB of K, NB of V
     float* ssc = (float*)(skv + 2 * NB * S::TB);                      // [SCB][K, V][KT]
-    __shared__ Bars bars;
+    __shared__ Bars<NB> bars;
     __shared__ Segs sg;
     __shared__ int more_s;
     __shared__ PlanBuf buf;
@@ -197,6 +206,7 @@ __global__ void __launch_bounds__(TcShape<KV, HD>::NTHREADS, 1) attn_tree_tc(
     __shared__ uint16_t odd_s[SCB][8];                             // per page: tokens whose v is not finite
     __shared__ __align__(16) float vmax_s[SCB][8];                 // per page: largest v scale
     __shared__ float part_max[2][PARTS][MR];      // [tile parity][part][row]
+    __shared__ int need_s[4];                     // tile % 4: some row's maximum grew beyond LAG
     __shared__ int fail_s;
     sb_grid_wait();
     sb_grid_release();
@@ -214,9 +224,9 @@ __global__ void __launch_bounds__(TcShape<KV, HD>::NTHREADS, 1) attn_tree_tc(
         for (int i = 0; i < 2; ++i) {
             bar_init(&bars.sfull[i], 1);
             bar_init(&bars.pfull[i], 32 * NSW);
+            bar_init(&bars.dfull[i], 1);
         }
-        bar_init(&bars.dfull, 1);
-        bar_init(&bars.dfree, 32 * NSW);
+        for (int i = 0; i < 4; ++i) need_s[i] = 0;
         fail_s = 0;
         sg.at = st_.at;
         sg.stop = st_.stop;
@@ -255,8 +265,7 @@ __global__ void __launch_bounds__(TcShape<KV, HD>::NTHREADS, 1) attn_tree_tc(
 
     if (warp < NSW) {
         // no spills: with 227 KB of shared memory the first-level cache is too small to hold them
-        if (PARTS == 4) asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
-        else asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
         while (next_segment()) {
             const Seq& sq_ = sg.sq;
             const int nt = sg.nt, kvh = sg.kvh, r_base = sg.r_base, n_rows = sg.n_rows, tok0 = sg.tok0;
@@ -278,7 +287,7 @@ __global__ void __launch_bounds__(TcShape<KV, HD>::NTHREADS, 1) attn_tree_tc(
                 }
                 part_max[0][h][r] = __uint_as_float(top);
             }
-            softmax_sync<32 * NSW>();
+            softmax_sync();
             uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < PARTS; ++i) top = max(top, __float_as_uint(part_max[0][i][r]));
@@ -301,177 +310,199 @@ __global__ void __launch_bounds__(TcShape<KV, HD>::NTHREADS, 1) attn_tree_tc(
             __syncthreads();
             tc_after();
             const uint64_t mk = r < n_rows ? __ldg(tr.mask + sq_.r0 + (r_base + r) / G) : 0;
-            float m = -INFINITY, l = 0.f, corr = 0.f;
-            int vexp = -80, vlast = -80;
+            float m = -INFINITY, l = 0.f;              // m: what p is taken against, in log2 units
+            int vexp = -80;                            // 8 bits: 2^vexp is above every v scale so far
             bool ok = true;
-            // O = O corr + D of tile j
-            const auto drain = [&](int j) {
-                ok = ok && __all_sync(FULL, bar_wait(&bars.dfull, (tb + j) & 1, fail));
-                if (!ok || !live) {
-                    bar_arrive(&bars.dfree);
-                    return;
-                }
+            const auto scales = [&](int j) { return ssc + (tb + j) % SCB * (2 * KT) + TQ * h; };
+            const auto s_part = [&](int j) { return sS((tb + j) & 1) + lanes + TQ * h; };
+            const auto first_token = [&](int j) { return tok0 + j * KT + TQ * h; };
+            const auto wait_s = [&](int j) {
+                ok = ok && __all_sync(FULL, bar_wait(&bars.sfull[(tb + j) & 1], phase2(tb + j), fail));
                 tc_after();
-                const float2 c2 = make_float2(corr, corr);
+            };
+            // The product of tile j is done.  Not waited for every tile: its barrier (of the tile's parity)
+            // is at most one phase ahead, since the tile after next needs this thread's p.
+            const auto wait_d = [&](int j) {
+                ok = ok && __all_sync(FULL, bar_wait(&bars.dfull[(tb + j) & 1], phase2(tb + j), fail));
+                tc_after();
+            };
+            // every row sees every token of the thread's part of tile j
+            const auto seen_by_all = [&](int j) {
+                return *(const uint32_t*)&gone_s[(tb + j) % SCB][TQ / 16 * h] == 0 && first_token(j) + TQ <= sq_.ctx;
+            };
+            // which of the part's 32 tokens from t the row sees
+            const auto seen = [&](int j, int t) {
+                const uint8_t* gone = &gone_s[(tb + j) % SCB][TQ / 16 * h + t / 16];
+                uint32_t v = 0xffffffffu;
+                if (gone[0]) v &= 0xffff0000u;
+                if (gone[1]) v &= 0x0000ffffu;
+                const int x = first_token(j) + t - sq_.ctx;            // < 0: tokens of the context first
+                if (x + 32 > 0) {
+                    const uint64_t all = mk & (sq_.n == 64 ? ~0ull : (1ull << sq_.n) - 1);
+                    v &= x >= 0 ? (x < 64 ? (uint32_t)(all >> x) : 0u) : (uint32_t)(all << -x) | ((1u << -x) - 1);
+                }
+                return v;
+            };
+            // the largest of 16 scores (8 bits: times the tokens' scales)
+            const auto max16 = [&](auto all, const uint32_t (&x)[16], const float* ks, uint32_t v, float mx) {
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    float y[4] = {__uint_as_float(x[i]), __uint_as_float(x[i + 1]), __uint_as_float(x[i + 2]),
+                                  __uint_as_float(x[i + 3])};
+                    if (Q8) {
+                        const float4 k4 = *(const float4*)(ks + i);
+                        const float2 y0 = __fmul2_rn(make_float2(y[0], y[1]), make_float2(k4.x, k4.y));
+                        const float2 y1 = __fmul2_rn(make_float2(y[2], y[3]), make_float2(k4.z, k4.w));
+                        y[0] = y0.x, y[1] = y0.y, y[2] = y1.x, y[3] = y1.y;
+                    }
+                    if (!all.value)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (!(v >> (i + e) & 1)) y[e] = -INFINITY;
+                    mx = fmaxf(fmaxf(mx, fmaxf(y[0], y[1])), fmaxf(y[2], y[3]));
+                }
+                return mx;
+            };
+            // 16 scores to p, as 8 pairs' high halves and then their low halves
+            const auto p16 = [&](auto all, const uint32_t (&x)[16], uint32_t (&pk)[16], const float* ks, uint32_t v,
+                                 float2 rs2, float2 nb2, float2& sum) {
+                float4 k4, v4;
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    float2 y = make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                    if (Q8 && i % 4 == 0) {
+                        k4 = *(const float4*)(ks + i);
+                        v4 = *(const float4*)(ks + KT + i);
+                    }
+                    if (Q8) y = __fmul2_rn(y, i % 4 ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y));
+                    y = __ffma2_rn(y, rs2, nb2);
+                    float2 p = make_float2(ex2(y.x), ex2(y.y));
+                    if (!all.value) {
+                        if (!(v >> i & 1)) p.x = 0.f;
+                        if (!(v >> (i + 1) & 1)) p.y = 0.f;
+                    }
+                    sum = __fadd2_rn(sum, p);
+                    if (Q8) {
+                        p = __fmul2_rn(p, i % 4 ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y));
+                        if (!all.value) {                              // 0 stays 0 whatever the scale
+                            if (!(v >> i & 1)) p.x = 0.f;
+                            if (!(v >> (i + 1) & 1)) p.y = 0.f;
+                        }
+                    }
+                    split_f16(p.x, p.y, pk[i / 2], pk[8 + i / 2]);
+                }
+            };
+            const auto tile_max = [&](auto all, int j) {
+                float mx = -INFINITY;
+#pragma unroll
+                for (int cc = 0; cc < TQ / 16; ++cc) {
+                    uint32_t x[16];
+                    tmem_ld(s_part(j) + 16 * cc, x);
+                    const uint32_t v = all.value ? 0xffffffffu : seen(j, 16 * cc & ~31) >> (16 * cc & 31);
+                    tmem_ld_wait();
+                    mx = max16(all, x, scales(j) + 16 * cc, v, mx);
+                }
+                return mx;
+            };
+            // p of tile j, written over the S that it came from, and its sum
+            const auto tile_p = [&](auto all, int j) {
+                const float base = (m == -INFINITY ? 0.f : m) - (float)(15 - LAG - (Q8 ? vexp : 0));
+                const float2 rs2 = make_float2(rs, rs), nb2 = make_float2(-base, -base);
+                float2 sum = make_float2(0.f, 0.f);
+#pragma unroll 1
+                for (int cc = 0; cc < TQ / 16; ++cc) {                 // 16 tokens: one step of the product
+                    uint32_t x[16], pk[16];
+                    tmem_ld(s_part(j) + 16 * cc, x);
+                    const uint32_t v = all.value ? 0xffffffffu : seen(j, 16 * cc & ~31) >> (16 * cc & 31);
+                    tmem_ld_wait();
+                    p16(all, x, pk, scales(j) + 16 * cc, v, rs2, nb2, sum);
+                    tmem_st(s_part(j) + 16 * cc, pk);
+                }
+                return sum.x + sum.y;
+            };
+            const auto v_exponent = [&](int j) {
+                const float* v = vmax_s[(tb + j) % SCB];
+                const float4 a = *(const float4*)v, z = *(const float4*)(v + 4);
+                const float vm = fmaxf(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)), fmaxf(fmaxf(z.x, z.y), fmaxf(z.z, z.w)));
+                return min(max((int)(__float_as_uint(vm) >> 23) - 126, -80), 126);
+            };
+            // the part's maximum of tile j for the row's other threads, and whether anything has to be
+            // rescaled for it; a barrier
+            const auto publish = [&](int j, float mx) {
+                const uint32_t t = tb + j;
+                if (ok && live) {
+                    part_max[t & 1][h][r] = mx;
+                    if (mx * rs > m + (float)LAG || (Q8 && v_exponent(j) > vexp)) need_s[t & 3] = 1;
+                }
+                softmax_sync();
+                if (tid == 0) need_s[(t + 2) & 3] = 0;
+            };
+            const auto add_d = [&]() {                 // O += D
 #pragma unroll
                 for (int cc = 0; cc < HO / 16; ++cc) {
                     uint32_t d[16];
                     tmem_ld(sD + lanes + HO * h + 16 * cc, d);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        const float2 x = __ffma2_rn(make_float2(O[16 * cc + i], O[16 * cc + i + 1]), c2,
-                                                    make_float2(__uint_as_float(d[i]), __uint_as_float(d[i + 1])));
-                        O[16 * cc + i] = x.x;
-                        O[16 * cc + i + 1] = x.y;
-                    }
-                }
-                tc_before();
-                bar_arrive(&bars.dfree);
-                // f16: infinities and NaN were taken out of the v that only some rows see; the
-                // rows that see them get them here
-                const int t0 = tok0 + j * KT;
-                if (!Q8 && t0 + KT > sq_.ctx) {
-                    for (int w = 0; w < 8; ++w)
-                        for (uint32_t rest = odd_s[(tb + j) % SCB][w]; rest; rest &= rest - 1) {
-                            const int t = t0 + 16 * w + __ffs(rest) - 1, x = t - sq_.ctx;
-                            const int page = sb_kv_page(c, sq_.slot, t);
-                            if (page < 0 || x < 0 || x >= sq_.n || !(mk >> x & 1)) continue;
-                            const __half* v = (const __half*)sb_kv_block(c, layer, page, 1, kvh) + (t & 15) * HD + HO * h;
-#pragma unroll
-                            for (int i = 0; i < HO; ++i) {
-                                const float y = __half2float(v[i]);
-                                if (!(fabsf(y) < INFINITY)) O[i] += y;
-                            }
-                        }
+                    for (int i = 0; i < 16; ++i) O[16 * cc + i] += __uint_as_float(d[i]);
                 }
             };
             for (int j = 0; j < nt; ++j) {             // to the end even after a failed wait: the barriers count
-                const uint32_t t_ = tb + j, sc_ = t_ % SCB;
-                const int b = t_ & 1;
-                ok = ok && __all_sync(FULL, bar_wait(&bars.sfull[b], phase2(t_), fail));
-                tc_after();
-                const bool work = ok && live;
-                const float* ks = ssc + sc_ * 2 * KT + TQ * h;
-                const float* vs = ks + KT;
-                const int t0 = tok0 + j * KT + TQ * h;                 // the part's first token
-                const uint8_t* gone = &gone_s[sc_][TQ / 16 * h];               // a byte a page
-                const bool any_gone = PARTS == 4 ? *(const uint16_t*)gone != 0 : *(const uint32_t*)gone != 0;
-                const uint32_t sp = sS(b) + lanes + TQ * h;
-                // which of the part's 32 tokens from t the row sees
-                const auto seen = [&](int t) {
-                    uint32_t v = 0xffffffffu;
-                    if (gone[t / 16]) v &= 0xffff0000u;
-                    if (gone[t / 16 + 1]) v &= 0x0000ffffu;
-                    const int x = t0 + t - sq_.ctx;                    // < 0: tokens of the context first
-                    if (x + 32 > 0) {
-                        const uint64_t all = mk & (sq_.n == 64 ? ~0ull : (1ull << sq_.n) - 1);
-                        v &= x >= 0 ? (x < 64 ? (uint32_t)(all >> x) : 0u) : (uint32_t)(all << -x) | ((1u << -x) - 1);
-                    }
-                    return v;
-                };
-                // Two passes over the part of S, 16 tokens at a time: the maximum; then p, its halves
-                // written over the S that they came from.  `all`: every row sees every token.
-                const auto tile_max = [&](auto all) {
-                    float mx = -INFINITY;
-#pragma unroll
-                    for (int cc = 0; cc < TQ / 16; ++cc) {
-                        uint32_t x[16];
-                        tmem_ld(sp + 16 * cc, x);
-                        const uint32_t v = all.value ? 0xffffffffu : seen(16 * cc & ~31) >> (16 * cc & 31);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            float y[4] = {__uint_as_float(x[i]), __uint_as_float(x[i + 1]), __uint_as_float(x[i + 2]),
-                                          __uint_as_float(x[i + 3])};
-                            if (Q8) {
-                                const float4 k4 = *(const float4*)(ks + 16 * cc + i);
-                                const float2 y0 = __fmul2_rn(make_float2(y[0], y[1]), make_float2(k4.x, k4.y));
-                                const float2 y1 = __fmul2_rn(make_float2(y[2], y[3]), make_float2(k4.z, k4.w));
-                                y[0] = y0.x, y[1] = y0.y, y[2] = y1.x, y[3] = y1.y;
-                            }
-                            if (!all.value)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    if (!(v >> (i + e) & 1)) y[e] = -INFINITY;
-                            mx = fmaxf(fmaxf(mx, fmaxf(y[0], y[1])), fmaxf(y[2], y[3]));
-                        }
-                    }
-                    return mx;
-                };
-                const auto tile_p = [&](auto all, float base) {
-                    float2 sum = make_float2(0.f, 0.f);
-                    const float2 rs2 = make_float2(rs, rs), nb2 = make_float2(-base, -base);
-#pragma unroll 1
-                    for (int cc = 0; cc < TQ / 16; ++cc) {             // 16 tokens: one step of the product
-                        uint32_t x[16], pk[16];                        // pk: hi of 8 pairs, then lo
-                        float4 k4, v4;
-                        tmem_ld(sp + 16 * cc, x);
-                        const uint32_t v = all.value ? 0xffffffffu : seen(16 * cc & ~31) >> (16 * cc & 31);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            float2 y = make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-                            if (Q8 && i % 4 == 0) {
-                                k4 = *(const float4*)(ks + 16 * cc + i);
-                                v4 = *(const float4*)(vs + 16 * cc + i);
-                            }
-                            if (Q8) y = __fmul2_rn(y, i % 4 ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y));
-                            y = __ffma2_rn(y, rs2, nb2);
-                            float2 p = make_float2(ex2(y.x), ex2(y.y));
-                            if (!all.value) {
-                                if (!(v >> i & 1)) p.x = 0.f;
-                                if (!(v >> (i + 1) & 1)) p.y = 0.f;
-                            }
-                            sum = __fadd2_rn(sum, p);
-                            if (Q8) {
-                                p = __fmul2_rn(p, i % 4 ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y));
-                                if (!all.value) {                      // 0 stays 0 whatever the scale
-                                    if (!(v >> i & 1)) p.x = 0.f;
-                                    if (!(v >> (i + 1) & 1)) p.y = 0.f;
-                                }
-                            }
-                            split_f16(p.x, p.y, pk[i / 2], pk[8 + i / 2]);
-                        }
-                        tmem_st(sp + 16 * cc, pk);
-                    }
-                    return sum.x + sum.y;
-                };
-                const bool all = !any_gone && t0 + TQ <= sq_.ctx;
-                if (work) part_max[b][h][r] = all ? tile_max(Yes{}) : tile_max(No{});
-                softmax_sync<32 * NSW>();
-                float ncorr = 0.f;
-                if (work) {
-                    float mx = part_max[b][0][r];
-#pragma unroll
-                    for (int i = 1; i < PARTS; ++i) mx = fmaxf(mx, part_max[b][i][r]);
-                    // the row's scores in log2 units; f16: p carries 2^15 itself
-                    const float top = mx == -INFINITY ? -INFINITY : mx * rs;
-                    const float mn = fmaxf(m, top);
-                    // p carries 2^up; 8 bits: 2^15 over a power of two above every v scale so far, so that
-                    // p vscale keeps f16's range
-                    int up = 15;
-                    if (Q8) {
-                        const float4 a = *(const float4*)vmax_s[sc_], z = *(const float4*)(vmax_s[sc_] + 4);
-                        const float vm = fmaxf(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)), fmaxf(fmaxf(z.x, z.y), fmaxf(z.z, z.w)));
-                        vexp = max(vexp, min(max((int)(__float_as_uint(vm) >> 23) - 126, -80), 126));
-                        up -= vexp;
-                    }
-                    const float base = (mn == -INFINITY ? 0.f : mn) - (float)up;
-                    ncorr = ex2(m - (mn == -INFINITY ? 0.f : mn));
+                const uint32_t t = tb + j;
+                wait_s(j);
+                const bool all = seen_by_all(j);
+                float mx = -INFINITY;
+                if (ok && live) mx = all ? tile_max(Yes{}, j) : tile_max(No{}, j);
+                publish(j, mx);
+                const bool need = need_s[t & 3];
+                if (j > 0 && (need || j % RUN == 0)) {
+                    wait_d(j - 1);
+                    if (ok && live) add_d();
+                }
+                if (need && ok && live) {
+                    mx = fmaxf(part_max[t & 1][0][r], part_max[t & 1][1][r]);
+                    const float mn = fmaxf(m, mx == -INFINITY ? -INFINITY : mx * rs);
+                    float corr = mn == -INFINITY ? 1.f : ex2(m - mn);
                     m = mn;
-                    const float ls = all ? tile_p(Yes{}, base) : tile_p(No{}, base);
-                    if (Q8) ncorr *= ex2((float)(vlast - vexp));       // l and o carry 2^up alike
-                    vlast = vexp;
-                    l = fmaf(l, ncorr, ls);
+                    if (Q8) {                          // l and O carry 2^(15 - LAG - vexp)
+                        const int e = max(vexp, v_exponent(j));
+                        corr *= ex2((float)(vexp - e));
+                        vexp = e;
+                    }
+                    l *= corr;
+#pragma unroll
+                    for (int i = 0; i < HO; ++i) O[i] *= corr;
+                }
+                if (ok && live) {
+                    l += all ? tile_p(Yes{}, j) : tile_p(No{}, j);
                     tmem_st_wait();
                 }
                 tc_before();
-                bar_arrive(&bars.pfull[b]);
-                if (j > 0) drain(j - 1);
-                corr = ncorr;
+                bar_arrive(&bars.pfull[t & 1]);
             }
-            drain(nt - 1);
+            wait_d(nt - 1);
+            if (ok && live) {
+                add_d();
+                // f16: infinities and NaN were taken out of the v that only some rows see (the last 64
+                // tokens at most); the rows that see them get them here
+                if (!Q8)
+                    for (int j = max(nt - 2, 0); j < nt; ++j) {
+                        const int t0 = tok0 + j * KT;
+                        if (t0 + KT <= sq_.ctx) continue;
+                        for (int w = 0; w < 8; ++w)
+                            for (uint32_t rest = odd_s[(tb + j) % SCB][w]; rest; rest &= rest - 1) {
+                                const int t = t0 + 16 * w + __ffs(rest) - 1, x = t - sq_.ctx;
+                                const int page = sb_kv_page(c, sq_.slot, t);
+                                if (page < 0 || x < 0 || x >= sq_.n || !(mk >> x & 1)) continue;
+                                const __half* v = (const __half*)sb_kv_block(c, layer, page, 1, kvh) + (t & 15) * HD + HO * h;
+#pragma unroll
+                                for (int i = 0; i < HO; ++i) {
+                                    const float y = __half2float(v[i]);
+                                    if (!(fabsf(y) < INFINITY)) O[i] += y;
+                                }
+                            }
+                    }
+            }
             tb += nt;
             if (live) part_max[0][h][r] = l;
             __syncthreads();                           // every product is done: q and the scales are free
@@ -501,8 +532,7 @@ __global__ void __launch_bounds__(TcShape<KV, HD>::NTHREADS, 1) attn_tree_tc(
             if (*fail) break;
         }
     } else {
-    if (PARTS == 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
-    else asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
     if (warp == NSW + NPW) {
         // ================= products: f32 accumulate, M = 128, N = 128 (scores) or HD (p v);
         // V is MN-major (bit 16)
@@ -514,21 +544,21 @@ __global__ void __launch_bounds__(TcShape<KV, HD>::NTHREADS, 1) attn_tree_tc(
                 bool ok = true;
                 const auto pv = [&](uint32_t t) {
                     const int b = t & 1, vb_ = t % NB;
-                    // D's last contents are in the softmax's registers
-                    ok = ok && bar_wait(&bars.vfull[vb_], phaseN(t), fail) && bar_wait(&bars.pfull[b], phase2(t), fail) &&
-                         (t == 0 || bar_wait(&bars.dfree, (t - 1) & 1, fail));
+                    ok = ok && bar_wait(&bars.vfull[vb_], phaseN(t), fail) && bar_wait(&bars.pfull[b], phase2(t), fail);
                     if (!ok) return;
+                    // D begins anew where the softmax has added it to O
+                    const bool anew = need_s[t & 3] || (t - tb) % RUN == 0;
                     fence_async();
                     tc_after();
                     const uint32_t vb = su32(skv) + (NB + vb_) * S::TB;
 #pragma unroll
                     for (int k = 0; k < KT / 16; ++k) {
                         const uint64_t bd = desc(vb + 2048 * k, 16384);
-                        mma_ts(sD, sS(b) + 16 * k + 8, bd, idv, k > 0);
+                        mma_ts(sD, sS(b) + 16 * k + 8, bd, idv, k > 0 || !anew);
                         mma_ts(sD, sS(b) + 16 * k, bd, idv, 1);
                     }
                     commit(&bars.vfree[vb_]);
-                    commit(&bars.dfull);
+                    commit(&bars.dfull[b]);
                 };
                 const uint32_t nt = sg.nt;
                 for (uint32_t t = tb; t < tb + nt && ok; ++t) {
@@ -601,7 +631,7 @@ __global__ void __launch_bounds__(TcShape<KV, HD>::NTHREADS, 1) attn_tree_tc(
                 };
                 const auto fetch = [&](Raw& r, int n) {
                     const int page = r.page = r.next;
-                    r.next = page_of(n + 3 * NPW);
+                    r.next = page_of(n + 2 * NPW);
                     const unsigned char* blk = pool + max(page, 0) * page_step + ((n & 8) ? kv_step : 0);
 #pragma unroll
                     for (int i = 0; i < NP; ++i)
@@ -649,22 +679,18 @@ __global__ void __launch_bounds__(TcShape<KV, HD>::NTHREADS, 1) attn_tree_tc(
                     }
                     arrive(n);
                 };
-                // three pages in flight, in registers of their own: the wait for one is not a wait for
+                // two pages in flight, in registers of their own: the wait for one is not a wait for
                 // the other
-                Raw a, d, z;
+                Raw a, z;
                 a.next = page_of(w);
-                d.next = page_of(w + NPW);
-                z.next = page_of(w + 2 * NPW);
+                z.next = page_of(w + NPW);
                 fetch(a, w);
-                fetch(d, w + NPW);
-                fetch(z, w + 2 * NPW);
-                for (int n = w; n < njobs && ok; n += 3 * NPW) {
+                fetch(z, w + NPW);
+                for (int n = w; n < njobs && ok; n += 2 * NPW) {
                     put(a, n);
-                    fetch(a, n + 3 * NPW);
-                    if (n + NPW < njobs) put(d, n + NPW);
-                    fetch(d, n + 4 * NPW);
-                    if (n + 2 * NPW < njobs) put(z, n + 2 * NPW);
-                    fetch(z, n + 5 * NPW);
+                    fetch(a, n + 2 * NPW);
+                    if (n + NPW < njobs) put(z, n + NPW);
+                    fetch(z, n + 3 * NPW);
                 }
             } else {
                 constexpr int CPT = HD / 8, TS = 32 / CPT, NP = 16 / TS;       // chunks a token; tokens a step
@@ -751,7 +777,7 @@ int launch(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq,
     static const cudaError_t ready =
         cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, TcShape<KV, HD>::SMEM);
     if (ready != cudaSuccess) return sb_cuda_check(ready, "attention_tree shared memory");
-    return sb_cuda_check(sb_launch_pdl(k, dim3(SMS), dim3(TcShape<KV, HD>::NTHREADS), TcShape<KV, HD>::SMEM, st, c, layer, tr, nq,
+    return sb_cuda_check(sb_launch_pdl(k, dim3(SMS), dim3(NTHREADS), TcShape<KV, HD>::SMEM, st, c, layer, tr, nq,
                                        out, ld_out, q, ld_q, scale, ws),
                          "attention_tree");
 }
