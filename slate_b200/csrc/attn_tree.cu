@@ -412,6 +412,13 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
                 for (int j = 0; j < NTK; ++j) sc[a][j][0] = sc[a][j][1] = sc[a][j][2] = sc[a][j][3] = 0.f;
             // ---- scores
             if constexpr (KV == SLATE_KV_F32) {
+                // the products with a low half in sums of their own: a tensor-core sum is cut off at every
+                // step, and the large one takes a third of the steps this way
+                float sx[MT][NTK][4];
+#pragma unroll
+                for (int a = 0; a < MT; ++a)
+#pragma unroll
+                    for (int j = 0; j < NTK; ++j) sx[a][j][0] = sx[a][j][1] = sx[a][j][2] = sx[a][j][3] = 0.f;
 #pragma unroll
                 for (int cc = 0; cc < HD / 16; ++cc) {
                     uint4 A[MT][2][S::HL];
@@ -436,12 +443,18 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
                             for (int a = 0; a < MT; ++a) {
                                 const uint4 h4 = A[a][k][0], l4 = A[a][k][S::HL - 1];
                                 const uint32_t ah[4] = {h4.x, h4.y, h4.z, h4.w}, al[4] = {l4.x, l4.y, l4.z, l4.w};
-                                mma_tf32(sc[a][j], ah, bl[2 * k], bl[2 * k + 1]);
-                                if (MODE) mma_tf32(sc[a][j], al, bh[2 * k], bh[2 * k + 1]);
+                                mma_tf32(sx[a][j], ah, bl[2 * k], bl[2 * k + 1]);
+                                if (MODE) mma_tf32(sx[a][j], al, bh[2 * k], bh[2 * k + 1]);
                                 mma_tf32(sc[a][j], ah, bh[2 * k], bh[2 * k + 1]);
                             }
                     }
                 }
+#pragma unroll
+                for (int a = 0; a < MT; ++a)
+#pragma unroll
+                    for (int j = 0; j < NTK; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sc[a][j][e] += sx[a][j][e];
             } else if constexpr (S::I8) {
                 // exact: |sum| <= 128 * 127 * 128 < 2^21.  The sums start at the bits of 1.5 * 2^23, so that
                 // the result read as a float is 1.5 * 2^23 + sum
@@ -627,34 +640,43 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
             }
             // ---- o = o corr + p v
             if constexpr (KV == SLATE_KV_F32) {
+                // up to 8 rows: rows 0-7 of ph hold the high halves, rows 8-15 the low ones
+                uint32_t ph[MT][NTK][4], pl[MT][NTK][4];
+#pragma unroll
+                for (int a = 0; a < MT; ++a)
+#pragma unroll
+                    for (int j = 0; j < NTK; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (MODE == 0) {
+                                split_tf32(p[0][j][e], ph[a][j][2 * e], ph[a][j][2 * e + 1]);
+                            } else {
+                                split_tf32(p[(2 * a) % RI][j][e], ph[a][j][2 * e], pl[a][j][2 * e]);
+                                split_tf32(p[(2 * a + 1) % RI][j][e], ph[a][j][2 * e + 1], pl[a][j][2 * e + 1]);
+                            }
 #pragma unroll
                 for (int jd = 0; jd < NTD; ++jd) {
                     float d[MT][4];
+                    uint32_t bh[NTK][2], bl[NTK][2];
 #pragma unroll
                     for (int a = 0; a < MT; ++a) d[a][0] = d[a][1] = d[a][2] = d[a][3] = 0.f;
 #pragma unroll
                     for (int j = 0; j < NTK; ++j) {
                         // k = t4 is token 2 t4, k = t4 + 4 token 2 t4 + 1 of the 8
                         const int r = 8 * j + 2 * t4, ch = 2 * jd + (g >> 2);
-                        uint32_t bh[2], bl[2];
-                        split_tf32(*(const float*)(st + KT * RB + swz<KV, RB>(r, ch) + 4 * (g & 3)), bh[0], bl[0]);
-                        split_tf32(*(const float*)(st + KT * RB + swz<KV, RB>(r + 1, ch) + 4 * (g & 3)), bh[1], bl[1]);
+                        split_tf32(*(const float*)(st + KT * RB + swz<KV, RB>(r, ch) + 4 * (g & 3)), bh[j][0], bl[j][0]);
+                        split_tf32(*(const float*)(st + KT * RB + swz<KV, RB>(r + 1, ch) + 4 * (g & 3)), bh[j][1], bl[j][1]);
+                    }
+                    // the products with a low half first, while the sum is small
 #pragma unroll
-                        for (int a = 0; a < MT; ++a) {
-                            uint32_t ah[4], al[4];
-                            if (MODE == 0) {
-                                split_tf32(p[0][j][0], ah[0], ah[1]);
-                                split_tf32(p[0][j][1], ah[2], ah[3]);
-                            } else {
-                                split_tf32(p[(2 * a) % RI][j][0], ah[0], al[0]);
-                                split_tf32(p[(2 * a + 1) % RI][j][0], ah[1], al[1]);
-                                split_tf32(p[(2 * a) % RI][j][1], ah[2], al[2]);
-                                split_tf32(p[(2 * a + 1) % RI][j][1], ah[3], al[3]);
-                                mma_tf32(d[a], al, bh[0], bh[1]);
-                            }
-                            mma_tf32(d[a], ah, bl[0], bl[1]);
-                            mma_tf32(d[a], ah, bh[0], bh[1]);
+                    for (int a = 0; a < MT; ++a) {
+#pragma unroll
+                        for (int j = 0; j < NTK; ++j) {
+                            if (MODE) mma_tf32(d[a], pl[a][j], bh[j][0], bh[j][1]);
+                            mma_tf32(d[a], ph[a][j], bl[j][0], bl[j][1]);
                         }
+#pragma unroll
+                        for (int j = 0; j < NTK; ++j) mma_tf32(d[a], ph[a][j], bh[j][0], bh[j][1]);
                     }
 #pragma unroll
                     for (int a = 0; a < MT; ++a)
