@@ -5,6 +5,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "sb_internal.h"
 #include "sb_kernels.h"
 #include "sb_kv.h"
@@ -88,92 +90,103 @@ __global__ void __launch_bounds__(256) rope_append_kernel(
 // The same in 16-byte vectors, for head_dim up to 128 and rot_dim % 8 == 0 (every
 // common head): LPH lanes hold a head, four dims each, so a pair's other half is in the
 // same lane (interleaved) or rot_dim / 8 lanes away (one shuffle an element), and a
-// warp keeps RU * 32 / LPH heads in flight.  Bound by HBM: q is read and written, k
-// and v read, the cache written once; nothing else moves.
-constexpr int RU = 4;
-template <int LPH, int KV>
+// warp keeps RU * 32 / LPH heads in flight; query heads and key/value heads go to warps
+// of their own, so neither carries the other's branches.  Bound by HBM: q is read and
+// written, k and v read, the cache written once; nothing else moves.  8191 rows of 32 + 8
+// + 8 heads of 128 on the 8-bit cache, with their read-back: 86 us, 5.1 TB/s (exact
+// division for every element: 101 us; q and k heads in one warp: 95 us).
+template <int LPH, int KV, int RU>
 __global__ void __launch_bounds__(256) rope_append_vec(
     const slate_kv_cache_t c, int layer, const slate_rope_t rope, int rows, int nq,
     float* q_out, int ld_qo, const float* q, int ld_q, const float* __restrict__ k, int ld_k,
     const float* __restrict__ v, int ld_v, const int32_t* __restrict__ row_slot,
-    const int32_t* __restrict__ row_index, const int32_t* __restrict__ row_pos, int parts) {
-    constexpr int HPW = 32 / LPH;
+    const int32_t* __restrict__ row_index, const int32_t* __restrict__ row_pos, int parts_q, int parts) {
+    constexpr int HPW = 32 / LPH;                          // heads a warp holds at once
     const int lane = threadIdx.x & 31, sub = lane % LPH, hd = c.head_dim, nkv = c.n_kv_heads;
-    const int heads = nq + 2 * nkv, half = rope.rot_dim / 2, d = 4 * sub;
-    const unsigned w = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-    const unsigned r = w / parts;
+    const int half = rope.rot_dim / 2, d = 4 * sub;
+    const unsigned w = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32, r = w / parts;
     if (r >= (unsigned)rows) return;
-    const int h0 = (int)(w % parts) * (RU * HPW) + lane / LPH;
+    // parts [0, parts_q) of a row are its query heads, the others its key and then value heads
+    const int part = (int)(w - r * parts);
+    const bool keys = part >= parts_q;
+    const int n = keys ? 2 * nkv : nq, h0 = (keys ? part - parts_q : part) * (RU * HPW) + lane / LPH;
     const int index = row_index[r], pos = row_pos[r], slot = row_slot[r];
-    if (index < 0 || pos < 0 || pos >= rope.n_pos) return;
-    float4 x[RU];
+    const bool in = d < hd;
+    float4 x[RU];                                          // asked for before the row is looked at
+    {
+        const float* first = (keys ? k + (size_t)r * ld_k : q + (size_t)r * ld_q) + d;
+        const float* vals = v + (size_t)r * ld_v - nkv * hd + d;
 #pragma unroll
-    for (int u = 0; u < RU; ++u) {
-        const int h = h0 + u * HPW;
-        x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (h < heads && d < hd) {
-            const float* p = h < nq ? q + (size_t)r * ld_q + (size_t)h * hd
-                             : h < nq + nkv ? k + (size_t)r * ld_k + (size_t)(h - nq) * hd
-                                            : v + (size_t)r * ld_v + (size_t)(h - nq - nkv) * hd;
-            x[u] = *(const float4*)(p + d);
+        for (int u = 0; u < RU; ++u) {
+            const int h = h0 + u * HPW;
+            x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (in && h < n) x[u] = *(const float4*)((keys && h >= nkv ? vals : first) + h * hd);
         }
     }
+    if (index < 0 || pos < 0 || pos >= rope.n_pos) return;
     const bool inter = rope.layout == SLATE_ROPE_INTERLEAVED, second = d >= half;
+    // An element is its own value times cos plus its partner's times sin, -sin for the first of a
+    // pair; dims beyond rot_dim keep their value (and are spared the product: 0 * NaN).
+    const bool turn = d < rope.rot_dim;
     float4 cs = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (d < rope.rot_dim) {
+    if (turn) {
         const size_t j = (size_t)pos * half + (inter ? d / 2 : second ? d - half : d);
         if (inter) {
             const float2 a = *(const float2*)(rope.cos + j), b = *(const float2*)(rope.sin + j);
             cs = make_float4(a.x, a.x, a.y, a.y);
-            sn = make_float4(b.x, b.x, b.y, b.y);
+            sn = make_float4(-b.x, b.x, -b.y, b.y);
         } else {
             cs = *(const float4*)(rope.cos + j);
             sn = *(const float4*)(rope.sin + j);
+            if (!second) sn = make_float4(-sn.x, -sn.y, -sn.z, -sn.w);
         }
     }
     const int from = inter ? lane : second ? lane - half / 4 : lane + half / 4;
-    const bool turn = d < rope.rot_dim;
+    const auto turned = [&](const float4& a) {
+        float4 o = make_float4(a.y, a.x, a.w, a.z);        // the partners
+        if (!inter) {
+            o.x = __shfl_sync(FULL, a.x, from & 31);
+            o.y = __shfl_sync(FULL, a.y, from & 31);
+            o.z = __shfl_sync(FULL, a.z, from & 31);
+            o.w = __shfl_sync(FULL, a.w, from & 31);
+        }
+        if (!turn) return a;
+        return make_float4(__fadd_rn(__fmul_rn(a.x, cs.x), __fmul_rn(o.x, sn.x)),
+                           __fadd_rn(__fmul_rn(a.y, cs.y), __fmul_rn(o.y, sn.y)),
+                           __fadd_rn(__fmul_rn(a.z, cs.z), __fmul_rn(o.z, sn.z)),
+                           __fadd_rn(__fmul_rn(a.w, cs.w), __fmul_rn(o.w, sn.w)));
+    };
+    if (!keys) {
+        float* o = q_out + (size_t)r * ld_qo + d;
+#pragma unroll
+        for (int u = 0; u < RU; ++u) {
+            const int h = h0 + u * HPW;
+            const float4 y = turned(x[u]);
+            if (in && h < n) *(float4*)(o + h * hd) = y;
+        }
+        return;
+    }
     const int page = sb_kv_page(c, slot, index), t = index % SB_PAGE_TOKENS;
+    if (page < 0) return;
+    unsigned char* blocks = sb_kv_block(c, layer, page, 0, 0);     // K heads, then V heads
+    const int bb = sb_kv_block_bytes(KV, hd);
 #pragma unroll
     for (int u = 0; u < RU; ++u) {
         const int h = h0 + u * HPW;
-        float4 y = x[u];
-        float4 o;
-        if (inter) {
-            o = make_float4(y.y, y.x, y.w, y.z);
-        } else {
-            o.x = __shfl_sync(FULL, y.x, from & 31);
-            o.y = __shfl_sync(FULL, y.y, from & 31);
-            o.z = __shfl_sync(FULL, y.z, from & 31);
-            o.w = __shfl_sync(FULL, y.w, from & 31);
-        }
-        if (turn && h < nq + nkv) {
-            // first of a pair: a c - b s; second: a s + b c
-            const auto one = [](float a, float b, float cs, float sn, bool sec) {
-                return sec ? __fadd_rn(__fmul_rn(b, sn), __fmul_rn(a, cs))
-                           : __fsub_rn(__fmul_rn(a, cs), __fmul_rn(b, sn));
-            };
-            y.x = one(x[u].x, o.x, cs.x, sn.x, inter ? false : second);
-            y.y = one(x[u].y, o.y, cs.y, sn.y, inter ? true : second);
-            y.z = one(x[u].z, o.z, cs.z, sn.z, inter ? false : second);
-            y.w = one(x[u].w, o.w, cs.w, sn.w, inter ? true : second);
-        }
+        float4 y = turned(x[u]);
+        if (h >= nkv) y = x[u];                            // (the shuffles above take every lane)
         uint32_t top = 0;
         if (KV == SLATE_KV_Q8) {
             const uint32_t m = 0x7fffffffu;
             top = max(max(__float_as_uint(y.x) & m, __float_as_uint(y.y) & m),
                       max(__float_as_uint(y.z) & m, __float_as_uint(y.w) & m));
+            if (LPH == 32) top = __reduce_max_sync(FULL, top);
+            else
 #pragma unroll
-            for (int z = LPH / 2; z; z >>= 1) top = max(top, __shfl_xor_sync(FULL, top, z));
+                for (int z = LPH / 2; z; z >>= 1) top = max(top, __shfl_xor_sync(FULL, top, z));
         }
-        if (h >= heads || d >= hd) continue;
-        if (h < nq) {
-            *(float4*)(q_out + (size_t)r * ld_qo + (size_t)h * hd + d) = y;
-            continue;
-        }
-        if (page < 0) continue;
-        const int hk = h - nq < nkv ? h - nq : h - nq - nkv;
-        unsigned char* blk = sb_kv_block(c, layer, page, h - nq < nkv ? 0 : 1, hk);
+        if (!in || h >= n) continue;
+        unsigned char* blk = blocks + (size_t)h * bb;
         if (KV == SLATE_KV_F32) {
             *(float4*)((float*)blk + t * hd + d) = y;
         } else if (KV == SLATE_KV_F16) {
@@ -181,13 +194,28 @@ __global__ void __launch_bounds__(256) rope_append_vec(
             *(uint2*)((__half*)blk + t * hd + d) = make_uint2(*(const uint32_t*)&a, *(const uint32_t*)&b);
         } else {
             const float scale = __fmul_rn(__uint_as_float(top), (float)(1.0 / 127.0));
-            const bool plain = scale > 0.f && scale < INFINITY;
-            const auto q8 = [&](float a) {
-                return plain ? (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(a, scale)), -127.f), 127.f) & 255u : 0u;
+            // rint(x / scale): from x * (1 / scale), off by at most 1.5e-5, and the division itself where
+            // that lies as near as 1e-4 to a boundary between two integers (or 1 / scale is no number).
+            // Adding 1.5 * 2^23 rounds to the integer and leaves it in the low byte.
+            const float inv = __frcp_rn(scale);
+            const bool plain = scale > 0.f && scale < INFINITY, fast = plain && inv < INFINITY;
+            const auto near = [&](float a) {
+                const float z = a * inv;
+                return fabsf(fabsf(z - ((z + 12582912.f) - 12582912.f)) - 0.5f) < 1e-4f;
             };
+            const auto divided = [&](float a) {
+                return plain ? (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(a, scale)), -127.f), 127.f) : 0u;
+            };
+            uint32_t q4[4];
+            if (!fast || near(y.x) || near(y.y) || near(y.z) || near(y.w)) {
+                q4[0] = divided(y.x), q4[1] = divided(y.y), q4[2] = divided(y.z), q4[3] = divided(y.w);
+            } else {
+                q4[0] = __float_as_uint(y.x * inv + 12582912.f), q4[1] = __float_as_uint(y.y * inv + 12582912.f);
+                q4[2] = __float_as_uint(y.z * inv + 12582912.f), q4[3] = __float_as_uint(y.w * inv + 12582912.f);
+            }
             if (sub == 0) ((float*)blk)[t] = scale;
             *(uint32_t*)(blk + SB_Q8_SCALES + t * hd + d) =
-                q8(y.x) | q8(y.y) << 8 | q8(y.z) << 16 | q8(y.w) << 24;
+                __byte_perm(__byte_perm(q4[0], q4[1], 0x0040), __byte_perm(q4[2], q4[3], 0x0040), 0x5410);
         }
     }
 }
@@ -416,7 +444,7 @@ extern "C" int slate_cuda_rope_append(const slate_kv_cache_t* cache, int layer,
         return -1;
     }
     if (rows == 0) return 0;
-    const int64_t warps = (int64_t)rows * (n_heads + 2 * nkv);
+    const int64_t warps = (int64_t)rows * (n_heads + 2 * nkv);      // of the scalar kernel, the most
     if ((warps + 7) / 8 > 0x7fffffff) {
         sb_set_error("rope_append: %d rows are too many", rows);
         return -1;
@@ -425,20 +453,30 @@ extern "C" int slate_cuda_rope_append(const slate_kv_cache_t* cache, int layer,
     // vectors need rows and tables on 16 bytes; other strides take the scalar kernel
     if (hd <= 128 && rope->rot_dim % 8 == 0 && al(q) && al(q_out) && al(k) && al(v) && al(rope->cos) &&
         al(rope->sin) && ld_q % 4 == 0 && ld_q_out % 4 == 0 && ld_k % 4 == 0 && ld_v % 4 == 0) {
-        const int lph = hd > 64 ? 32 : hd > 32 ? 16 : 8, at_once = RU * (32 / lph);
-        const int parts = (n_heads + 2 * nkv + at_once - 1) / at_once;
+        const int lph = hd > 64 ? 32 : hd > 32 ? 16 : 8, hpw = 32 / lph, heads = n_heads + 2 * nkv;
+        // RU head groups a warp in flight: four where two would still make a full wave of warps (64 an
+        // SM; 8191 rows of 48 heads: 86 us against 101 with two), else two (16 such rows: 6.9 against 7.5)
+        const int ru = (int64_t)rows * heads / (2 * hpw) > 148 * 64 ? 4 : 2;
+        const int parts_q = (n_heads + ru * hpw - 1) / (ru * hpw);
+        const int parts = parts_q + (2 * nkv + ru * hpw - 1) / (ru * hpw);
         const int64_t n = (int64_t)rows * parts;
         const auto go = [&](auto kernel) {
             kernel<<<(unsigned)((n + 7) / 8), 256, 0, (cudaStream_t)stream>>>(
                 *cache, layer, *rope, rows, n_heads, q_out, ld_q_out, q, ld_q, k, ld_k, v, ld_v, row_slot,
-                row_index, row_pos, parts);
+                row_index, row_pos, parts_q, parts);
         };
-        const auto by_type = [&](auto f32, auto f16, auto q8) {
-            cache->kv_dtype == SLATE_KV_F32 ? go(f32) : cache->kv_dtype == SLATE_KV_F16 ? go(f16) : go(q8);
+        const auto by_type = [&](auto l, auto u) {
+            constexpr int L = decltype(l)::value, U = decltype(u)::value;
+            cache->kv_dtype == SLATE_KV_F32   ? go(rope_append_vec<L, SLATE_KV_F32, U>)
+            : cache->kv_dtype == SLATE_KV_F16 ? go(rope_append_vec<L, SLATE_KV_F16, U>)
+                                              : go(rope_append_vec<L, SLATE_KV_Q8, U>);
         };
-        if (lph == 32) by_type(rope_append_vec<32, SLATE_KV_F32>, rope_append_vec<32, SLATE_KV_F16>, rope_append_vec<32, SLATE_KV_Q8>);
-        else if (lph == 16) by_type(rope_append_vec<16, SLATE_KV_F32>, rope_append_vec<16, SLATE_KV_F16>, rope_append_vec<16, SLATE_KV_Q8>);
-        else by_type(rope_append_vec<8, SLATE_KV_F32>, rope_append_vec<8, SLATE_KV_F16>, rope_append_vec<8, SLATE_KV_Q8>);
+        const auto by_ru = [&](auto l) {
+            ru == 2 ? by_type(l, std::integral_constant<int, 2>{}) : by_type(l, std::integral_constant<int, 4>{});
+        };
+        if (lph == 32) by_ru(std::integral_constant<int, 32>{});
+        else if (lph == 16) by_ru(std::integral_constant<int, 16>{});
+        else by_ru(std::integral_constant<int, 8>{});
         return sb_cuda_check(cudaGetLastError(), "rope_append");
     }
     rope_append_kernel<<<(unsigned)((warps + 7) / 8), 256, 0, (cudaStream_t)stream>>>(
