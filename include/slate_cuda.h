@@ -269,7 +269,7 @@ int slate_cuda_kv_read(const slate_kv_cache_t* cache, int layer0, int n_layers, 
 #define SLATE_TREE_MAX_NODES 64
 typedef struct slate_tree {
     int n_seq, rows;             /* rows = row_off[n_seq] */
-    int max_nodes;               /* of a sequence; picks the kernel, 1..64 */
+    int max_nodes;               /* of a sequence, 1..64; picks the kernel. Attention leaves out nodes beyond */
     const int32_t* row_off;      /* [n_seq + 1] */
     const int32_t* slot;         /* [n_seq] */
     const int32_t* ctx;          /* [n_seq] */

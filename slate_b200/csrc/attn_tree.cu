@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(32 * NW) attn_tree_rows(
     }
     const int r0 = max(tr.row_off[lo], 0), slot = tr.slot[lo];
     const int ctx = min(max(tr.ctx[lo], 0), c.max_pages * SB_PAGE_TOKENS);
-    const int n = min(max(min(tr.row_off[lo + 1], tr.rows) - r0, 0), SLATE_TREE_MAX_NODES);
+    const int n = min(max(min(tr.row_off[lo + 1], tr.rows) - r0, 0), tr.max_nodes);
     const bool in = row >= r0 && row < r0 + n;
     const uint64_t mask = in ? tr.mask[row] : 0;
     const int end = in ? ctx + n : 0;
@@ -132,12 +132,9 @@ __global__ void __launch_bounds__(32 * NW) attn_tree_rows(
 }
 
 // ------------------------------------------------------------ tensor-core path
-#ifndef SB_T0
-#define SB_T0 2
-#endif
-constexpr int MAXC = 4 * SMS;               // CTAs at most
+constexpr int CTAS = 2 * SMS;               // two an SM
 constexpr int UNIT = 64;
-static_assert(MAXC * 32 <= SMS * TC_ROWS, "workspace");
+static_assert(CTAS * 32 <= SMS * TC_ROWS, "workspace");
 constexpr int MW = 4;                       // warps a CTA
 constexpr float DIG = 127.f * 65536.f;      // three digits to base 256 stay within 8 bits each
 
@@ -189,8 +186,7 @@ struct Shape {
     static constexpr int KS = I8 ? HD / 32 : KV == SLATE_KV_F32 ? HD / 8 : HD / 16;    // k steps of a score
     static constexpr int HL = I8 ? MODE + 2 : MODE == 0 ? 1 : 2;    // A operands a k step
     static constexpr int QB = MT * KS * HL * 512;
-    static constexpr int CPS = MODE == 0 ? SB_T0 : 2;                // CTAs an SM
-    static constexpr int NS0 = ((CPS == 2 ? 112 : CPS == 3 ? 74 : 55) * 1024 - QB) / (MW * TB);
+    static constexpr int NS0 = (112 * 1024 - QB) / (MW * TB);
     static constexpr int NS = NS0 > 6 ? 6 : NS0;
     static constexpr int MERGE = MW * MR * (HD + 2) * 4;
     static constexpr int RING = MW * NS * TB > MERGE ? MW * NS * TB : MERGE;
@@ -209,7 +205,7 @@ __device__ __forceinline__ uint32_t swz(int row, int chunk) {
 
 // Partial of one cut item: [MR][HD + 2]: (max in log2 units, sum, o) rows.
 template <int KV, int HD, int MODE>
-__global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_mma(
+__global__ void __launch_bounds__(32 * MW, CTAS / SMS) attn_tree_mma(
     const slate_kv_cache_t c, int layer, const slate_tree_t tr, int nq, float* __restrict__ out,
     int ld_out, const float* __restrict__ q, int ld_q, float scale, float* __restrict__ ws) {
     using S = Shape<KV, HD, MODE>;
@@ -914,10 +910,10 @@ int launch_mma(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int
     static const cudaError_t ready =
         cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (ready != cudaSuccess) return sb_cuda_check(ready, "attention_tree shared memory");
-    const int rc = sb_cuda_check(sb_launch_pdl(k, dim3(S::CPS * SMS), dim3(32 * MW), S::SMEM, st, c, layer, tr, nq, out, ld_out, q,
-                                               ld_q, scale, ws),
+    const int rc = sb_cuda_check(sb_launch_pdl(k, dim3(CTAS), dim3(32 * MW), S::SMEM, st, c, layer, tr, nq, out,
+                                               ld_out, q, ld_q, scale, ws),
                                  "attention_tree");
-    return rc ? rc : join<HD>(c, tr, nq, S::MR, UNIT, S::CPS * SMS, out, ld_out, ws, st);
+    return rc ? rc : join<HD>(c, tr, nq, S::MR, UNIT, CTAS, out, ld_out, ws, st);
 }
 template <int KV, int HD>
 int launch_mode(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq, float* out,
@@ -925,13 +921,14 @@ int launch_mode(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, in
     const int M = tr.max_nodes * (nq / c.n_kv_heads);
     // attn_tree_mma with 32 rows against attn_tree_tc, 16 sequences of 8 nodes x 4 heads over 8000
     // tokens: f16 at head_dim 128 113 and 93 us, at 64 62 and 79, 8 bits at 128 103 and 129
-    if (KV != SLATE_KV_F32 && M > (KV == SLATE_KV_F16 && HD == 128 ? 16 : 32)) {
-        const int rc = attend_tc(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);
-        return rc ? rc : join<HD>(c, tr, nq, TC_ROWS, TC_UNIT, SMS, out, ld_out, ws, st);
-    }
-    return M <= 8    ? launch_mma<KV, HD, 0>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st)
-           : M <= 16 ? launch_mma<KV, HD, 1>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st)
-                     : launch_mma<KV, HD, 2>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);
+    constexpr int few = KV == SLATE_KV_F16 && HD == 128 ? 16 : 32;
+    if (M <= 8) return launch_mma<KV, HD, 0>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);
+    if (M <= 16) return launch_mma<KV, HD, 1>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);
+    if constexpr (few > 16)
+        if (KV == SLATE_KV_F32 || M <= few)
+            return launch_mma<KV, HD, 2>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);
+    const int rc = attend_tc(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);
+    return rc ? rc : join<HD>(c, tr, nq, TC_ROWS, TC_UNIT, SMS, out, ld_out, ws, st);
 }
 bool takes_mma(const slate_kv_cache_t* c) { return c->head_dim == 64 || c->head_dim == 128; }
 
@@ -940,7 +937,7 @@ bool takes_mma(const slate_kv_cache_t* c) { return c->head_dim == 64 || c->head_
 extern "C" size_t slate_cuda_attention_tree_workspace(const slate_kv_cache_t* cache, int n_heads,
                                                       int n_seq, int rows, int max_nodes) {
     if (!cache || n_heads < 1 || n_seq < 1 || rows < 0 || max_nodes < 1) return 0;
-    // two partials for each CTA: 148 of 128 rows, up to 4 * 148 of 32
+    // two partials for each CTA: 148 of 128 rows, or 2 * 148 of 32 at most
     return takes_mma(cache) ? (size_t)2 * SMS * TC_ROWS * (cache->head_dim + 2) * 4 : 16;
 }
 
@@ -951,7 +948,8 @@ extern "C" int slate_cuda_attention_tree(const slate_kv_cache_t* cache, int laye
     if (sb_kv_check(cache, "attention_tree") || sb_tree_check(tree, "attention_tree")) return -1;
     const int hd = cache->head_dim;
     if (layer < 0 || layer >= cache->n_layers || n_heads < 1 || n_heads % cache->n_kv_heads ||
-        n_heads > 65535 || (int64_t)tree->n_seq * tree->max_nodes * n_heads > 0x7fffffff || !out || !q || ld_out < n_heads * hd || ld_q < n_heads * hd ||
+        n_heads > 65535 || (int64_t)tree->n_seq * tree->max_nodes * n_heads > 0x7fffffff || !out || !q ||
+        ld_out < n_heads * hd || ld_q < n_heads * hd ||
         !(fabsf(scale) < INFINITY)) {
         sb_set_error("attention_tree: bad arguments");
         return -1;

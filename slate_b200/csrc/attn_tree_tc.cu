@@ -6,19 +6,20 @@
 // tensor memory.  The cache streams past in tiles of 128 tokens:
 //   S = Qhi K^T + Qlo K^T           128 x 128, in tensor memory, f32
 //   P = exp(S - max), hi and lo     written over S, the next product's A operand
-//   D = Phi V + Plo V               128 x head_dim, in tensor memory
-//   O += D                          in registers, every RUN tiles
+//   D += Phi V + Plo V              128 x head_dim, in tensor memory
+//   O += D, D = 0                   in registers, every RUN tiles or when a maximum grew by 2^LAG
 // S has two buffers: while the softmax warps work on tile j, the tensor cores run P V of
-// tile j - 1 and Q K^T of tile j + 1.  D is drained every tile because an
-// accumulator carried over a long context in the tensor cores would truncate at every step.
-// Warps 0-15: softmax; four threads share a row, each with a quarter of the tile's tokens
-// (they exchange the row's maximum) and of O's dims: the work is mostly latency, and four
-// warps a scheduler hide it where two with twice the row did not.  Warps 16-22 bring K and V
-// page by page in turn into the operands' swizzled layout (f16: 16-byte asynchronous copies;
-// 8 bits: through registers, two pages ahead, widened to f16 on the way).  Warp 23 issues the
-// products.
-// What bounds it: the tensor cores, 2 x the plain formula's products for the two
-// halves, from 64 rows up; the exponentials and splits take nearly as many issue slots.
+// tile j - 1 and Q K^T of tile j + 1.
+// Warps 0-7: softmax; two threads share a row, each with half of the tile's tokens (they
+// exchange the row's maximum) and of O's dims.  Four threads a row hid no more of the latency
+// and left each too few registers.  Warps 8-14 bring K and V page by page in turn into the
+// operands' swizzled layout (f16: 16-byte asynchronous copies; 8 bits: through registers, two
+// pages ahead, widened to f16 on the way).  Warp 15 issues the products.
+// What bounds it.  256 rows and more over long contexts (4 sequences of 64 nodes, 64 heads over
+// 8, 32000 tokens of 8 bits: 466 us, 389 TFLOP/s of the formula, 778 with both halves): the
+// softmax's issue slots, two passes over S with an exponential and a split a score, next to tensor cores that
+// are busy about half of the time.  Few rows (8 sequences of 16 nodes, 32 heads over 8, 8000 tokens
+// of f16: 69 us, 2.3 TB/s): a tile of 64 live rows costs the products of 128.
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -28,10 +29,6 @@
 #include "sb_kv.h"
 #include "sb_pdl.h"
 #include "sb_tree.h"
-
-#ifndef SB_RUN
-#define SB_RUN 8
-#endif
 
 using namespace sb_tree;
 
@@ -47,7 +44,7 @@ constexpr int SCB = 8;                        // tiles whose scales and flags ar
 constexpr int LAG = 8;
 // Tiles that D may add up before it is drained (a power of two).  The tensor cores cut each
 // step's sum off: 8 tiles, 128 steps, cost 1e-6 of the output at worst, one tile 1e-7.
-constexpr int RUN = SB_RUN;
+constexpr int RUN = 8;
 
 template <int KV, int HD>
 struct TcShape {
@@ -245,7 +242,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
     tc_after();
     const uint32_t tmem = tmem_s;
     // Every role walks the same segments; four barriers of the CTA a segment: the last one has
-    // left the buffers, the next is known, q is there, every product is done and the quarter rows'
+    // left the buffers, the next is known, q is there, every product is done and the half rows'
     // sums are there.
     const auto next_segment = [&]() {
         __syncthreads();
@@ -532,6 +529,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
             if (*fail) break;
         }
     } else {
+    // (256 x 144 + 256 x 112 registers are the 512 x 128 that the block starts with)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
     if (warp == NSW + NPW) {
         // ================= products: f32 accumulate, M = 128, N = 128 (scores) or HD (p v);
@@ -591,7 +589,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
         }
     } else {
         // ================= K and V: job n is page n % 8 of K (n / 8 even) or V of tile n / 16;
-        // warp 16 + w takes jobs w, w + 7, ...
+        // warp 8 + w takes jobs w, w + 7, ...
         const int w = warp - NSW;
         while (next_segment()) {
             const int nt = sg.nt, kvh = sg.kvh, tok0 = sg.tok0, end = sg.end, ctx = sg.sq.ctx, slot = sg.sq.slot;

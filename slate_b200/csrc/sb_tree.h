@@ -34,7 +34,7 @@ __device__ __forceinline__ Seq seq_of(const slate_kv_cache_t& c, const slate_tre
     Seq q;
     q.s = s;
     q.r0 = max(__ldg(tr.row_off + s), 0);
-    q.n = min(max(min(__ldg(tr.row_off + s + 1), tr.rows) - q.r0, 0), SLATE_TREE_MAX_NODES);
+    q.n = min(max(min(__ldg(tr.row_off + s + 1), tr.rows) - q.r0, 0), tr.max_nodes);
     q.slot = __ldg(tr.slot + s);
     q.ctx = min(max(__ldg(tr.ctx + s), 0), c.max_pages * SB_PAGE_TOKENS);
     q.tiles = (q.n * G + MR - 1) / MR;
