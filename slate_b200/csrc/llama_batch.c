@@ -771,6 +771,10 @@ slate_llama_batch_t* slate_llama_batch_new_desc(const slate_llama_desc_t* m,
         sb_set_error("max_batch %d out of range", o->max_batch);
         return NULL;
     }
+    if (o->kv_dtype == SLATE_KV_Q8) {
+        sb_set_error("the engine keeps an f32 or f16 cache; 8 bits are for the cache operators");
+        return NULL;
+    }
     const int tp = o->tp_size > 1 ? o->tp_size : 1, rank = tp > 1 ? o->tp_rank : 0;
     if (tp > 1) {
         /* column slices of Wo (K = nq*hd) and down (K = F) must stay whole
