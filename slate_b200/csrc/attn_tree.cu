@@ -836,16 +836,16 @@ __global__ void __launch_bounds__(32 * MW, CTAS / SMS) attn_tree_mma(
     }
 }
 
-// Joins the partials of the cut items: one CTA a (sequence, kv head, `rpc` rows), a warp a
-// row: lane i forms the weight of record i, then the lanes sum their dims over the records,
-// eight loads in flight.
-template <int HD>
-__global__ void __launch_bounds__(128) attn_tree_join(const slate_kv_cache_t c, const slate_tree_t tr,
-                                                      int nq, int MR, int unit, int ctas, int rpc,
-                                                      float* __restrict__ out, int ld_out,
-                                                      const float* __restrict__ ws) {
+// Joins the partials of the cut items: a CTA a (sequence, kv head, `rpc` rows), W warps a row,
+// each with every W-th record: lane i forms the weight of the warp's record i, then the lanes
+// sum their dims over the records, eight records in flight.  The loads' latency is what bounds it.
+template <int HD, int W>
+__global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) attn_tree_join(
+    const slate_kv_cache_t c, const slate_tree_t tr, int nq, int MR, int unit, int ctas, int rpc,
+    float* __restrict__ out, int ld_out, const float* __restrict__ ws) {
     constexpr int E = HD / 32;                           // dims a lane: 2 or 4
     __shared__ PlanBuf buf;
+    __shared__ float sm[W], sl[W], so[W][HD];
     const int nkv = c.n_kv_heads, G = nq / nkv, tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
     const int chunks = (tr.max_nodes * G + rpc - 1) / rpc, s = blockIdx.x / chunks, kvh = blockIdx.y;
     // no early release: the next call's CTAs have to find the SMs empty, all of them at once
@@ -854,8 +854,8 @@ __global__ void __launch_bounds__(128) attn_tree_join(const slate_kv_cache_t c, 
     const int64_t total = plan_of(c, tr, G, MR, unit, s, buf, q, before);
     const Cut cut(total, ctas);
     sb_grid_wait();        // the partials; before any return, so that the chain stays ordered
-    const int row0 = blockIdx.x % chunks * rpc;
-    for (int row = row0 + warp; row < min(row0 + rpc, q.n * G); row += 4) {
+    const int row0 = blockIdx.x % chunks * rpc, w = W == 1 ? 0 : warp;
+    for (int row = row0 + (W == 1 ? warp : 0); row < min(row0 + rpc, q.n * G); row += W == 1 ? 4 : 1) {
         const int64_t first = before + (int64_t)(kvh * q.tiles + row / MR) * q.units;
         const int c0 = cut.owner(first), n = cut.owner(first + q.units - 1) - c0 + 1;
         if (n == 1) continue;                            // written by its CTA
@@ -864,42 +864,84 @@ __global__ void __launch_bounds__(128) attn_tree_join(const slate_kv_cache_t c, 
         const float* base = ws + (size_t)2 * c0 * rec + (size_t)(row % MR) * (HD + 2);
         const size_t late = cut.first(c0) < first ? rec : 0;
         float M = -INFINITY, L = 0.f, O[E];
-        for (int i = lane; i < n; i += 32) M = fmaxf(M, base[2 * i * rec + (i ? 0 : late)]);
+        for (int i = w + W * lane; i < n; i += 32 * W) M = fmaxf(M, base[2 * i * rec + (i ? 0 : late)]);
         for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(FULL, M, x));
 #pragma unroll
         for (int k = 0; k < E; ++k) O[k] = 0.f;
-        for (int i0 = 0; i0 < n; i0 += 32) {
+        for (int i0 = w; i0 < n; i0 += 32 * W) {
             float f = 0.f;
-            if (i0 + lane < n) {
-                const float2 ml = *(const float2*)(base + 2 * (i0 + lane) * rec + (i0 + lane ? 0 : late));
+            if (i0 + W * lane < n) {
+                const int i = i0 + W * lane;
+                const float2 ml = *(const float2*)(base + 2 * i * rec + (i ? 0 : late));
                 f = ml.x == -INFINITY ? 1.f : ex2(ml.x - M);
                 L = fmaf(ml.y, f, L);
             }
-#pragma unroll 8
-            for (int i = 0; i < min(n - i0, 32); ++i) {
-                const float w = __shfl_sync(FULL, f, i);
-                const float* o = base + 2 * (i0 + i) * rec + (i0 + i ? 0 : late) + 2 + E * lane;
+            for (int j0 = 0; j0 < 32 && i0 + W * j0 < n; j0 += 8) {
+                float2 y[8][E / 2];
 #pragma unroll
-                for (int k = 0; k < E; k += 2) {
-                    const float2 y = *(const float2*)(o + k);
-                    O[k] = fmaf(y.x, w, O[k]);
-                    O[k + 1] = fmaf(y.y, w, O[k + 1]);
+                for (int u = 0; u < 8; ++u) {
+                    const int i = i0 + W * (j0 + u);
+                    if (i >= n) break;
+#pragma unroll
+                    for (int k = 0; k < E / 2; ++k)
+                        y[u][k] = *(const float2*)(base + 2 * i * rec + (i ? 0 : late) + 2 + E * lane + 2 * k);
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    if (i0 + W * (j0 + u) >= n) break;
+                    const float v = __shfl_sync(FULL, f, j0 + u);
+#pragma unroll
+                    for (int k = 0; k < E / 2; ++k) {
+                        O[2 * k] = fmaf(y[u][k].x, v, O[2 * k]);
+                        O[2 * k + 1] = fmaf(y[u][k].y, v, O[2 * k + 1]);
+                    }
                 }
             }
         }
         for (int x = 16; x; x >>= 1) L += __shfl_xor_sync(FULL, L, x);
-        float* o = out + (size_t)(q.r0 + row / G) * ld_out + (size_t)(kvh * G + row % G) * HD + E * lane;
+        float* o = out + (size_t)(q.r0 + row / G) * ld_out + (size_t)(kvh * G + row % G) * HD;
+        if (W == 1) {
 #pragma unroll
-        for (int k = 0; k < E; ++k) o[k] = L == 0.f ? 0.f : O[k] / L;
+            for (int k = 0; k < E; ++k) o[E * lane + k] = L == 0.f ? 0.f : O[k] / L;
+            continue;
+        }
+        // (one row a CTA: nothing of a row before it is still read)
+        if (lane == 0) {
+            sm[w] = M;
+            sl[w] = L;
+        }
+#pragma unroll
+        for (int k = 0; k < E; ++k) so[w][E * lane + k] = O[k];
+        __syncthreads();
+        if (tid >= HD) return;
+        M = -INFINITY, L = 0.f;
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) M = fmaxf(M, sm[i]);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const float f = sm[i] == -INFINITY ? 1.f : ex2(sm[i] - M);
+            L = fmaf(sl[i], f, L);
+            x = fmaf(so[i][tid], f, x);
+        }
+        o[tid] = L == 0.f ? 0.f : x / L;
     }
 }
 
 template <int HD>
 int join(const slate_kv_cache_t& c, const slate_tree_t& tr, int nq, int MR, int unit, int ctas, float* out, int ld_out,
          const float* ws, cudaStream_t st) {
-    const int R = tr.max_nodes * (nq / c.n_kv_heads), rpc = R >= 128 ? 16 : 4;
+    const int R = tr.max_nodes * (nq / c.n_kv_heads);
+    // eight warps a row where an item, if long, is cut into eight records or more: one token over 3000
+    // tokens of 8 heads 13.5 us against 18.7 with a warp a row (whole calls); more items than that fill
+    // the GPU with a warp a row
+    if ((int64_t)tr.n_seq * c.n_kv_heads * ((R + MR - 1) / MR) * 8 <= ctas)
+        return sb_cuda_check(sb_launch_pdl(attn_tree_join<HD, 8>, dim3((unsigned)(tr.n_seq * R), (unsigned)c.n_kv_heads), dim3(256), 0,
+                                           st, c, tr, nq, MR, unit, ctas, 1, out, ld_out, ws),
+                             "attention_tree join");
+    const int rpc = R >= 128 ? 16 : 4;
     const dim3 grid((unsigned)(tr.n_seq * ((R + rpc - 1) / rpc)), (unsigned)c.n_kv_heads);
-    return sb_cuda_check(sb_launch_pdl(attn_tree_join<HD>, grid, dim3(128), 0, st, c, tr, nq, MR, unit, ctas, rpc, out, ld_out, ws),
+    return sb_cuda_check(sb_launch_pdl(attn_tree_join<HD, 1>, grid, dim3(128), 0, st, c, tr, nq, MR, unit, ctas, rpc, out, ld_out, ws),
                          "attention_tree join");
 }
 template <int KV, int HD, int MODE>
