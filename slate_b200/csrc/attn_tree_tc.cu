@@ -55,6 +55,7 @@ struct TcShape {
     static constexpr int TB = KT * HD * 2;                 // a K or V tile in f16
     static constexpr int SC = SCB * 2 * KT * 4;
     static constexpr int SMEM = 2 * NB * TB + SC + 1024;
+    static_assert(MR * (HD + 1) * 4 <= 2 * NB * TB, "q and O pass through the tiles");
 };
 
 struct Yes {
@@ -271,11 +272,29 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
             const int h = warp >> 2, r = tid & 127;
             const bool live = (warp & 3) * 32 < n_rows;                 // of the warp
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-            const int row = r_base + min(r, n_rows - 1);
             // ---- q, each row divided by the power of two below its maximum; scale's sign joins q
+            // ---- (a row at a time through the K and V tiles, which nobody else uses yet: a thread that
+            // read its own row would ask for a sector an element)
             float O[HO];
             {
-                const float* x = q + (size_t)(sq_.r0 + row / G) * ld_q + (size_t)(kvh * G + row % G) * HD + HO * h;
+                float* stage = (float*)skv;
+                for (int i0 = warp; i0 < n_rows; i0 += 4 * NSW) {
+                    float x[4][HD / 32];               // four rows in flight
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int rr = r_base + min(i0 + u * NSW, n_rows - 1);
+                        const float* src = q + (size_t)(sq_.r0 + rr / G) * ld_q + (size_t)(kvh * G + rr % G) * HD + lane;
+#pragma unroll
+                        for (int k = 0; k < HD / 32; ++k) x[u][k] = src[32 * k];
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+#pragma unroll
+                        for (int k = 0; k < HD / 32; ++k)
+                            if (i0 + u * NSW < n_rows) stage[(i0 + u * NSW) * (HD + 1) + lane + 32 * k] = x[u][k];
+                }
+                softmax_sync();
+                const float* x = stage + min(r, n_rows - 1) * (HD + 1) + HO * h;
                 uint32_t top = 0;
 #pragma unroll
                 for (int i = 0; i < HO; ++i) {
@@ -508,23 +527,23 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
 #pragma unroll
                 for (int i = 1; i < PARTS; ++i) L += part_max[0][i][r];
                 const float bad = *fail ? NAN : 0.f;   // a wait ran out: no number may pass for a result
-                float* o = sg.whole ? out + (size_t)(sq_.r0 + row / G) * ld_out + (size_t)(kvh * G + row % G) * HD + HO * h
-                                    : ws + ((size_t)(2 * blockIdx.x + (sg.seg ? 1 : 0)) * MR + r) * (HD + 2) + 2 + HO * h;
                 if (!sg.whole && h == 0) {
-                    o[-2] = Q8 ? m + (float)vexp : m;  // 2^up of another part may differ
-                    o[-1] = L + bad;
+                    float* o = ws + ((size_t)(2 * blockIdx.x + (sg.seg ? 1 : 0)) * MR + r) * (HD + 2);
+                    o[0] = Q8 ? m + (float)vexp : m;   // 2^up of another part may differ
+                    o[1] = L + bad;
                 }
                 const float f = (sg.whole ? (L == 0.f ? 0.f : 1.f / L) : 1.f); // l and o carry the same power of two
+                float* x = (float*)skv + r * (HD + 1) + HO * h;
 #pragma unroll
-                for (int i = 0; i < HO; i += 2) {
-                    const float2 y = make_float2(O[i] * f + bad, O[i + 1] * f + bad);
-                    if (sg.whole) {
-                        o[i] = y.x;
-                        o[i + 1] = y.y;
-                    } else {
-                        *(float2*)(o + i) = y;
-                    }
-                }
+                for (int i = 0; i < HO; ++i) x[i] = O[i] * f + bad;
+            }
+            softmax_sync();
+            for (int i = warp; i < n_rows; i += NSW) { // through the tiles again, a row at a time
+                const int rr = r_base + i;
+                float* o = sg.whole ? out + (size_t)(sq_.r0 + rr / G) * ld_out + (size_t)(kvh * G + rr % G) * HD
+                                    : ws + ((size_t)(2 * blockIdx.x + (sg.seg ? 1 : 0)) * MR + i) * (HD + 2) + 2;
+#pragma unroll
+                for (int k = 0; k < HD / 32; ++k) o[lane + 32 * k] = ((const float*)skv)[i * (HD + 1) + lane + 32 * k];
             }
             if (*fail) break;
         }
