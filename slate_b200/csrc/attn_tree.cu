@@ -175,6 +175,9 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
 // chunk each) nor the f32 reads (4 or 8 rows) meet in a bank.
 template <int KV, int HD, int MODE>
 struct Shape {
+    // (f32: a unit's arithmetic takes longer than what a second range costs; 16 x 7 nodes over 1501
+    // tokens 43.2 us, with 2 45.4)
+    static constexpr int SLACK = KV == SLATE_KV_F32 ? 1 : 4;
     static constexpr int RB = KV == SLATE_KV_F32 ? 4 * HD : KV == SLATE_KV_F16 ? 2 * HD : HD;
     static constexpr int KT = RB == 512 ? 8 : RB == 256 ? 16 : 32;
     static constexpr int CPR = RB / 16;
@@ -224,7 +227,8 @@ __global__ void __launch_bounds__(32 * MW, CTAS / SMS) attn_tree_mma(
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     const int nkv = c.n_kv_heads, G = nq / nkv;
     Start st_;
-    if (!plan_start(c, tr, G, MR, UNIT, gridDim.x, buf, st_)) return;
+    int unit = UNIT;
+    if (!plan_start(c, tr, G, MR, unit, S::SLACK, gridDim.x, buf, st_)) return;
     int64_t at = st_.at, seq_before = st_.seq_before;
     const int64_t stop = st_.stop;
     Seq sq_ = st_.sq;
@@ -236,14 +240,14 @@ __global__ void __launch_bounds__(32 * MW, CTAS / SMS) attn_tree_mma(
     for (int seg = 0; at < stop; ++seg) {
         while (at >= seq_before + seq_units(sq_, nkv)) {
             seq_before += seq_units(sq_, nkv);
-            sq_ = seq_of(c, tr, ++s, G, MR, UNIT);
+            sq_ = seq_of(c, tr, ++s, G, MR, unit);
         }
         const uint32_t rel = (uint32_t)(at - seq_before);     // < 2^31: 2^24 tokens of 64 rows a head at most
         const int item = (int)(rel / (uint32_t)sq_.units), u0 = (int)(rel % (uint32_t)sq_.units);
         const int u1 = (int)min((int64_t)sq_.units, u0 + (stop - at));
         const int kvh = item / sq_.tiles, r_base = (item % sq_.tiles) * MR;
         const int n_rows = min(MR, sq_.n * G - r_base);
-        const int end = sq_.ctx + sq_.n, tok0 = u0 * UNIT, tok1 = min(end, u1 * UNIT);
+        const int end = sq_.ctx + sq_.n, tok0 = u0 * unit, tok1 = min(end, u1 * unit);
         at += u1 - u0;
 
         // ---- q as A fragments, each row divided by the power of two below its maximum
@@ -841,7 +845,7 @@ __global__ void __launch_bounds__(32 * MW, CTAS / SMS) attn_tree_mma(
 // sum their dims over the records, eight records in flight.  The loads' latency is what bounds it.
 template <int HD, int W>
 __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) attn_tree_join(
-    const slate_kv_cache_t c, const slate_tree_t tr, int nq, int MR, int unit, int ctas, int rpc,
+    const slate_kv_cache_t c, const slate_tree_t tr, int nq, int MR, int unit, int slack, int ctas, int rpc,
     float* __restrict__ out, int ld_out, const float* __restrict__ ws) {
     constexpr int E = HD / 32;                           // dims a lane: 2 or 4
     __shared__ PlanBuf buf;
@@ -851,7 +855,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) attn_tree_join(
     // no early release: the next call's CTAs have to find the SMs empty, all of them at once
     Seq q;
     int64_t before;
-    const int64_t total = plan_of(c, tr, G, MR, unit, s, buf, q, before);
+    const int64_t total = plan_of(c, tr, G, MR, unit, slack, ctas, s, buf, q, before);
     const Cut cut(total, ctas);
     sb_grid_wait();        // the partials; before any return, so that the chain stays ordered
     const int row0 = blockIdx.x % chunks * rpc, w = W == 1 ? 0 : warp;
@@ -929,19 +933,20 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) attn_tree_join(
 }
 
 template <int HD>
-int join(const slate_kv_cache_t& c, const slate_tree_t& tr, int nq, int MR, int unit, int ctas, float* out, int ld_out,
-         const float* ws, cudaStream_t st) {
+int join(const slate_kv_cache_t& c, const slate_tree_t& tr, int nq, int MR, int unit, int slack, int ctas, float* out,
+         int ld_out, const float* ws, cudaStream_t st) {
     const int R = tr.max_nodes * (nq / c.n_kv_heads);
     // eight warps a row where an item, if long, is cut into eight records or more: one token over 3000
     // tokens of 8 heads 13.5 us against 18.7 with a warp a row (whole calls); more items than that fill
     // the GPU with a warp a row
     if ((int64_t)tr.n_seq * c.n_kv_heads * ((R + MR - 1) / MR) * 8 <= ctas)
         return sb_cuda_check(sb_launch_pdl(attn_tree_join<HD, 8>, dim3((unsigned)(tr.n_seq * R), (unsigned)c.n_kv_heads), dim3(256), 0,
-                                           st, c, tr, nq, MR, unit, ctas, 1, out, ld_out, ws),
+                                           st, c, tr, nq, MR, unit, slack, ctas, 1, out, ld_out, ws),
                              "attention_tree join");
     const int rpc = R >= 128 ? 16 : 4;
     const dim3 grid((unsigned)(tr.n_seq * ((R + rpc - 1) / rpc)), (unsigned)c.n_kv_heads);
-    return sb_cuda_check(sb_launch_pdl(attn_tree_join<HD, 1>, grid, dim3(128), 0, st, c, tr, nq, MR, unit, ctas, rpc, out, ld_out, ws),
+    return sb_cuda_check(sb_launch_pdl(attn_tree_join<HD, 1>, grid, dim3(128), 0, st, c, tr, nq, MR, unit, slack, ctas, rpc, out,
+                                       ld_out, ws),
                          "attention_tree join");
 }
 template <int KV, int HD, int MODE>
@@ -955,7 +960,7 @@ int launch_mma(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int
     const int rc = sb_cuda_check(sb_launch_pdl(k, dim3(CTAS), dim3(32 * MW), S::SMEM, st, c, layer, tr, nq, out,
                                                ld_out, q, ld_q, scale, ws),
                                  "attention_tree");
-    return rc ? rc : join<HD>(c, tr, nq, S::MR, UNIT, CTAS, out, ld_out, ws, st);
+    return rc ? rc : join<HD>(c, tr, nq, S::MR, UNIT, S::SLACK, CTAS, out, ld_out, ws, st);
 }
 template <int KV, int HD>
 int launch_mode(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq, float* out,
@@ -970,7 +975,7 @@ int launch_mode(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, in
         if (KV == SLATE_KV_F32 || M <= few)
             return launch_mma<KV, HD, 2>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);
     const int rc = attend_tc(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);
-    return rc ? rc : join<HD>(c, tr, nq, TC_ROWS, TC_UNIT, SMS, out, ld_out, ws, st);
+    return rc ? rc : join<HD>(c, tr, nq, TC_ROWS, TC_UNIT, TC_SLACK, SMS, out, ld_out, ws, st);
 }
 bool takes_mma(const slate_kv_cache_t* c) { return c->head_dim == 64 || c->head_dim == 128; }
 

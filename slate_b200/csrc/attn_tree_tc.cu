@@ -157,27 +157,27 @@ __device__ __forceinline__ uint32_t op_at(int r, int ch) {
 // thread: the roles have no registers to spare for it.
 struct Segs {
     int64_t at, stop, seq_before;
-    int s, seg;
+    int s, seg, unit;                   // unit: in tokens, a multiple of KT
     Seq sq;
-    int u0, nt, kvh, r_base, n_rows, end, tok0;
+    int nt, kvh, r_base, n_rows, end, tok0;
     bool whole;
     __device__ __forceinline__ bool next(const slate_kv_cache_t& c, const slate_tree_t& tr, int G) {
         if (at >= stop) return false;
         while (at >= seq_before + seq_units(sq, c.n_kv_heads)) {
             seq_before += seq_units(sq, c.n_kv_heads);
-            sq = seq_of(c, tr, ++s, G, MR, KT);
+            sq = seq_of(c, tr, ++s, G, MR, unit);
         }
         const uint32_t rel = (uint32_t)(at - seq_before);
         const int item = (int)(rel / (uint32_t)sq.units);
-        u0 = (int)(rel % (uint32_t)sq.units);
-        nt = (int)min((int64_t)sq.units, u0 + (stop - at)) - u0;
+        const int u0 = (int)(rel % (uint32_t)sq.units), nu = (int)min((int64_t)sq.units, u0 + (stop - at)) - u0;
         kvh = item / sq.tiles;
         r_base = (item % sq.tiles) * MR;
         n_rows = min(MR, sq.n * G - r_base);
         end = sq.ctx + sq.n;
-        tok0 = u0 * KT;
-        whole = nt == sq.units;
-        at += nt;
+        tok0 = u0 * unit;
+        nt = (min(end - tok0, nu * unit) + KT - 1) / KT;
+        whole = nu == sq.units;
+        at += nu;
         ++seg;
         return true;
     }
@@ -211,7 +211,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int nkv = c.n_kv_heads, G = nq / nkv;
     Start st_;
-    if (!plan_start(c, tr, G, MR, KT, gridDim.x, buf, st_)) return;
+    int unit = KT;
+    if (!plan_start(c, tr, G, MR, unit, TC_SLACK, gridDim.x, buf, st_)) return;
     if (tid == 0) {
         for (int i = 0; i < NB; ++i) {
             bar_init(&bars.kfull[i], 8);          // pages
@@ -229,6 +230,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
         sg.at = st_.at;
         sg.stop = st_.stop;
         sg.seg = -1;
+        sg.unit = unit;
         sg.s = st_.sq.s;
         sg.seq_before = st_.seq_before;
         sg.sq = st_.sq;

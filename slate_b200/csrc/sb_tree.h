@@ -24,7 +24,8 @@ constexpr int SMS = 148;
 // of MR rows), its work ceil(tokens / unit) units; the items' units in order are
 // cut into as many equal ranges as there are CTAs.  A CTA that holds the whole of
 // an item writes its output; of a cut item each CTA leaves a partial (max, sum, o)
-// for attn_tree_join.  Contexts of any lengths thereby load every SM alike.
+// for attn_tree_join.  Contexts of any lengths thereby load every SM alike.  With few items the
+// unit grows (below), so that a CTA has one range of one item and starts once.
 struct Seq {
     int s, r0, n, slot, ctx;      // rows r0 .. r0 + n - 1
     int tiles, units;             // row tiles a head; units an item
@@ -129,11 +130,28 @@ __device__ __forceinline__ Seq seq_from(const Seq& q, int lane) {
     r.units = __shfl_sync(FULL, q.units, lane);
     return r;
 }
+// A second range costs a CTA about `slack` units (q, the first tile's latency, O): a unit of T
+// units, T up to `slack` more than the even share, is taken if that leaves a CTA one range.
+// 8 x 16 nodes over 8000 tokens of f16: 54 us against 60 with even ranges (slack 4; 16 made 20000
+// tokens slower, 140 against 131); one token over 3000 of 8 bits: 9.9 against 13.6.
 __device__ __forceinline__ int64_t plan_warp(const slate_kv_cache_t& c, const slate_tree_t& tr, int G, int MR,
-                                             int unit, Seq& q, int64_t& before) {
+                                             int& unit, int slack, int ctas, Seq& q, int64_t& before) {
     const int lane = threadIdx.x & 31;
     q = seq_of(c, tr, min(lane, tr.n_seq - 1), G, MR, unit);
-    const int64_t mine = lane < tr.n_seq ? seq_units(q, c.n_kv_heads) : 0;
+    int64_t mine = lane < tr.n_seq ? seq_units(q, c.n_kv_heads) : 0;
+    const uint32_t sum = __reduce_add_sync(FULL, (uint32_t)min(mine, (int64_t)1 << 26));
+    if (sum > (uint32_t)ctas) {
+        const uint32_t items = mine ? min((uint32_t)(q.tiles * c.n_kv_heads), 1000u) : 0;
+        const uint32_t even = (sum + ctas - 1) / ctas;
+        for (uint32_t T = even; T <= even + slack; ++T) {
+            const uint32_t n = (q.units + T - 1) / T;
+            if (__reduce_add_sync(FULL, items * min(n, 1000u)) > (uint32_t)ctas) continue;
+            unit *= T;
+            q.units = (int)n;
+            mine = (int64_t)items * n;
+            break;
+        }
+    }
     int64_t incl = mine;
     for (int o = 1; o < 32; o <<= 1) {
         const int64_t x = __shfl_up_sync(FULL, incl, o);
@@ -142,12 +160,12 @@ __device__ __forceinline__ int64_t plan_warp(const slate_kv_cache_t& c, const sl
     before = incl - mine;
     return __shfl_sync(FULL, incl, 31);
 }
-__device__ __forceinline__ bool plan_start(const slate_kv_cache_t& c, const slate_tree_t& tr, int G, int MR, int unit,
-                                           int ctas, PlanBuf& buf, Start& st) {
+__device__ __forceinline__ bool plan_start(const slate_kv_cache_t& c, const slate_tree_t& tr, int G, int MR, int& unit,
+                                           int slack, int ctas, PlanBuf& buf, Start& st) {
     int64_t before;
     if (tr.n_seq <= 32) {
         Seq q;
-        const int64_t total = plan_warp(c, tr, G, MR, unit, q, before);
+        const int64_t total = plan_warp(c, tr, G, MR, unit, slack, ctas, q, before);
         const Cut cut(total, ctas);
         if ((int)blockIdx.x >= cut.C) return false;
         st.at = cut.first(blockIdx.x);
@@ -170,11 +188,11 @@ __device__ __forceinline__ bool plan_start(const slate_kv_cache_t& c, const slat
 }
 // Sequence s, the units before it, and the total.
 __device__ __forceinline__ int64_t plan_of(const slate_kv_cache_t& c, const slate_tree_t& tr, int G, int MR, int unit,
-                                           int s, PlanBuf& buf, Seq& sq, int64_t& before) {
+                                           int slack, int ctas, int s, PlanBuf& buf, Seq& sq, int64_t& before) {
     if (tr.n_seq <= 32) {
         Seq q;
         int64_t b;
-        const int64_t total = plan_warp(c, tr, G, MR, unit, q, b);
+        const int64_t total = plan_warp(c, tr, G, MR, unit, slack, ctas, q, b);
         sq = seq_from(q, s);
         before = __shfl_sync(FULL, b, s);
         return total;
@@ -229,7 +247,7 @@ __device__ __forceinline__ uint32_t i8_f16(uint32_t w) {
 
 // attn_tree_tc.cu: rows in tiles of TC_ROWS, units of TC_UNIT tokens, SMS CTAs; two
 // partials of TC_ROWS x (head_dim + 2) floats for each in ws.
-constexpr int TC_ROWS = 128, TC_UNIT = 128;
+constexpr int TC_ROWS = 128, TC_UNIT = 128, TC_SLACK = 4;
 int attend_tc(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq, float* out, int ld_out,
               const float* q, int ld_q, float scale, float* ws, cudaStream_t st);
 
