@@ -429,25 +429,30 @@ __global__ void __launch_bounds__(32 * MW, CTAS / SMS) attn_tree_mma(
 #pragma unroll
                             for (int h = 0; h < S::HL; ++h)
                                 A[a][k][h] = sq[((size_t)(a * KS + 2 * cc + k) * S::HL + h) * 32 + lane];
+                    uint32_t bh[NTK][4], bl[NTK][4];
 #pragma unroll
                     for (int j = 0; j < NTK; ++j) {
                         const float4 x = *(const float4*)(st + swz<KV, RB>(8 * j + g, 4 * cc + t4));
-                        uint32_t bh[4], bl[4];
-                        split_tf32(x.x, bh[0], bl[0]);
-                        split_tf32(x.y, bh[1], bl[1]);
-                        split_tf32(x.z, bh[2], bl[2]);
-                        split_tf32(x.w, bh[3], bl[3]);
-#pragma unroll
-                        for (int k = 0; k < 2; ++k)
-#pragma unroll
-                            for (int a = 0; a < MT; ++a) {
-                                const uint4 h4 = A[a][k][0], l4 = A[a][k][S::HL - 1];
-                                const uint32_t ah[4] = {h4.x, h4.y, h4.z, h4.w}, al[4] = {l4.x, l4.y, l4.z, l4.w};
-                                mma_tf32(sx[a][j], ah, bl[2 * k], bl[2 * k + 1]);
-                                if (MODE) mma_tf32(sx[a][j], al, bh[2 * k], bh[2 * k + 1]);
-                                mma_tf32(sc[a][j], ah, bh[2 * k], bh[2 * k + 1]);
-                            }
+                        split_tf32(x.x, bh[j][0], bl[j][0]);
+                        split_tf32(x.y, bh[j][1], bl[j][1]);
+                        split_tf32(x.z, bh[j][2], bl[j][2]);
+                        split_tf32(x.w, bh[j][3], bl[j][3]);
                     }
+                    // (a sum's next product stands behind those of the other sums)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int z = 0; z < 3; ++z)        // hi lo, hi hi, lo hi
+#pragma unroll
+                            for (int j = 0; j < NTK; ++j)
+#pragma unroll
+                                for (int a = 0; a < MT; ++a) {
+                                    const uint4 q4 = A[a][k][z < 2 ? 0 : S::HL - 1];
+                                    const uint32_t aq[4] = {q4.x, q4.y, q4.z, q4.w};
+                                    if (z == 0) mma_tf32(sx[a][j], aq, bl[j][2 * k], bl[j][2 * k + 1]);
+                                    if (z == 1) mma_tf32(sc[a][j], aq, bh[j][2 * k], bh[j][2 * k + 1]);
+                                    if (z == 2 && MODE) mma_tf32(sx[a][j], aq, bh[j][2 * k], bh[j][2 * k + 1]);
+                                }
                 }
 #pragma unroll
                 for (int a = 0; a < MT; ++a)
@@ -511,20 +516,24 @@ __global__ void __launch_bounds__(32 * MW, CTAS / SMS) attn_tree_mma(
                         uint32_t r[4];
                         ldsm4(ks_ + swz<KV, RB>(16 * jp + (lane >> 4) * 8 + (lane & 7), 2 * cc + ((lane >> 3) & 1)), r);
 #pragma unroll
-                        for (int jj = 0; jj < 2; ++jj)
+                        for (int k = 0; k < KPL; ++k) {
+                            uint32_t b[2][2];
 #pragma unroll
-                            for (int k = 0; k < KPL; ++k) {
-                                const uint32_t b0 = KV == SLATE_KV_Q8 ? i8_f16<0x4140>(r[2 * jj + k]) : r[2 * jj];
-                                const uint32_t b1 = KV == SLATE_KV_Q8 ? i8_f16<0x4342>(r[2 * jj + k]) : r[2 * jj + 1];
+                            for (int jj = 0; jj < 2; ++jj) {
+                                b[jj][0] = KV == SLATE_KV_Q8 ? i8_f16<0x4140>(r[2 * jj + k]) : r[2 * jj];
+                                b[jj][1] = KV == SLATE_KV_Q8 ? i8_f16<0x4342>(r[2 * jj + k]) : r[2 * jj + 1];
+                            }
 #pragma unroll
-                                for (int a = 0; a < MT; ++a)
+                            for (int h = S::HL - 1; h >= 0; --h)
 #pragma unroll
-                                    for (int h = S::HL - 1; h >= 0; --h) {
+                                for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+                                    for (int a = 0; a < MT; ++a) {
                                         const uint4 x = A[a][k][h];
                                         const uint32_t af[4] = {x.x, x.y, x.z, x.w};
-                                        mma_f16(sc[a][2 * jp + jj], af, b0, b1);
+                                        mma_f16(sc[a][2 * jp + jj], af, b[jj][0], b[jj][1]);
                                     }
-                            }
+                        }
                     }
                 }
             }
@@ -655,34 +664,42 @@ __global__ void __launch_bounds__(32 * MW, CTAS / SMS) attn_tree_mma(
                                 split_tf32(p[(2 * a + 1) % RI][j][e], ph[a][j][2 * e + 1], pl[a][j][2 * e + 1]);
                             }
 #pragma unroll
-                for (int jd = 0; jd < NTD; ++jd) {
-                    float d[MT][4];
-                    uint32_t bh[NTK][2], bl[NTK][2];
+                for (int jd = 0; jd < NTD; jd += 2) {
+                    float d[2][MT][4];
+                    uint32_t bh[2][NTK][2], bl[2][NTK][2];
 #pragma unroll
-                    for (int a = 0; a < MT; ++a) d[a][0] = d[a][1] = d[a][2] = d[a][3] = 0.f;
+                    for (int x = 0; x < 2; ++x) {
 #pragma unroll
-                    for (int j = 0; j < NTK; ++j) {
-                        // k = t4 is token 2 t4, k = t4 + 4 token 2 t4 + 1 of the 8
-                        const int r = 8 * j + 2 * t4, ch = 2 * jd + (g >> 2);
-                        split_tf32(*(const float*)(st + KT * RB + swz<KV, RB>(r, ch) + 4 * (g & 3)), bh[j][0], bl[j][0]);
-                        split_tf32(*(const float*)(st + KT * RB + swz<KV, RB>(r + 1, ch) + 4 * (g & 3)), bh[j][1], bl[j][1]);
+                        for (int a = 0; a < MT; ++a) d[x][a][0] = d[x][a][1] = d[x][a][2] = d[x][a][3] = 0.f;
+#pragma unroll
+                        for (int j = 0; j < NTK; ++j) {
+                            // k = t4 is token 2 t4, k = t4 + 4 token 2 t4 + 1 of the 8
+                            const int r = 8 * j + 2 * t4, ch = 2 * (jd + x) + (g >> 2);
+                            split_tf32(*(const float*)(st + KT * RB + swz<KV, RB>(r, ch) + 4 * (g & 3)), bh[x][j][0], bl[x][j][0]);
+                            split_tf32(*(const float*)(st + KT * RB + swz<KV, RB>(r + 1, ch) + 4 * (g & 3)), bh[x][j][1], bl[x][j][1]);
+                        }
                     }
                     // the products with a low half first, while the sum is small
 #pragma unroll
-                    for (int a = 0; a < MT; ++a) {
+                    for (int z = 0; z < 3; ++z)            // lo hi, hi lo, hi hi
 #pragma unroll
-                        for (int j = 0; j < NTK; ++j) {
-                            if (MODE) mma_tf32(d[a], pl[a][j], bh[j][0], bh[j][1]);
-                            mma_tf32(d[a], ph[a][j], bl[j][0], bl[j][1]);
-                        }
+                        for (int j = 0; j < NTK; ++j)
 #pragma unroll
-                        for (int j = 0; j < NTK; ++j) mma_tf32(d[a], ph[a][j], bh[j][0], bh[j][1]);
-                    }
+                            for (int x = 0; x < 2; ++x)
 #pragma unroll
-                    for (int a = 0; a < MT; ++a)
+                                for (int a = 0; a < MT; ++a) {
+                                    if (z == 0 && MODE) mma_tf32(d[x][a], pl[a][j], bh[x][j][0], bh[x][j][1]);
+                                    if (z == 1) mma_tf32(d[x][a], ph[a][j], bl[x][j][0], bl[x][j][1]);
+                                    if (z == 2) mma_tf32(d[x][a], ph[a][j], bh[x][j][0], bh[x][j][1]);
+                                }
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            o[a][jd][e] = fmaf(o[a][jd][e], corr[MODE == 0 ? 0 : (2 * a + (e >> 1)) % RI], d[a][e]);
+                    for (int x = 0; x < 2; ++x)
+#pragma unroll
+                        for (int a = 0; a < MT; ++a)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                o[a][jd + x][e] =
+                                    fmaf(o[a][jd + x][e], corr[MODE == 0 ? 0 : (2 * a + (e >> 1)) % RI], d[x][a][e]);
                 }
             } else {
                 constexpr int PH = MODE == 0 ? 1 : 2;
@@ -721,15 +738,14 @@ __global__ void __launch_bounds__(32 * MW, CTAS / SMS) attn_tree_mma(
 #pragma unroll
                             for (int k = 0; k < 2; ++k)
 #pragma unroll
-                                for (int x = 0; x < 2; ++x) {
-                                    const uint32_t b0 = x ? i8_f16<0x4341>(r[2 * k]) : i8_f16<0x4240>(r[2 * k]);
-                                    const uint32_t b1 = x ? i8_f16<0x4341>(r[2 * k + 1]) : i8_f16<0x4240>(r[2 * k + 1]);
+                                for (int h = PH - 1; h >= 0; --h)
 #pragma unroll
-                                    for (int a = 0; a < MT; ++a)
+                                    for (int x = 0; x < 2; ++x) {
+                                        const uint32_t b0 = x ? i8_f16<0x4341>(r[2 * k]) : i8_f16<0x4240>(r[2 * k]);
+                                        const uint32_t b1 = x ? i8_f16<0x4341>(r[2 * k + 1]) : i8_f16<0x4240>(r[2 * k + 1]);
 #pragma unroll
-                                        for (int h = PH - 1; h >= 0; --h)
-                                            mma_f16(d[a][x], P[a][2 * k2 + k][h], b0, b1);
-                                }
+                                        for (int a = 0; a < MT; ++a) mma_f16(d[a][x], P[a][2 * k2 + k][h], b0, b1);
+                                    }
                         }
                     } else {
 #pragma unroll
@@ -737,12 +753,11 @@ __global__ void __launch_bounds__(32 * MW, CTAS / SMS) attn_tree_mma(
                             uint32_t r[4];
                             ldsm4t(vs_ + swz<KV, RB>(16 * k + ((lane >> 3) & 1) * 8 + (lane & 7), jd + (lane >> 4)), r);
 #pragma unroll
-                            for (int x = 0; x < 2; ++x)
+                            for (int h = PH - 1; h >= 0; --h)
 #pragma unroll
-                                for (int a = 0; a < MT; ++a)
+                                for (int x = 0; x < 2; ++x)
 #pragma unroll
-                                    for (int h = PH - 1; h >= 0; --h)
-                                        mma_f16(d[a][x], P[a][k][h], r[2 * x], r[2 * x + 1]);
+                                    for (int a = 0; a < MT; ++a) mma_f16(d[a][x], P[a][k][h], r[2 * x], r[2 * x + 1]);
                         }
                     }
 #pragma unroll
