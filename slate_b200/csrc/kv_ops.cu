@@ -10,8 +10,17 @@
 #include "sb_internal.h"
 #include "sb_kernels.h"
 #include "sb_kv.h"
+#include "sb_pdl.h"
 
 namespace {
+
+// Every kernel here begins with it: it may have been launched before the one ahead of it in the
+// stream ended, and lets the next one do so if its own blocks are all running by then (blocks
+// that wait would take the place of those still to come).
+__device__ __forceinline__ void chain() {
+    sb_grid_wait();
+    if (gridDim.x * gridDim.y <= 2 * 148) sb_grid_release();
+}
 
 constexpr unsigned FULL = 0xffffffffu;
 
@@ -24,6 +33,7 @@ __global__ void __launch_bounds__(256) rope_append_kernel(
     float* __restrict__ q_out, int ld_qo, const float* q, int ld_q, const float* __restrict__ k,
     int ld_k, const float* __restrict__ v, int ld_v, const int32_t* __restrict__ row_slot,
     const int32_t* __restrict__ row_index, const int32_t* __restrict__ row_pos) {
+    chain();
     const int lane = threadIdx.x & 31, hd = c.head_dim, nkv = c.n_kv_heads;
     const int heads = nq + 2 * nkv, half = rope.rot_dim / 2;
     const int64_t w = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
@@ -101,6 +111,7 @@ __global__ void __launch_bounds__(256) rope_append_vec(
     float* q_out, int ld_qo, const float* q, int ld_q, const float* __restrict__ k, int ld_k,
     const float* __restrict__ v, int ld_v, const int32_t* __restrict__ row_slot,
     const int32_t* __restrict__ row_index, const int32_t* __restrict__ row_pos, int parts_q, int parts) {
+    chain();
     constexpr int HPW = 32 / LPH;                          // heads a warp holds at once
     const int lane = threadIdx.x & 31, sub = lane % LPH, hd = c.head_dim, nkv = c.n_kv_heads;
     const int half = rope.rot_dim / 2, d = 4 * sub;
@@ -255,6 +266,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(
     const slate_kv_cache_t c, int layer0, int n_layers, int rows,
     const int32_t* __restrict__ row_slot, const int32_t* __restrict__ row_index,
     OT* __restrict__ K, OT* __restrict__ V) {
+    chain();
     using T = typename Vec4<KV>::T;
     const int lane = threadIdx.x & 31, hd4 = c.head_dim / 4, nv = c.n_kv_heads * hd4;
     const int64_t w = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
@@ -299,6 +311,7 @@ __global__ void __launch_bounds__(256) kv_read_scalar(
     const slate_kv_cache_t c, int layer0, int n_layers, int rows,
     const int32_t* __restrict__ row_slot, const int32_t* __restrict__ row_index,
     OT* __restrict__ K, OT* __restrict__ V) {
+    chain();
     const int lane = threadIdx.x & 31, hd = c.head_dim, nkv = c.n_kv_heads;
     int64_t w = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
     if (w >= (int64_t)n_layers * rows * 2 * nkv) return;
@@ -356,6 +369,7 @@ __global__ void __launch_bounds__(AT) tree_accept_kernel(
     const slate_kv_cache_t c, const slate_tree_t tr, const int32_t* __restrict__ parent,
     const int32_t* __restrict__ token, const int32_t* __restrict__ target, int32_t* out_count,
     int32_t* out_node, int32_t* out_token) {
+    chain();
     __shared__ uint32_t ok_s[2];
     __shared__ int best_s[2];
     __shared__ int src_page[64], src_t[64], dst_page[64], dst_t[64];
@@ -461,28 +475,28 @@ extern "C" int slate_cuda_rope_append(const slate_kv_cache_t* cache, int layer,
         const int parts = parts_q + (2 * nkv + ru * hpw - 1) / (ru * hpw);
         const int64_t n = (int64_t)rows * parts;
         const auto go = [&](auto kernel) {
-            kernel<<<(unsigned)((n + 7) / 8), 256, 0, (cudaStream_t)stream>>>(
-                *cache, layer, *rope, rows, n_heads, q_out, ld_q_out, q, ld_q, k, ld_k, v, ld_v, row_slot,
-                row_index, row_pos, parts_q, parts);
+            return sb_launch_pdl(kernel, dim3((unsigned)((n + 7) / 8)), dim3(256), 0, (cudaStream_t)stream, *cache,
+                                 layer, *rope, rows, n_heads, q_out, ld_q_out, q, ld_q, k, ld_k, v, ld_v, row_slot,
+                                 row_index, row_pos, parts_q, parts);
         };
         const auto by_type = [&](auto l, auto u) {
             constexpr int L = decltype(l)::value, U = decltype(u)::value;
-            cache->kv_dtype == SLATE_KV_F32   ? go(rope_append_vec<L, SLATE_KV_F32, U>)
-            : cache->kv_dtype == SLATE_KV_F16 ? go(rope_append_vec<L, SLATE_KV_F16, U>)
-                                              : go(rope_append_vec<L, SLATE_KV_Q8, U>);
+            return cache->kv_dtype == SLATE_KV_F32   ? go(rope_append_vec<L, SLATE_KV_F32, U>)
+                   : cache->kv_dtype == SLATE_KV_F16 ? go(rope_append_vec<L, SLATE_KV_F16, U>)
+                                                     : go(rope_append_vec<L, SLATE_KV_Q8, U>);
         };
         const auto by_ru = [&](auto l) {
-            ru == 2 ? by_type(l, std::integral_constant<int, 2>{}) : by_type(l, std::integral_constant<int, 4>{});
+            return ru == 2 ? by_type(l, std::integral_constant<int, 2>{}) : by_type(l, std::integral_constant<int, 4>{});
         };
-        if (lph == 32) by_ru(std::integral_constant<int, 32>{});
-        else if (lph == 16) by_ru(std::integral_constant<int, 16>{});
-        else by_ru(std::integral_constant<int, 8>{});
-        return sb_cuda_check(cudaGetLastError(), "rope_append");
+        return sb_cuda_check(lph == 32   ? by_ru(std::integral_constant<int, 32>{})
+                             : lph == 16 ? by_ru(std::integral_constant<int, 16>{})
+                                         : by_ru(std::integral_constant<int, 8>{}),
+                             "rope_append");
     }
-    rope_append_kernel<<<(unsigned)((warps + 7) / 8), 256, 0, (cudaStream_t)stream>>>(
-        *cache, layer, *rope, rows, n_heads, q_out, ld_q_out, q, ld_q, k, ld_k, v, ld_v, row_slot,
-        row_index, row_pos);
-    return sb_cuda_check(cudaGetLastError(), "rope_append");
+    return sb_cuda_check(sb_launch_pdl(rope_append_kernel, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0,
+                                       (cudaStream_t)stream, *cache, layer, *rope, rows, n_heads, q_out, ld_q_out, q,
+                                       ld_q, k, ld_k, v, ld_v, row_slot, row_index, row_pos),
+                         "rope_append");
 }
 
 extern "C" int slate_cuda_kv_read(const slate_kv_cache_t* cache, int layer0, int n_layers, int rows,
@@ -503,24 +517,21 @@ extern "C" int slate_cuda_kv_read(const slate_kv_cache_t* cache, int layer0, int
     const cudaStream_t st = (cudaStream_t)stream;
     const uintptr_t mis = ((uintptr_t)K | (uintptr_t)V) & (out_dtype == SLATE_KV_F16 ? 7 : 15);
     const auto go = [&](auto vec, auto scalar, auto* k, auto* v) {
-        if (mis)
-            scalar<<<(unsigned)((warps + 7) / 8), 256, 0, st>>>(*cache, layer0, n_layers, rows, row_slot, row_index, k, v);
-        else
-            vec<<<(unsigned)(((int64_t)n_layers * rows + 7) / 8), 256, 0, st>>>(*cache, layer0, n_layers, rows, row_slot,
-                                                                               row_index, k, v);
+        const int64_t n = mis ? warps : (int64_t)n_layers * rows;
+        return sb_launch_pdl(mis ? scalar : vec, dim3((unsigned)((n + 7) / 8)), dim3(256), 0, st, *cache, layer0, n_layers,
+                             rows, row_slot, row_index, k, v);
     };
     const int kt = cache->kv_dtype;
-    if (out_dtype == SLATE_KV_F16)
-        go(kt == SLATE_KV_F32   ? kv_read_kernel<__half, SLATE_KV_F32>
-           : kt == SLATE_KV_F16 ? kv_read_kernel<__half, SLATE_KV_F16>
-                                : kv_read_kernel<__half, SLATE_KV_Q8>,
-           kv_read_scalar<__half>, (__half*)K, (__half*)V);
-    else
-        go(kt == SLATE_KV_F32   ? kv_read_kernel<float, SLATE_KV_F32>
-           : kt == SLATE_KV_F16 ? kv_read_kernel<float, SLATE_KV_F16>
-                                : kv_read_kernel<float, SLATE_KV_Q8>,
-           kv_read_scalar<float>, (float*)K, (float*)V);
-    return sb_cuda_check(cudaGetLastError(), "kv_read");
+    const cudaError_t err =
+        out_dtype == SLATE_KV_F16 ? go(kt == SLATE_KV_F32   ? kv_read_kernel<__half, SLATE_KV_F32>
+                                       : kt == SLATE_KV_F16 ? kv_read_kernel<__half, SLATE_KV_F16>
+                                                            : kv_read_kernel<__half, SLATE_KV_Q8>,
+                                       kv_read_scalar<__half>, (__half*)K, (__half*)V)
+                                  : go(kt == SLATE_KV_F32   ? kv_read_kernel<float, SLATE_KV_F32>
+                                       : kt == SLATE_KV_F16 ? kv_read_kernel<float, SLATE_KV_F16>
+                                                            : kv_read_kernel<float, SLATE_KV_Q8>,
+                                       kv_read_scalar<float>, (float*)K, (float*)V);
+    return sb_cuda_check(err, "kv_read");
 }
 
 extern "C" int slate_cuda_tree_accept(const slate_kv_cache_t* cache, const slate_tree_t* tree,
@@ -533,8 +544,8 @@ extern "C" int slate_cuda_tree_accept(const slate_kv_cache_t* cache, const slate
         sb_set_error("tree_accept: bad arguments");
         return -1;
     }
-    tree_accept_kernel<<<dim3((unsigned)tree->n_seq, (unsigned)cache->n_layers), AT, 0,
-                         (cudaStream_t)stream>>>(*cache, *tree, parent, token, target, out_count,
-                                                 out_node, out_token);
-    return sb_cuda_check(cudaGetLastError(), "tree_accept");
+    return sb_cuda_check(sb_launch_pdl(tree_accept_kernel, dim3((unsigned)tree->n_seq, (unsigned)cache->n_layers), dim3(AT),
+                                       0, (cudaStream_t)stream, *cache, *tree, parent, token, target, out_count, out_node,
+                                       out_token),
+                         "tree_accept");
 }
