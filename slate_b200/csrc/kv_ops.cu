@@ -103,10 +103,12 @@ __global__ void __launch_bounds__(256) rope_append_kernel(
 // warp keeps RU * 32 / LPH heads in flight; query heads and key/value heads go to warps
 // of their own, so neither carries the other's branches.  Bound by HBM: q is read and
 // written, k and v read, the cache written once; nothing else moves.  8191 rows of 32 + 8
-// + 8 heads of 128 on the 8-bit cache, with their read-back: 86 us, 5.1 TB/s (exact
-// division for every element: 101 us; q and k heads in one warp: 95 us).
+// + 8 heads of 128 on the 8-bit cache, with their read-back: 82 us, 5.4 TB/s (exact
+// division for every element: 101 us; q and k heads in one warp: 95 us).  Blocks an SM: six
+// on 8 bits, where instructions count (82 us; 86 with the four that registers would leave),
+// five else (8191 rows of f16 62 us; six spill, 66).
 template <int LPH, int KV, int RU>
-__global__ void __launch_bounds__(256) rope_append_vec(
+__global__ void __launch_bounds__(256, KV == SLATE_KV_Q8 ? 6 : 5) rope_append_vec(
     const slate_kv_cache_t c, int layer, const slate_rope_t rope, int rows, int nq,
     float* q_out, int ld_qo, const float* q, int ld_q, const float* __restrict__ k, int ld_k,
     const float* __restrict__ v, int ld_v, const int32_t* __restrict__ row_slot,
@@ -233,7 +235,8 @@ __global__ void __launch_bounds__(256) rope_append_vec(
 
 // A warp per (layer, row), K and V: its n_kv_heads * head_dim / 4 vectors of four in
 // steps of 32, RV vectors of each in flight.  Consecutive lanes write consecutive 16
-// (f16: 8) bytes, and read 4, 8 or 16.  Bound by HBM, mostly by what it writes.
+// (f16: 8) bytes, and read 4, 8 or 16.  Bound by HBM, mostly by what it writes: 32760 rows of
+// 4 layers from 8 bits to f32 in 210 us, 6.4 TB/s; 517 rows of 2 layers 2.8 us, launch and latency.
 constexpr int RV = 4;
 template <int KV>
 struct Vec4 {
@@ -339,7 +342,9 @@ __global__ void __launch_bounds__(256) kv_read_scalar(
 // (64 nodes, two warp votes), then each thread moves 16-byte (or 4-byte) columns
 // of the path's rows in order.  The path's indexes rise, so the k-th row's place
 // (k) never lies at or behind a later row's source (path[k'] >= k' > k): moving
-// in order never overwrites what is still to be read, nor does reading MU rows ahead.
+// in order never overwrites what is still to be read, nor does reading MU rows ahead.  Bound by
+// latency for few sequences (13 nodes, 16 layers: 3.6 us) and by scattered rows of HBM for many (48
+// x 40 nodes, 32 layers of f16: 21 us, 4.9 TB/s).
 constexpr int AT = 256, MU = 8;
 template <typename U>
 __device__ void move_rows(const slate_kv_cache_t& c, int layer, int n, const int* src_page,
@@ -469,7 +474,7 @@ extern "C" int slate_cuda_rope_append(const slate_kv_cache_t* cache, int layer,
         al(rope->sin) && ld_q % 4 == 0 && ld_q_out % 4 == 0 && ld_k % 4 == 0 && ld_v % 4 == 0) {
         const int lph = hd > 64 ? 32 : hd > 32 ? 16 : 8, hpw = 32 / lph, heads = n_heads + 2 * nkv;
         // RU head groups a warp in flight: four where two would still make a full wave of warps (64 an
-        // SM; 8191 rows of 48 heads: 86 us against 101 with two), else two (16 such rows: 6.9 against 7.5)
+        // SM; 8191 rows of 48 heads: 82 us against 95 with two), else two (16 such rows: 6.9 against 7.5)
         const int ru = (int64_t)rows * heads / (2 * hpw) > 148 * 64 ? 4 : 2;
         const int parts_q = (n_heads + ru * hpw - 1) / (ru * hpw);
         const int parts = parts_q + (2 * nkv + ru * hpw - 1) / (ru * hpw);
