@@ -58,7 +58,10 @@ struct TcShape {
     static constexpr int TB = KT * HD * 2;                 // a K or V tile in f16
     static constexpr int SC = SCB * 2 * KT * 4;
     static constexpr int SMEM = 2 * NB * TB + SC + 1024;
-    static_assert(MR * (HD + 1) * 4 <= 2 * NB * TB, "q and O pass through the tiles");
+    // q and O pass through the tiles; f16: behind K and all but the last page of V of a CTA's first
+    // tile, which come in meanwhile
+    static constexpr int STAGE = KV == SLATE_KV_Q8 ? 0 : 2 * NB * TB - MR * (HD + 1) * 4;
+    static_assert(KV == SLATE_KV_Q8 ? MR * (HD + 1) * 4 <= 2 * NB * TB : STAGE >= (NB + 1) * TB - 16 * 128, "");
 };
 
 struct Yes {
@@ -282,7 +285,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
             // read its own row would ask for a sector an element)
             float O[HO];
             {
-                float* stage = (float*)skv;
+                float* stage = (float*)(skv + S::STAGE);
                 for (int i0 = warp; i0 < n_rows; i0 += 4 * NSW) {
                     float x[4][HD / 32];               // four rows in flight
 #pragma unroll
@@ -538,7 +541,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                     o[1] = L + bad;
                 }
                 const float f = (sg.whole ? (L == 0.f ? 0.f : 1.f / L) : 1.f); // l and o carry the same power of two
-                float* x = (float*)skv + r * (HD + 1) + HO * h;
+                float* x = (float*)(skv + S::STAGE) + r * (HD + 1) + HO * h;
 #pragma unroll
                 for (int i = 0; i < HO; ++i) x[i] = O[i] * f + bad;
             }
@@ -548,7 +551,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                 float* o = sg.whole ? out + (size_t)(sq_.r0 + rr / G) * ld_out + (size_t)(kvh * G + rr % G) * HD
                                     : ws + ((size_t)(2 * blockIdx.x + (sg.seg ? 1 : 0)) * MR + i) * (HD + 2) + 2;
 #pragma unroll
-                for (int k = 0; k < HD / 32; ++k) o[lane + 32 * k] = ((const float*)skv)[i * (HD + 1) + lane + 32 * k];
+                for (int k = 0; k < HD / 32; ++k) o[lane + 32 * k] = ((const float*)(skv + S::STAGE))[i * (HD + 1) + lane + 32 * k];
             }
             if (*fail) break;
         }
@@ -617,7 +620,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
         const int w = warp - NSW;
         while (next_segment()) {
             const int nt = sg.nt, kvh = sg.kvh, tok0 = sg.tok0, end = sg.end, ctx = sg.sq.ctx, slot = sg.sq.slot;
-            __syncthreads();
+            if (Q8 || tb) __syncthreads();
             bool ok = true;
             const int njobs = 16 * nt;
             const size_t kv_step = (size_t)nkv * sb_kv_block_bytes(KV, HD), page_step = 2 * kv_step;
@@ -744,10 +747,22 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                     }
                     arrive(n);
                 };
-                int page = page_of(w);
-                for (int n = w; n < njobs && ok; n += NPW) {
+                // Lane i holds the page of the warp's job i, of 32 jobs and the 32 after them: no job waits
+                // for its page's number.
+                const auto pages_of = [&](int first) { return page_of(w + NPW * (first + lane)); };
+                int window = pages_of(0), window2 = pages_of(32), job = 0;
+                bool q_gone = tb > 0;
+                for (int n = w; n < njobs && ok; n += NPW, ++job) {
                     const int j = n >> 4, pg = n & 7, t0 = tok0 + j * KT + 16 * pg;
-                    const int next = page_of(n + NPW);
+                    if (job && (job & 31) == 0) {
+                        window = window2;
+                        window2 = pages_of(job + 32);
+                    }
+                    const int page = __shfl_sync(FULL, window, job & 31);
+                    if (!q_gone && n >= 15) {
+                        q_gone = true;
+                        __syncthreads();
+                    }
                     wait_free(n);
                     if (!ok) break;
                     const uint32_t dst = su32(skv) + (((n & 8) ? NB : 0) + (tb + j) % NB) * S::TB + pg * 2048;
@@ -758,7 +773,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                              page >= 0 && t0 + lane / CPT + TS * i < end);
                     if (lane == 0 && !(n & 8)) gone_s[(tb + j) % SCB][pg] = page < 0;
                     cp_commit();
-                    page = next;
                     // DEPTH jobs stay in flight; what a job waits for lies at least 33 jobs back, so the
                     // ones still to land cannot be in its way
                     if (n >= DEPTH * NPW) {
@@ -766,6 +780,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                         land(n - DEPTH * NPW);
                     }
                 }
+                if (!q_gone) __syncthreads();
                 const int mine = (njobs - w + NPW - 1) / NPW;      // the last of the warp's jobs
                 cp_wait<0>();
                 for (int i = max(mine - DEPTH, 0); i < mine && ok; ++i) land(w + i * NPW);
