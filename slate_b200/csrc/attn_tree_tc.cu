@@ -620,7 +620,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
         const int w = warp - NSW;
         while (next_segment()) {
             const int nt = sg.nt, kvh = sg.kvh, tok0 = sg.tok0, end = sg.end, ctx = sg.sq.ctx, slot = sg.sq.slot;
-            if (Q8 || tb) __syncthreads();
+            if (!Q8 && tb) __syncthreads();
             bool ok = true;
             const int njobs = 16 * nt;
             const size_t kv_step = (size_t)nkv * sb_kv_block_bytes(KV, HD), page_step = 2 * kv_step;
@@ -711,6 +711,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                 z.next = page_of(w + NPW);
                 fetch(a, w);
                 fetch(z, w + NPW);
+                __syncthreads();                       // q has left the tiles
                 for (int n = w; n < njobs && ok; n += 2 * NPW) {
                     put(a, n);
                     fetch(a, n + 2 * NPW);
