@@ -133,9 +133,7 @@ __global__ void __launch_bounds__(32 * NW) attn_tree_rows(
 }
 
 // ------------------------------------------------------------ tensor-core path
-constexpr int CTAS = 2 * SMS;               // two an SM
 constexpr int UNIT = 64;
-static_assert(CTAS * 32 <= SMS * TC_ROWS, "workspace");
 constexpr int MW = 4;                       // warps a CTA
 constexpr float DIG = 127.f * 65536.f;      // three digits to base 256 stay within 8 bits each
 
@@ -171,7 +169,7 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
     lo = __float_as_uint(x - __uint_as_float(hi));
 }
 // KT tokens of K and V a tile and warp, ~8 KB, in a ring of NS tiles for each warp
-// (the ring and q fit twice into an SM's shared memory).  A row's 16-byte chunks are
+// (the ring and q fit CPS times into an SM's shared memory).  A row's 16-byte chunks are
 // exchanged by XOR with a function of the row, so that neither ldmatrix (8 rows, one
 // chunk each) nor the f32 reads (4 or 8 rows) meet in a bank.
 template <int KV, int HD, int MODE>
@@ -190,7 +188,11 @@ struct Shape {
     static constexpr int KS = I8 ? HD / 32 : KV == SLATE_KV_F32 ? HD / 8 : HD / 16;    // k steps of a score
     static constexpr int HL = I8 ? MODE + 2 : MODE == 0 ? 1 : 2;    // A operands a k step
     static constexpr int QB = MT * KS * HL * 512;
-    static constexpr int NS0 = (112 * 1024 - QB) / (MW * TB);
+    // CTAs an SM: three where 168 registers a thread do (64 sequences of one node over 4096 tokens 54.9
+    // us, with two 60.3; head_dim 128 spills, 93 against 84)
+    static constexpr int CPS = KV == SLATE_KV_Q8 && HD == 64 && MODE == 0 ? 3 : 2;
+    static_assert(CPS * MR <= TC_ROWS, "workspace");
+    static constexpr int NS0 = ((CPS == 3 ? 74 : 112) * 1024 - QB) / (MW * TB);
     static constexpr int NS = NS0 > 6 ? 6 : NS0;
     static constexpr int MERGE = MW * MR * (HD + 2) * 4;
     static constexpr int RING = MW * NS * TB > MERGE ? MW * NS * TB : MERGE;
@@ -215,7 +217,7 @@ __device__ __forceinline__ uint32_t swz(int row, int chunk) {
 // reads.
 // Partial of one cut item: [MR][HD + 2]: (max in log2 units, sum, o) rows.
 template <int KV, int HD, int MODE>
-__global__ void __launch_bounds__(32 * MW, CTAS / SMS) attn_tree_mma(
+__global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_mma(
     const slate_kv_cache_t c, int layer, const slate_tree_t tr, int nq, float* __restrict__ out,
     int ld_out, const float* __restrict__ q, int ld_q, float scale, float* __restrict__ ws) {
     using S = Shape<KV, HD, MODE>;
@@ -979,10 +981,10 @@ int launch_mma(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int
     static const cudaError_t ready =
         cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (ready != cudaSuccess) return sb_cuda_check(ready, "attention_tree shared memory");
-    const int rc = sb_cuda_check(sb_launch_pdl(k, dim3(CTAS), dim3(32 * MW), S::SMEM, st, c, layer, tr, nq, out,
+    const int rc = sb_cuda_check(sb_launch_pdl(k, dim3(S::CPS * SMS), dim3(32 * MW), S::SMEM, st, c, layer, tr, nq, out,
                                                ld_out, q, ld_q, scale, ws),
                                  "attention_tree");
-    return rc ? rc : join<HD>(c, tr, nq, S::MR, UNIT, S::SLACK, CTAS, out, ld_out, ws, st);
+    return rc ? rc : join<HD>(c, tr, nq, S::MR, UNIT, S::SLACK, S::CPS * SMS, out, ld_out, ws, st);
 }
 template <int KV, int HD>
 int launch_mode(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq, float* out,
@@ -1006,7 +1008,7 @@ bool takes_mma(const slate_kv_cache_t* c) { return c->head_dim == 64 || c->head_
 extern "C" size_t slate_cuda_attention_tree_workspace(const slate_kv_cache_t* cache, int n_heads,
                                                       int n_seq, int rows, int max_nodes) {
     if (!cache || n_heads < 1 || n_seq < 1 || rows < 0 || max_nodes < 1) return 0;
-    // two partials for each CTA: 148 of 128 rows, or 2 * 148 of 32 at most
+    // two partials for each CTA: 148 of 128 rows, or 3 * 148 of 8, 2 * 148 of 32 at most
     return takes_mma(cache) ? (size_t)2 * SMS * TC_ROWS * (cache->head_dim + 2) * 4 : 16;
 }
 
