@@ -27,6 +27,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "sb_internal.h"
 #include "sb_kernels.h"
 #include "sb_kv.h"
@@ -189,7 +191,7 @@ struct Segs {
     }
 };
 
-template <int KV, int HD>
+template <int KV, int HD, bool SPLIT>
 __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
     const slate_kv_cache_t c, int layer, const slate_tree_t tr, int nq, float* __restrict__ out,
     int ld_out, const float* __restrict__ q, int ld_q, float scale, float* __restrict__ ws) {
@@ -276,9 +278,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
             const Seq& sq_ = sg.sq;
             const int nt = sg.nt, kvh = sg.kvh, r_base = sg.r_base, n_rows = sg.n_rows, tok0 = sg.tok0;
             // ================= softmax: thread = row, part h of the tile's tokens and of O's dims
-            constexpr int HO = HD / PARTS, TQ = KT / PARTS;
-            const int h = warp >> 2, r = tid & 127;
-            const bool live = (warp & 3) * 32 < n_rows;                 // of the warp
+            // SPLIT: lanes 64-127 hold rows 0-63 again; a row's two lanes take half of the tokens each and
+            // are joined at the segment's end
+            constexpr int HO = HD / PARTS, TQ = KT / PARTS / (SPLIT ? 2 : 1), RMASK = SPLIT ? 63 : 127;
+            const int h = warp >> 2, r = tid & 127, rq = r & RMASK;     // lane; row
+            const auto toff = [&]() { return TQ * h + (SPLIT ? r & 64 : 0); };     // the thread's first token of a tile
+            const bool live = ((warp & 3) * 32 & RMASK) < n_rows;       // of the warp
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
             // ---- q, each row divided by the power of two below its maximum; scale's sign joins q
             // ---- (a row at a time through the K and V tiles, which nobody else uses yet: a thread that
@@ -302,7 +307,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                             if (i0 + u * NSW < n_rows) stage[(i0 + u * NSW) * (HD + 1) + lane + 32 * k] = x[u][k];
                 }
                 softmax_sync();
-                const float* x = stage + min(r, n_rows - 1) * (HD + 1) + HO * h;
+                const float* x = stage + min(rq, n_rows - 1) * (HD + 1) + HO * h;
                 uint32_t top = 0;
 #pragma unroll
                 for (int i = 0; i < HO; ++i) {
@@ -333,13 +338,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
             for (int i = 0; i < HO; ++i) O[i] = 0.f;
             __syncthreads();
             tc_after();
-            const uint64_t mk = r < n_rows ? __ldg(tr.mask + sq_.r0 + (r_base + r) / G) : 0;
+            const uint64_t mk = rq < n_rows ? __ldg(tr.mask + sq_.r0 + (r_base + rq) / G) : 0;
             float m = -INFINITY, l = 0.f;              // m: what p is taken against, in log2 units
             int vexp = -80;                            // 8 bits: 2^vexp is above every v scale so far
             bool ok = true;
-            const auto scales = [&](int j) { return ssc + (tb + j) % SCB * (2 * KT) + TQ * h; };
-            const auto s_part = [&](int j) { return sS((tb + j) & 1) + lanes + TQ * h; };
-            const auto first_token = [&](int j) { return tok0 + j * KT + TQ * h; };
+            const auto scales = [&](int j) { return ssc + (tb + j) % SCB * (2 * KT) + toff(); };
+            const auto s_part = [&](int j) { return sS((tb + j) & 1) + lanes + toff(); };
+            const auto first_token = [&](int j) { return tok0 + j * KT + toff(); };
             const auto wait_s = [&](int j) {
                 ok = ok && __all_sync(FULL, bar_wait(&bars.sfull[(tb + j) & 1], phase2(tb + j), fail));
                 tc_after();
@@ -352,11 +357,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
             };
             // every row sees every token of the thread's part of tile j
             const auto seen_by_all = [&](int j) {
-                return *(const uint32_t*)&gone_s[(tb + j) % SCB][TQ / 16 * h] == 0 && first_token(j) + TQ <= sq_.ctx;
+                const uint8_t* gone = &gone_s[(tb + j) % SCB][toff() / 16];
+                return (SPLIT ? *(const uint16_t*)gone : *(const uint32_t*)gone) == 0 && first_token(j) + TQ <= sq_.ctx;
             };
             // which of the part's 32 tokens from t the row sees
             const auto seen = [&](int j, int t) {
-                const uint8_t* gone = &gone_s[(tb + j) % SCB][TQ / 16 * h + t / 16];
+                const uint8_t* gone = &gone_s[(tb + j) % SCB][toff() / 16 + t / 16];
                 uint32_t v = 0xffffffffu;
                 if (gone[0]) v &= 0xffff0000u;
                 if (gone[1]) v &= 0x0000ffffu;
@@ -497,6 +503,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
 #pragma unroll
                     for (int i = 0; i < HO; ++i) O[i] *= corr;
                 }
+                if (SPLIT && ok && live) {             // nothing of the other lane's tokens
+                    const uint32_t zero[16] = {};
+                    const uint32_t other = sS(t & 1) + lanes + (toff() ^ 64);
+                    tmem_st(other, zero);
+                    tmem_st(other + 16, zero);
+                }
                 if (ok && live) {
                     l += all ? tile_p(Yes{}, j) : tile_p(No{}, j);
                     tmem_st_wait();
@@ -518,6 +530,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                                 const int t = t0 + 16 * w + __ffs(rest) - 1, x = t - sq_.ctx;
                                 const int page = sb_kv_page(c, sq_.slot, t);
                                 if (page < 0 || x < 0 || x >= sq_.n || !(mk >> x & 1)) continue;
+                                if (SPLIT && (w >> 2) != (r >> 6)) continue;   // the other lane's token
                                 const __half* v = (const __half*)sb_kv_block(c, layer, page, 1, kvh) + (t & 15) * HD + HO * h;
 #pragma unroll
                                 for (int i = 0; i < HO; ++i) {
@@ -530,28 +543,60 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
             tb += nt;
             if (live) part_max[0][h][r] = l;
             __syncthreads();                           // every product is done: q and the scales are free
-            if (r < n_rows) {
-                float L = part_max[0][0][r];
-#pragma unroll
-                for (int i = 1; i < PARTS; ++i) L += part_max[0][i][r];
+            if constexpr (SPLIT) {
                 const float bad = *fail ? NAN : 0.f;   // a wait ran out: no number may pass for a result
-                if (!sg.whole && h == 0) {
-                    float* o = ws + ((size_t)(2 * blockIdx.x + (sg.seg ? 1 : 0)) * MR + r) * (HD + 2);
-                    o[0] = Q8 ? m + (float)vexp : m;   // 2^up of another part may differ
-                    o[1] = L + bad;
+                if (rq < n_rows) {
+                    // l and o carry the same power of two; that of another part may differ
+                    if (h == 0) part_max[1][0][r] = Q8 ? m + (float)vexp : m;
+                    else part_max[1][1][r] = part_max[0][0][r] + part_max[0][1][r] + bad;
+                    float* x = (float*)(skv + S::STAGE) + r * (HD + 1) + HO * h;
+#pragma unroll
+                    for (int i = 0; i < HO; ++i) x[i] = O[i] + bad;
                 }
-                const float f = (sg.whole ? (L == 0.f ? 0.f : 1.f / L) : 1.f); // l and o carry the same power of two
-                float* x = (float*)(skv + S::STAGE) + r * (HD + 1) + HO * h;
+                softmax_sync();
+                for (int i = warp; i < n_rows; i += NSW) {             // a row at a time, its two lanes joined
+                    const int rr = r_base + i;
+                    float* o = sg.whole ? out + (size_t)(sq_.r0 + rr / G) * ld_out + (size_t)(kvh * G + rr % G) * HD
+                                        : ws + ((size_t)(2 * blockIdx.x + (sg.seg ? 1 : 0)) * MR + i) * (HD + 2) + 2;
+                    const float* x = (const float*)(skv + S::STAGE) + i * (HD + 1) + lane;
+                    const float ma = part_max[1][0][i], mb = part_max[1][0][i + 64], M = fmaxf(ma, mb);
+                    float fa = ma == -INFINITY ? 1.f : ex2(ma - M), fb = mb == -INFINITY ? 1.f : ex2(mb - M);
+                    const float L = fmaf(part_max[1][1][i], fa, part_max[1][1][i + 64] * fb);
+                    if (sg.whole) {
+                        const float inv = L == 0.f ? 0.f : 1.f / L;
+                        fa *= inv;
+                        fb *= inv;
+                    } else if (lane == 0) {
+                        o[-2] = M;
+                        o[-1] = L;
+                    }
 #pragma unroll
-                for (int i = 0; i < HO; ++i) x[i] = O[i] * f + bad;
-            }
-            softmax_sync();
-            for (int i = warp; i < n_rows; i += NSW) { // through the tiles again, a row at a time
-                const int rr = r_base + i;
-                float* o = sg.whole ? out + (size_t)(sq_.r0 + rr / G) * ld_out + (size_t)(kvh * G + rr % G) * HD
-                                    : ws + ((size_t)(2 * blockIdx.x + (sg.seg ? 1 : 0)) * MR + i) * (HD + 2) + 2;
+                    for (int k = 0; k < HD / 32; ++k) o[lane + 32 * k] = fmaf(x[32 * k], fa, x[64 * (HD + 1) + 32 * k] * fb);
+                }
+            } else {
+                if (r < n_rows) {
+                    float L = part_max[0][0][r];
 #pragma unroll
-                for (int k = 0; k < HD / 32; ++k) o[lane + 32 * k] = ((const float*)(skv + S::STAGE))[i * (HD + 1) + lane + 32 * k];
+                    for (int i = 1; i < PARTS; ++i) L += part_max[0][i][r];
+                    const float bad = *fail ? NAN : 0.f;
+                    if (!sg.whole && h == 0) {
+                        float* o = ws + ((size_t)(2 * blockIdx.x + (sg.seg ? 1 : 0)) * MR + r) * (HD + 2);
+                        o[0] = Q8 ? m + (float)vexp : m;
+                        o[1] = L + bad;
+                    }
+                    const float f = (sg.whole ? (L == 0.f ? 0.f : 1.f / L) : 1.f);
+                    float* x = (float*)(skv + S::STAGE) + r * (HD + 1) + HO * h;
+#pragma unroll
+                    for (int i = 0; i < HO; ++i) x[i] = O[i] * f + bad;
+                }
+                softmax_sync();
+                for (int i = warp; i < n_rows; i += NSW) {             // through the tiles again, a row at a time
+                    const int rr = r_base + i;
+                    float* o = sg.whole ? out + (size_t)(sq_.r0 + rr / G) * ld_out + (size_t)(kvh * G + rr % G) * HD
+                                        : ws + ((size_t)(2 * blockIdx.x + (sg.seg ? 1 : 0)) * MR + i) * (HD + 2) + 2;
+#pragma unroll
+                    for (int k = 0; k < HD / 32; ++k) o[lane + 32 * k] = ((const float*)(skv + S::STAGE))[i * (HD + 1) + lane + 32 * k];
+                }
             }
             if (*fail) break;
         }
@@ -808,10 +853,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
     if (warp == NSW + NPW) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
-template <int KV, int HD>
+template <int KV, int HD, bool SPLIT>
 int launch(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq, float* out, int ld_out,
            const float* q, int ld_q, float scale, float* ws, cudaStream_t st) {
-    const auto k = attn_tree_tc<KV, HD>;
+    const auto k = attn_tree_tc<KV, HD, SPLIT>;
     static const cudaError_t ready =
         cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, TcShape<KV, HD>::SMEM);
     if (ready != cudaSuccess) return sb_cuda_check(ready, "attention_tree shared memory");
@@ -824,7 +869,14 @@ int launch(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq,
 
 int sb_tree::attend_tc(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq, float* out, int ld_out,
                        const float* q, int ld_q, float scale, float* ws, cudaStream_t st) {
-    const auto f = c.kv_dtype == SLATE_KV_F16 ? (c.head_dim == 64 ? launch<SLATE_KV_F16, 64> : launch<SLATE_KV_F16, 128>)
-                                              : (c.head_dim == 64 ? launch<SLATE_KV_Q8, 64> : launch<SLATE_KV_Q8, 128>);
+    const auto by_rows = [&](auto kv, auto hd) {
+        constexpr int KV = decltype(kv)::value, HD = decltype(hd)::value;
+        return tr.max_nodes * (nq / c.n_kv_heads) <= 64 ? launch<KV, HD, true> : launch<KV, HD, false>;
+    };
+    const auto by_hd = [&](auto kv) {
+        return c.head_dim == 64 ? by_rows(kv, std::integral_constant<int, 64>{}) : by_rows(kv, std::integral_constant<int, 128>{});
+    };
+    const auto f = c.kv_dtype == SLATE_KV_F16 ? by_hd(std::integral_constant<int, SLATE_KV_F16>{})
+                                              : by_hd(std::integral_constant<int, SLATE_KV_Q8>{});
     return f(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);
 }
