@@ -990,9 +990,10 @@ template <int KV, int HD>
 int launch_mode(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq, float* out,
                 int ld_out, const float* q, int ld_q, float scale, float* ws, cudaStream_t st) {
     const int M = tr.max_nodes * (nq / c.n_kv_heads);
-    // attn_tree_mma with 32 rows against attn_tree_tc, 16 sequences of 8 nodes x 4 heads over 8000
-    // tokens: f16 at head_dim 128 113 and 93 us, at 64 62 and 79, 8 bits at 128 103 and 129
-    constexpr int few = KV == SLATE_KV_F16 && HD == 128 ? 16 : 32;
+    // attn_tree_mma with 32 rows against attn_tree_tc, 16 sequences of 8 nodes x 4 heads: head_dim 128 over
+    // 1000 tokens of 8 bits 36 and 31 us, over 8000 103 and 103, of f16 113 and 87; head_dim 64 over 8000 of
+    // f16 63 and 69, of 8 bits 61 and 91
+    constexpr int few = KV != SLATE_KV_F32 && HD == 128 ? 16 : 32;
     if (M <= 8) return launch_mma<KV, HD, 0>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);
     if (M <= 16) return launch_mma<KV, HD, 1>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);
     if constexpr (few > 16)

@@ -17,12 +17,16 @@
 // pages ahead, widened to f16 on the way).  Warp 15 issues the products.
 // q comes and O leaves a row at a time through the tiles' shared memory (a thread that read or wrote
 // its own row moved a sector an element: 15.5 us for one tile a CTA against 21.8).
+// SPLIT, up to 64 rows: lanes 64-127 would idle, and the softmax of a tile is what the next waits for;
+// so they hold the rows again, each lane takes half of a tile's tokens (P is 0 for the others), and
+// a row's two lanes are joined like two CTAs' parts (8 x 16 nodes of f16: 50.5 us against 52.3, at
+// head_dim 64 42.8 against 47.0).
 // What bounds it.  256 rows and more over long contexts (4 sequences of 64 nodes, 64 heads over
-// 8, 32000 tokens of 8 bits: 438 us, 414 TFLOP/s of the formula, 827 with both halves): the softmax's
+// 8, 32000 tokens of 8 bits: 436 us, 415 TFLOP/s of the formula, 830 with both halves): the softmax's
 // issue slots, two passes over S with an exponential and a split a score, next to tensor cores that
 // are busy about half of the time.  Few rows (8 sequences of 16 nodes, 32 heads over 8, 8000 tokens
-// of f16: 54 us, 3.0 TB/s): HBM within the tiles (3400 clocks each, 5.4 TB/s), then what a CTA does
-// before the first tile and after the last, some 20 us of the call.
+// of f16: 50.6 us, 3.2 TB/s): the loads within the tiles, then what a CTA does before the first tile
+// and after the last, some 20 us of the call.
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
