@@ -431,13 +431,20 @@ __global__ void __launch_bounds__(AT) tree_accept_kernel(
     else
         move_rows<uint32_t>(c, layer, cnt, src_page, src_t, dst_page, dst_t);
     if (c.kv_dtype == SLATE_KV_Q8)
-        for (int hw = tid; hw < 2 * c.n_kv_heads; hw += AT)
-            for (int k = 0; k < cnt; ++k) {
-                if (src_page[k] < 0 || dst_page[k] < 0) continue;
-                const int which = hw / c.n_kv_heads, h = hw % c.n_kv_heads;
-                ((float*)sb_kv_block(c, layer, dst_page[k], which, h))[dst_t[k]] =
-                    ((const float*)sb_kv_block(c, layer, src_page[k], which, h))[src_t[k]];
+        for (int hw = AT - 1 - tid; hw < 2 * c.n_kv_heads; hw += AT) { // the scales, alike, by threads that had fewer columns
+            const int which = hw / c.n_kv_heads, h = hw % c.n_kv_heads;
+            for (int k0 = 0; k0 < cnt; k0 += MU) {
+                float x[MU];
+#pragma unroll
+                for (int u = 0; u < MU; ++u)
+                    if (k0 + u < cnt && src_page[k0 + u] >= 0 && dst_page[k0 + u] >= 0)
+                        x[u] = ((const float*)sb_kv_block(c, layer, src_page[k0 + u], which, h))[src_t[k0 + u]];
+#pragma unroll
+                for (int u = 0; u < MU; ++u)
+                    if (k0 + u < cnt && src_page[k0 + u] >= 0 && dst_page[k0 + u] >= 0)
+                        ((float*)sb_kv_block(c, layer, dst_page[k0 + u], which, h))[dst_t[k0 + u]] = x[u];
             }
+        }
 }
 
 }  // namespace
