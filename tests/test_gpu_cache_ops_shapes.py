@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 import torch
 
+import test_gpu_cache_ops as ops
 from test_gpu_cache_ops import F16, F32, NP, Q8, Cache, attend, check, dev, f32_quant, f32_rotate, plain, random_tree
 
 pytestmark = pytest.mark.gpu
@@ -134,6 +135,49 @@ def test_attention_tree_long_contexts(sb, nodes, ctx, nq, nkv, hd, kv):
     """Items that many workers share, over several row tiles."""
     rng = np.random.default_rng(sum(ctx))
     c = Cache(sb, kv, 1, nkv, hd, [x + n for x, n in zip(ctx, nodes)], seed=9)
+    masks = np.concatenate([sb.tree_masks(random_tree(rng, n)) for n in nodes])
+    q = rng.normal(0, 1, (sum(nodes), nq, hd)).astype(np.float32)
+    check(attend(sb, c, 0, nodes, ctx, masks, q, hd ** -0.5), *plain(c, 0, nodes, ctx, masks, q, hd ** -0.5))
+
+
+@pytest.mark.parametrize("kv", [F32, F16, Q8])
+@pytest.mark.parametrize("hd,nodes", [(64, 8), (64, 16), (64, 20), (64, 32), (128, 9), (128, 16), (128, 32), (64, 64), (128, 64)])
+def test_attention_tree_ignores_what_it_does_not_see_at_every_row_count(sb, hd, nodes, kv):
+    """16 to 128 rows a kv head: each kernel and its limits."""
+    ops.test_attention_tree_ignores_what_it_does_not_see(sb, kv=kv, hd=hd, nodes=nodes)
+
+
+@pytest.mark.parametrize("kv", [F16, Q8])
+@pytest.mark.parametrize("nodes,nq,nkv,hd", [(10, 8, 2, 128), (16, 8, 2, 64), (13, 4, 1, 64), (20, 8, 2, 128)])
+@pytest.mark.parametrize("q_size,v_size,scale", [(1e5, 1.0, 1e-6), (1e-5, 1.0, 1e4), (30.0, 1.0, 0.2), (1.0, 1e-3, 0.1), (1.0, 200.0, 0.1)])
+def test_attention_tree_sizes_of_values_with_many_rows(sb, nodes, nq, nkv, hd, q_size, v_size, scale, kv):
+    rng = np.random.default_rng(nodes)
+    ctx = 500
+    c = Cache(sb, kv, 1, nkv, hd, [ctx + nodes], seed=4)
+    raw = c.raw().copy()
+    if kv == Q8:
+        raw[:, :, 1, :, :64] = (raw[:, :, 1, :, :64].copy().view(np.float32) * np.float32(v_size)).view(np.uint8)
+    else:
+        raw[:, :, 1] = (raw[:, :, 1].copy().view(NP[kv]).astype(np.float32) * np.float32(v_size)).astype(NP[kv]).view(np.uint8)
+    c.pool.copy_(torch.from_numpy(raw.reshape(-1)))
+    masks = sb.tree_masks(random_tree(rng, nodes))
+    q = (rng.normal(0, 1, (nodes, nq, hd)) * q_size).astype(np.float32)
+    check(attend(sb, c, 0, [nodes], [ctx], masks, q, scale), *plain(c, 0, [nodes], [ctx], masks, q, scale))
+
+
+@pytest.mark.parametrize("kv", [F32, F16, Q8])
+@pytest.mark.parametrize("nodes,nq,hd", [(10, 4, 128), (16, 4, 64), (9, 4, 64)])
+@pytest.mark.parametrize("step", [0.5, 40.0, -40.0])
+def test_attention_tree_maxima_that_grow_on_two_lanes(sb, nodes, nq, hd, step, kv):
+    test_attention_tree_maxima_that_grow(sb, nodes, nq, 1, hd, step, kv)
+
+
+@pytest.mark.parametrize("kv", [F32, F16, Q8])
+@pytest.mark.parametrize("nodes,ctx,nq,nkv,hd", [([16], [20011], 4, 1, 64), ([13, 3, 16], [9001, 0, 127], 4, 1, 128), ([12], [1], 8, 2, 128),
+                                                 ([11], [0], 8, 2, 64), ([16, 16], [128, 63], 4, 1, 64)])
+def test_attention_tree_up_to_64_rows(sb, nodes, ctx, nq, nkv, hd, kv):
+    rng = np.random.default_rng(sum(ctx))
+    c = Cache(sb, kv, 1, nkv, hd, [x + n for x, n in zip(ctx, nodes)], seed=11)
     masks = np.concatenate([sb.tree_masks(random_tree(rng, n)) for n in nodes])
     q = rng.normal(0, 1, (sum(nodes), nq, hd)).astype(np.float32)
     check(attend(sb, c, 0, nodes, ctx, masks, q, hd ** -0.5), *plain(c, 0, nodes, ctx, masks, q, hd ** -0.5))
