@@ -139,11 +139,11 @@ constexpr float DIG = 127.f * 65536.f;      // three digits to base 256 stay wit
 
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
 __device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
@@ -655,6 +655,7 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
                     }
                 }
                 odd = __reduce_or_sync(FULL, odd);
+                __syncwarp();                          // other lanes read the words that this one changed
             }
             // ---- o = o corr + p v
             if constexpr (KV == SLATE_KV_F32) {
