@@ -418,11 +418,12 @@ __global__ void __launch_bounds__(AT) tree_accept_kernel(
         }
         if (layer == 0) {
             if (tid == 0) out_count[s] = cnt;
+            const size_t o = (size_t)s * SLATE_TREE_MAX_NODES;       // passes 32 bits from 2^25 sequences
             if (on) {
-                out_node[s * 64 + k] = tid;
-                out_token[s * 64 + k] = target[r0 + tid];
+                out_node[o + k] = tid;
+                out_token[o + k] = target[r0 + tid];
             }
-            if (tid >= cnt) out_node[s * 64 + tid] = out_token[s * 64 + tid] = -1;
+            if (tid >= cnt) out_node[o + tid] = out_token[o + tid] = -1;
         }
     }
     __syncthreads();

@@ -46,3 +46,22 @@ def test_infinities_in_v_of_many_nodes(sb, ctx, nodes, nq, nkv, hd, kv):
         dirty = attend(sb, c, 0, [nodes], [ctx], masks, q, 0.1)
         assert np.array_equal(dirty[others], clean[others])
         assert not np.isfinite(dirty[bad][..., ::3]).any()
+
+
+def test_accept_of_more_sequences_than_32_bits_of_outputs(sb):
+    """The last of 2^25 + 3 sequences: its outputs lie beyond 2^31 elements."""
+    n = (1 << 25) + 3
+    if torch.cuda.mem_get_info()[0] < 4 * (2 * 64 * n) + (4 << 30):
+        pytest.skip("needs 21 GB")
+    c = Cache(sb, F16, 1, 1, 4, [8])
+    off = torch.zeros(n + 1, dtype=torch.int32, device="cuda")
+    off[n] = 2                                           # two nodes of the last sequence, the second one matches
+    slot, ctx, cnt = (torch.zeros(n, dtype=torch.int32, device="cuda") for _ in range(3))
+    mask, parent = dev(np.array([1, 3], np.int64)), dev(np.array([-1, 0], np.int32))
+    token, target = dev(np.array([5, 6], np.int32)), dev(np.array([6, 7], np.int32))
+    node, new = (torch.full((n, 64), -7, dtype=torch.int32, device="cuda") for _ in range(2))
+    tree = sb.TreeBatch(n_seq=n, rows=2, max_nodes=2, row_off=off.data_ptr(), slot=slot.data_ptr(), ctx=ctx.data_ptr(), mask=mask.data_ptr())
+    sb.tree_accept(c.desc, tree, parent.data_ptr(), token.data_ptr(), target.data_ptr(), cnt.data_ptr(), node.data_ptr(), new.data_ptr())
+    assert cnt[:3].tolist() == [0, 0, 0] and cnt[-2:].tolist() == [0, 2]
+    assert node[-1].tolist() == [0, 1] + [-1] * 62 and new[-1].tolist() == [6, 7] + [-1] * 62
+    assert bool((node[:5] == -1).all()) and bool((new[-9:-1] == -1).all())
