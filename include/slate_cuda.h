@@ -194,7 +194,7 @@ int slate_cuda_attention_paged_gqa_noalloc(float* out, const float* q, const int
  * without synchronisation or allocation, so every call can be captured into a
  * graph.  Each returns 0, -1 for bad arguments (before any launch; the message
  * is in slate_cuda_last_error()) or -5 when a launch fails.  head_dim is a
- * multiple of 4 from 4 to 256.  Table entries, slots and indexes are checked on
+ * multiple of 4 from 4 to 256, max_pages at most 2^26.  Table entries, slots and indexes are checked on
  * the device: a token without a page is neither read nor written. */
 typedef struct slate_kv_cache {
     void* pool;                  /* n_layers * n_pages * 2 * n_kv_heads blocks */

@@ -251,8 +251,8 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
             seq_before += seq_units(sq_, nkv);
             sq_ = seq_of(c, tr, ++s, G, MR, unit);
         }
-        const uint32_t rel = (uint32_t)(at - seq_before);     // < 2^31: 2^24 tokens of 64 rows a head at most
-        const int item = (int)(rel / (uint32_t)sq_.units), u0 = (int)(rel % (uint32_t)sq_.units);
+        int u0;
+        const int item = item_of(at - seq_before, sq_.units, u0);
         const int u1 = (int)min((int64_t)sq_.units, u0 + (stop - at));
         const int kvh = item / sq_.tiles, r_base = (item % sq_.tiles) * MR;
         const int n_rows = min(MR, sq_.n * G - r_base);

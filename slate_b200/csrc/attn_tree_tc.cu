@@ -179,9 +179,8 @@ struct Segs {
             seq_before += seq_units(sq, c.n_kv_heads);
             sq = seq_of(c, tr, ++s, G, MR, unit);
         }
-        const uint32_t rel = (uint32_t)(at - seq_before);
-        const int item = (int)(rel / (uint32_t)sq.units);
-        const int u0 = (int)(rel % (uint32_t)sq.units), nu = (int)min((int64_t)sq.units, u0 + (stop - at)) - u0;
+        int u0;
+        const int item = item_of(at - seq_before, sq.units, u0), nu = (int)min((int64_t)sq.units, u0 + (stop - at)) - u0;
         kvh = item / sq.tiles;
         r_base = (item % sq.tiles) * MR;
         n_rows = min(MR, sq.n * G - r_base);

@@ -465,8 +465,8 @@ extern "C" int slate_cuda_rope_append(const slate_kv_cache_t* cache, int layer,
         return -1;
     }
     if (layer < 0 || layer >= cache->n_layers || rows < 0 || n_heads < 1 || !q_out || !q || !k || !v ||
-        !row_slot || !row_index || !row_pos || ld_q < n_heads * hd || ld_q_out < n_heads * hd ||
-        ld_k < nkv * hd || ld_v < nkv * hd) {
+        !row_slot || !row_index || !row_pos || ld_q < (int64_t)n_heads * hd || ld_q_out < (int64_t)n_heads * hd ||
+        ld_k < (int64_t)nkv * hd || ld_v < (int64_t)nkv * hd) {
         sb_set_error("rope_append: bad arguments");
         return -1;
     }
@@ -522,11 +522,12 @@ extern "C" int slate_cuda_kv_read(const slate_kv_cache_t* cache, int layer0, int
         return -1;
     }
     if (rows == 0) return 0;
-    const int64_t warps = (int64_t)n_layers * rows * 2 * cache->n_kv_heads;   // of the scalar kernel
-    if ((warps + 7) / 8 > 0x7fffffff) {
+    const int64_t each = (int64_t)n_layers * 2 * cache->n_kv_heads;          // warps a row of the scalar kernel
+    if (rows > 0x3fffffff8 / each) {                                         // 2^31 - 1 blocks of 8 warps
         sb_set_error("kv_read: %d rows of %d layers are too many", rows, n_layers);
         return -1;
     }
+    const int64_t warps = rows * each;
     const cudaStream_t st = (cudaStream_t)stream;
     const uintptr_t mis = ((uintptr_t)K | (uintptr_t)V) & (out_dtype == SLATE_KV_F16 ? 7 : 15);
     const auto go = [&](auto vec, auto scalar, auto* k, auto* v) {

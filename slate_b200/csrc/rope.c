@@ -5,6 +5,7 @@
 #define _GNU_SOURCE
 #include "sb_internal.h"
 #include "sb_kernels.h"
+#include "sb_kv.h"
 
 #include <math.h>
 
@@ -80,7 +81,7 @@ int slate_tree_masks(uint64_t* mask, const int32_t* parent, int n) {
 int sb_kv_check(const slate_kv_cache_t* c, const char* who) {
     if (!c || !c->pool || !c->page_table || ((uintptr_t)c->pool & 15) || c->n_pages < 1 ||
         c->n_pages > 0x7fffffff || c->n_slots < 1 || c->max_pages < 1 ||
-        c->max_pages > 0x7fffffff / SB_PAGE_TOKENS || c->n_layers < 1 || c->n_kv_heads < 1) {
+        c->max_pages > SB_KV_MAX_PAGES || c->n_layers < 1 || c->n_kv_heads < 1) {
         sb_set_error("%s: bad cache descriptor", who);
         return -1;
     }

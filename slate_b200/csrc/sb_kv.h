@@ -12,6 +12,7 @@
 
 #include "sb_kernels.h"
 
+#define SB_KV_MAX_PAGES (1 << 26)           /* a slot: 2^30 tokens, so that ends and looks ahead stay within an int */
 #define SB_Q8_SCALES (4 * SB_PAGE_TOKENS)   /* bytes of scales in front of a block's int8 rows */
 
 /* Bytes of one (page, K|V, head) block and of one row of it. */

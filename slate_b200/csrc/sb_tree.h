@@ -111,6 +111,12 @@ struct Cut {
         return more + (int)(x < 0x7fffffff ? (uint32_t)x / (uint32_t)each : x / each);
     }
 };
+// The item that holds unit `rel` of a sequence, and the unit's place in it.
+__device__ __forceinline__ int item_of(int64_t rel, int units, int& u0) {
+    const int item = (int)(rel < 0x7fffffff ? (uint32_t)rel / (uint32_t)units : rel / units);
+    u0 = (int)(rel - (int64_t)item * units);
+    return item;
+}
 
 // Where a CTA begins: its units [at, stop), the sequence that holds `at`, the units before
 // that sequence.  False for a CTA without work.  Up to 32 sequences (the calls where the
