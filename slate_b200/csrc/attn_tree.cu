@@ -350,7 +350,9 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
             l[i] = 0.f;
             rs[i] = rowscale[8 * i + g];
         }
-        float vref = 1.f;                              // Q8: o is in units of vref * 2^-15
+        float vtop[RI];                                // 8 bits: row's o is in units of 2^(vtop - 15)
+#pragma unroll
+        for (int i = 0; i < RI; ++i) vtop[i] = -1e30f;
 
         // ---- the warp's tiles: KT tokens each, tiles warp, warp + MW, ...
         const int tiles = (tok1 - tok0 + KT - 1) / KT;
@@ -588,7 +590,8 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
                 for (int j = 0; j < NTK; ++j) mx = fmaxf(mx, fmaxf(p[ri][j][0], p[ri][j][1]));
                 mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 2));
-                const float mn = fmaxf(m[ri], mx), base = mn == -INFINITY ? 0.f : mn;
+                // (8 bits: to the integer above it, so that o's units, powers of two, can be set against it)
+                const float mn = fmaxf(m[ri], KV == SLATE_KV_Q8 ? ceilf(mx) : mx), base = mn == -INFINITY ? 0.f : mn;
                 corr[ri] = ex2(m[ri] - base);
                 m[ri] = mn;
                 l[ri] *= corr[ri];
@@ -600,8 +603,9 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
                         l[ri] += p[ri][j][e];
                     }
             }
-            // ---- weights of v: 8 bits: p vscale / vref (vref: a power of two not below any
-            // vscale met), so that they keep f16's range; 0 stays 0 whatever the scale
+            // ---- weights of v: 8 bits: p vscale against the row's largest so far: that of the tokens which it
+            // sees, with their p, so that no scale that weighs nothing in a row takes the others' bits in f16.
+            // vtop = m + its exponent only grows: o is rescaled by a power of two.  0 stays 0 whatever the scale
             if (KV == SLATE_KV_Q8) {
                 float vf[NTK][2];
 #pragma unroll
@@ -609,26 +613,25 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
                     const float2 x = *(const float2*)(vsc + 8 * j + 2 * t4);
                     vf[j][0] = x.x, vf[j][1] = x.y;
                 }
-                // the tile's largest: lane = token, as bits
-                const float v1 = vsc[lane];
-                const float vm = __uint_as_float(__reduce_max_sync(FULL, t0 + lane < end && v1 > 0.f && v1 < INFINITY ? __float_as_uint(v1) : 0u));
-                if (i == 0 || vm > vref) {
-                    const int e = min(max((int)(__float_as_uint(vm) >> 23) - 126, -80), 126);
-                    const float nref = __int_as_float((127 + e) << 23), f = i ? vref / nref : 0.f;
 #pragma unroll
-                    for (int ri = 0; ri < RI; ++ri) corr[ri] *= f;        // o is rescaled once
-                    vref = nref;
+                for (int ri = 0; ri < RI; ++ri) {
+                    float top = 0.f;
+#pragma unroll
+                    for (int j = 0; j < NTK; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            p[ri][j][e] = tail && p[ri][j][e] == 0.f ? 0.f : p[ri][j][e] * vf[j][e];
+                            top = fmaxf(top, fabsf(p[ri][j][e]));
+                        }
+                    top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
+                    const float grown = fmaxf(vtop[ri], m[ri] + (float)max((int)(__float_as_uint(top) >> 23) - 126, -100));
+                    corr[ri] = __int_as_float((127 + max((int)(vtop[ri] - grown), -126)) << 23);
+                    vtop[ri] = grown;
+                    const float f = __int_as_float((142 + min(max((int)(m[ri] - grown), -129), 100)) << 23);
+#pragma unroll
+                    for (int j = 0; j < NTK; ++j) p[ri][j][0] *= f, p[ri][j][1] *= f;
                 }
-                const float vi = 32768.f / vref;
-#pragma unroll
-                for (int j = 0; j < NTK; ++j)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float f = vf[j][e] * vi;
-#pragma unroll
-                        for (int ri = 0; ri < RI; ++ri)
-                            p[ri][j][e] = tail && p[ri][j][e] == 0.f ? 0.f : p[ri][j][e] * f;
-                    }
             }
             // An infinity or NaN in a v that only some rows see would reach the others as
             // 0 * inf: such values are taken out of the tile and added for the rows that see them.
@@ -813,10 +816,12 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
 
         // ---- join the four warps: [MW][MR][HD + 2]
         float* mg = (float*)ring;
-        const float of = KV == SLATE_KV_Q8 ? vref * 0x1p-15f : KV == SLATE_KV_F16 ? 0x1p-15f : 1.f;
 #pragma unroll
         for (int ri = 0; ri < RI; ++ri) {
             float* rec = mg + ((size_t)warp * MR + 8 * ri + g) * (HD + 2);
+            const float of = KV == SLATE_KV_Q8    ? __int_as_float((112 + min(max((int)(vtop[ri] - m[ri]), -111), 130)) << 23)
+                             : KV == SLATE_KV_F16 ? 0x1p-15f
+                                                  : 1.f;
             float ls = l[ri];
             ls += __shfl_xor_sync(FULL, ls, 1);
             ls += __shfl_xor_sync(FULL, ls, 2);

@@ -51,6 +51,11 @@ constexpr int SCB = 8;                        // tiles whose scales and flags ar
 // The maximum that p is taken against may lag behind the true one by 2^LAG: only then are O and
 // the sum rescaled.  p carries 2^(15 - LAG), so that it stays below f16's end all the same.
 constexpr int LAG = 8;
+// 8 bits: as long as a range's v scales lie within 2^SPAN (and below 2^TALL), p v's factor in f16 is set
+// by the largest of them, for all rows alike: a row's top token then keeps 31 - SPAN bits, and the sum l takes the
+// same factor.  From the first tile on where they do not, each row has its own, by the tokens that it sees and
+// their p, and l none (see `wide`).  Weights and activations leave scales within 2^7 or so.
+constexpr int SPAN = 10, TALL = 40;
 // Tiles that D may add up before it is drained (a power of two).  The tensor cores cut each
 // step's sum off: 8 tiles, 128 steps, cost 1e-6 of the output at worst, one tile 1e-7.
 constexpr int RUN = 8;
@@ -213,8 +218,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
     __shared__ uint32_t tmem_s;
     __shared__ __align__(8) uint8_t gone_s[SCB][8];                // per page: the table has none
     __shared__ uint16_t odd_s[SCB][8];                             // per page: tokens whose v is not finite
-    __shared__ __align__(16) float vmax_s[SCB][8];                 // per page: largest v scale
+    __shared__ uint4 vexp_s[SCB][2];                               // per page, 16 bits: exponent of its largest v scale; 255 - that
+                                                                   // of the smallest (0: it has none)
     __shared__ float part_max[2][PARTS][MR];      // [tile parity][part][row]
+    __shared__ float part_top[Q8 ? 2 : 1][PARTS][Q8 ? MR : 1];     // alike, of score + exponent of the v scale
     __shared__ int need_s[4];                     // tile % 4: some row's maximum grew beyond LAG
     __shared__ int fail_s;
     sb_grid_wait();
@@ -343,7 +350,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
             tc_after();
             const uint64_t mk = rq < n_rows ? __ldg(tr.mask + sq_.r0 + (r_base + rq) / G) : 0;
             float m = -INFINITY, l = 0.f;              // m: what p is taken against, in log2 units
-            int vexp = -80;                            // 8 bits: 2^vexp is above every v scale so far
+            // 8 bits: O is in units of 2^(m + a - (15 - LAG)); 2^a is above every v scale so far, and l's units are
+            // the same; once `wide`, a is the row's own and l's units are 2^(m - (15 - LAG))
+            float a = -80.f;
+            int vlow = 0;                              // 255 - the smallest v scale's exponent so far
+            bool wide = false;
             bool ok = true;
             const auto scales = [&](int j) { return ssc + (tb + j) % SCB * (2 * KT) + toff(); };
             const auto s_part = [&](int j) { return sS((tb + j) & 1) + lanes + toff(); };
@@ -358,6 +369,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                 ok = ok && __all_sync(FULL, bar_wait(&bars.dfull[(tb + j) & 1], phase2(tb + j), fail));
                 tc_after();
             };
+            // 2^exponent is above |x|, and 2^(exponent - 1) not (0: -126, infinity and NaN: 129)
+            const auto exponent = [](float x) { return (int)(__float_as_uint(x) >> 23 & 255) - 126; };
             // every row sees every token of the thread's part of tile j
             const auto seen_by_all = [&](int j) {
                 const uint8_t* gone = &gone_s[(tb + j) % SCB][toff() / 16];
@@ -376,8 +389,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                 }
                 return v;
             };
-            // the largest of 16 scores (8 bits: times the tokens' scales)
-            const auto max16 = [&](auto all, const uint32_t (&x)[16], const float* ks, uint32_t v, float mx) {
+            // the largest of 16 scores (8 bits: times the tokens' scales; top: of score + exponent of the v scale)
+            const auto max16 = [&](auto all, const uint32_t (&x)[16], const float* ks, uint32_t v, float mx, float& top) {
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
                     float y[4] = {__uint_as_float(x[i]), __uint_as_float(x[i + 1]), __uint_as_float(x[i + 2]),
@@ -392,13 +405,19 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             if (!(v >> (i + e) & 1)) y[e] = -INFINITY;
+                    if (Q8 && !all.value && wide) {
+                        const float4 v4 = *(const float4*)(ks + KT + i);
+                        const float vv[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaf(y[e], rs, (float)max(exponent(vv[e]), -80)));
+                    }
                     mx = fmaxf(fmaxf(mx, fmaxf(y[0], y[1])), fmaxf(y[2], y[3]));
                 }
                 return mx;
             };
             // 16 scores to p, as 8 pairs' high halves and then their low halves
             const auto p16 = [&](auto all, const uint32_t (&x)[16], uint32_t (&pk)[16], const float* ks, uint32_t v,
-                                 float2 rs2, float2 nb2, float2& sum) {
+                                 float2 rs2, float2 nb2, float2& sum, float2 pf, float2 vf) {
                 float4 k4, v4;
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
@@ -416,7 +435,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                     }
                     sum = __fadd2_rn(sum, p);
                     if (Q8) {
-                        p = __fmul2_rn(p, i % 4 ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y));
+                        float2 z = i % 4 ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y);
+                        if (!all.value) {
+                            p = __fmul2_rn(p, pf);
+                            z = __fmul2_rn(z, vf);
+                        }
+                        p = __fmul2_rn(p, z);
                         if (!all.value) {                              // 0 stays 0 whatever the scale
                             if (!(v >> i & 1)) p.x = 0.f;
                             if (!(v >> (i + 1) & 1)) p.y = 0.f;
@@ -425,7 +449,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                     split_f16(p.x, p.y, pk[i / 2], pk[8 + i / 2]);
                 }
             };
-            const auto tile_max = [&](auto all, int j) {
+            const auto tile_max = [&](auto all, int j, float& top) {
                 float mx = -INFINITY;
 #pragma unroll
                 for (int cc = 0; cc < TQ / 16; ++cc) {
@@ -433,13 +457,17 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                     tmem_ld(s_part(j) + 16 * cc, x);
                     const uint32_t v = all.value ? 0xffffffffu : seen(j, 16 * cc & ~31) >> (16 * cc & 31);
                     tmem_ld_wait();
-                    mx = max16(all, x, scales(j) + 16 * cc, v, mx);
+                    mx = max16(all, x, scales(j) + 16 * cc, v, mx, top);
                 }
                 return mx;
             };
             // p of tile j, written over the S that it came from, and its sum
             const auto tile_p = [&](auto all, int j) {
-                const float base = (m == -INFINITY ? 0.f : m) - (float)(15 - LAG - (Q8 ? vexp : 0));
+                const float base = (m == -INFINITY ? 0.f : m) - ((float)(15 - LAG) - (Q8 && !wide ? a : 0.f));
+                // the row's own factor 2^-a: with p alone where it is above 1, else half with v's scale, so that
+                // neither overflows
+                const float f = Q8 && !all.value && wide ? ex2(a < 0.f ? -a : -0.5f * a) : 1.f;
+                const float2 pf = make_float2(f, f), vf = a < 0.f ? make_float2(1.f, 1.f) : pf;
                 const float2 rs2 = make_float2(rs, rs), nb2 = make_float2(-base, -base);
                 float2 sum = make_float2(0.f, 0.f);
 #pragma unroll 1
@@ -448,24 +476,24 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                     tmem_ld(s_part(j) + 16 * cc, x);
                     const uint32_t v = all.value ? 0xffffffffu : seen(j, 16 * cc & ~31) >> (16 * cc & 31);
                     tmem_ld_wait();
-                    p16(all, x, pk, scales(j) + 16 * cc, v, rs2, nb2, sum);
+                    p16(all, x, pk, scales(j) + 16 * cc, v, rs2, nb2, sum, pf, vf);
                     tmem_st(s_part(j) + 16 * cc, pk);
                 }
                 return sum.x + sum.y;
             };
-            const auto v_exponent = [&](int j) {
-                const float* v = vmax_s[(tb + j) % SCB];
-                const float4 a = *(const float4*)v, z = *(const float4*)(v + 4);
-                const float vm = fmaxf(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)), fmaxf(fmaxf(z.x, z.y), fmaxf(z.z, z.w)));
-                return min(max((int)(__float_as_uint(vm) >> 23) - 126, -80), 126);
+            const auto of_pages = [&](int j, int k) {
+                const uint4 x = vexp_s[(tb + j) % SCB][k];
+                const uint32_t y = __vmaxu2(__vmaxu2(x.x, x.y), __vmaxu2(x.z, x.w));
+                return (int)max(y & 0xffffu, y >> 16);
             };
             // the part's maximum of tile j for the row's other threads, and whether anything has to be
             // rescaled for it; a barrier
-            const auto publish = [&](int j, float mx) {
+            const auto publish = [&](int j, float mx, float top, float high) {
                 const uint32_t t = tb + j;
                 if (ok && live) {
                     part_max[t & 1][h][r] = mx;
-                    if (mx * rs > m + (float)LAG || (Q8 && v_exponent(j) > vexp)) need_s[t & 3] = 1;
+                    if (Q8 && wide) part_top[Q8 ? t & 1 : 0][h][Q8 ? r : 0] = top;
+                    if (mx * rs > m + (float)LAG || (Q8 && (wide ? top > m + a + (float)LAG : high > a))) need_s[t & 3] = 1;
                 }
                 softmax_sync();
                 if (tid == 0) need_s[(t + 2) & 3] = 0;
@@ -483,10 +511,19 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
             for (int j = 0; j < nt; ++j) {             // to the end even after a failed wait: the barriers count
                 const uint32_t t = tb + j;
                 wait_s(j);
-                const bool all = seen_by_all(j);
-                float mx = -INFINITY;
-                if (ok && live) mx = all ? tile_max(Yes{}, j) : tile_max(No{}, j);
-                publish(j, mx);
+                float high = a;
+                if (Q8 && !wide) {                     // (alike in every thread)
+                    vlow = max(vlow, of_pages(j, 1));
+                    high = fmaxf(a, (float)(of_pages(j, 0) - 126));
+                    if (high > (float)TALL || high + (float)vlow > (float)(SPAN + 129)) {
+                        wide = true;
+                        l *= ex2(a);
+                    }
+                }
+                const bool all = seen_by_all(j) && !wide;
+                float mx = -INFINITY, top = -INFINITY;
+                if (ok && live) mx = all ? tile_max(Yes{}, j, top) : tile_max(No{}, j, top);
+                publish(j, mx, top, high);
                 const bool need = need_s[t & 3];
                 if (j > 0 && (need || j % RUN == 0)) {
                     wait_d(j - 1);
@@ -496,13 +533,23 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                     mx = fmaxf(part_max[t & 1][0][r], part_max[t & 1][1][r]);
                     const float mn = fmaxf(m, mx == -INFINITY ? -INFINITY : mx * rs);
                     float corr = mn == -INFINITY ? 1.f : ex2(m - mn);
+                    const float before = m;
                     m = mn;
-                    if (Q8) {                          // l and O carry 2^(15 - LAG - vexp)
-                        const int e = max(vexp, v_exponent(j));
-                        corr *= ex2((float)(vexp - e));
-                        vexp = e;
+                    if (Q8 && wide) {
+                        l *= corr;
+                        top = fmaxf(part_top[Q8 ? t & 1 : 0][0][Q8 ? r : 0], part_top[Q8 ? t & 1 : 0][1][Q8 ? r : 0]);
+                        if (mn != -INFINITY) {
+                            top = fmaxf(before + a, top);
+                            corr = ex2(before + a - top);
+                            a = top - mn;
+                        }
+                    } else {
+                        if (Q8) {
+                            corr *= ex2(a - high);
+                            a = high;
+                        }
+                        l *= corr;
                     }
-                    l *= corr;
 #pragma unroll
                     for (int i = 0; i < HO; ++i) O[i] *= corr;
                 }
@@ -544,13 +591,17 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                     }
             }
             tb += nt;
+            if (Q8 && wide) {                          // l in O's units again
+                const float f = ex2(-0.5f * a);
+                l = l * f * f;
+            }
             if (live) part_max[0][h][r] = l;
             __syncthreads();                           // every product is done: q and the scales are free
             if constexpr (SPLIT) {
                 const float bad = *fail ? NAN : 0.f;   // a wait ran out: no number may pass for a result
                 if (rq < n_rows) {
                     // l and o carry the same power of two; that of another part may differ
-                    if (h == 0) part_max[1][0][r] = Q8 ? m + (float)vexp : m;
+                    if (h == 0) part_max[1][0][r] = Q8 ? m + a : m;
                     else part_max[1][1][r] = part_max[0][0][r] + part_max[0][1][r] + bad;
                     float* x = (float*)(skv + S::STAGE) + r * (HD + 1) + HO * h;
 #pragma unroll
@@ -584,7 +635,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                     const float bad = *fail ? NAN : 0.f;
                     if (!sg.whole && h == 0) {
                         float* o = ws + ((size_t)(2 * blockIdx.x + (sg.seg ? 1 : 0)) * MR + r) * (HD + 2);
-                        o[0] = Q8 ? m + (float)vexp : m;
+                        o[0] = Q8 ? m + a : m;
                         o[1] = L + bad;
                     }
                     const float f = (sg.whole ? (L == 0.f ? 0.f : 1.f / L) : 1.f);
@@ -732,7 +783,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                         *(uint4*)(dst + (to[i & 1] ^ 16) + TS * i * 128) = z;
                     }
                     if (!(n & 8)) {                    // before kfull: the softmax reads them after the scores
-                        float vm = 0.f;
+                        uint32_t vm = 0, vn = 0;
                         if (lane < 4) {
                             float* sc = ssc + sc_ * 2 * KT + 16 * pg + 4 * lane;
                             *(float4*)sc = k4;
@@ -741,12 +792,16 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                             const float vv[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                if (t + i < end && vv[i] < INFINITY) vm = fmaxf(vm, vv[i]);
+                                if (const uint32_t e = __float_as_uint(vv[i]) >> 23 & 255; t + i < end && vv[i] != 0.f && e < 255) {
+                                    vm = max(vm, e);
+                                    vn = max(vn, 255 - e);
+                                }
                         }
-                        vm = fmaxf(vm, __shfl_xor_sync(FULL, vm, 1));
-                        vm = fmaxf(vm, __shfl_xor_sync(FULL, vm, 2));
+                        vm = __reduce_max_sync(FULL, vm);
+                        vn = __reduce_max_sync(FULL, vn);
                         if (lane == 0) {
-                            vmax_s[sc_][pg] = vm;
+                            ((uint16_t*)&vexp_s[sc_][0])[pg] = (uint16_t)vm;
+                            ((uint16_t*)&vexp_s[sc_][1])[pg] = (uint16_t)vn;
                             gone_s[sc_][pg] = r.page < 0;
                         }
                     }

@@ -65,3 +65,83 @@ def test_accept_of_more_sequences_than_32_bits_of_outputs(sb):
     assert cnt[:3].tolist() == [0, 0, 0] and cnt[-2:].tolist() == [0, 2]
     assert node[-1].tolist() == [0, 1] + [-1] * 62 and new[-1].tolist() == [6, 7] + [-1] * 62
     assert bool((node[:5] == -1).all()) and bool((new[-9:-1] == -1).all())
+
+
+# ------------------------------------------------------------- scales of any size
+def dim0(c, index, k, which=0, slot=0):
+    """The key at `index` becomes k in dim 0 and 0 elsewhere (for every head)."""
+    raw = c.raw().copy()
+    page, t = c.table[slot, index // 16], index % 16
+    row = np.zeros(c.hd)
+    row[0] = k
+    if c.kv == Q8:
+        raw[0, page, which, :, 64 + t * c.hd:64 + (t + 1) * c.hd] = np.where(np.arange(c.hd) == 0, 100, 0).astype(np.int8).view(np.uint8)
+        raw[0, page, which, :, 4 * t:4 * t + 4] = np.array([k / 100], np.float32).view(np.uint8)
+    else:
+        b = c.hd * (2 if c.kv == F16 else 4)
+        raw[0, page, which, :, t * b:(t + 1) * b] = row.astype(NP[c.kv]).view(np.uint8)
+    c.pool.copy_(torch.from_numpy(raw.reshape(-1)))
+
+
+@pytest.mark.parametrize("nodes,nq,nkv,hd", ROWS)
+@pytest.mark.parametrize("size", [1e3, 1e6, 1e12, 1e30])
+@pytest.mark.parametrize("ctx", [40, 700])
+def test_a_large_v_scale_that_a_row_does_not_see(sb, ctx, size, nodes, nq, nkv, hd):
+    """8 bits: a finite scale of a masked node, of any size, takes nothing from the other rows; the row
+    that sees it gets its own sum right."""
+    rng = np.random.default_rng(nodes + ctx)
+    c = Cache(sb, Q8, 1, nkv, hd, [ctx + nodes], seed=3)
+    bad = nodes // 2
+    masks = sb.tree_masks(random_tree(rng, nodes))
+    masks[np.arange(nodes) != bad] &= ~np.uint64(1 << bad)
+    q = rng.normal(0, 1, (nodes, nq, hd)).astype(np.float32)
+    set_rows(c, 1, ctx + bad, size)
+    got = attend(sb, c, 0, [nodes], [ctx], masks, q, hd ** -0.5)
+    want, n = plain(c, 0, [nodes], [ctx], masks, q, hd ** -0.5)
+    others = np.arange(nodes) != bad
+    check(got[others], want[others], n)
+    check(got[bad], want[bad], n)
+
+
+@pytest.mark.parametrize("nodes,nq,nkv,hd", ROWS)
+@pytest.mark.parametrize("size,score", [(1e6, -60.0), (1e12, -80.0), (1e30, -150.0), (1e30, -95.0)])
+@pytest.mark.parametrize("at", [0, 77, 390])
+def test_a_large_v_scale_of_little_weight(sb, at, size, score, nodes, nq, nkv, hd):
+    """8 bits: a token of the context with a large scale and a weight so small that it does not count
+    leaves the others' sum as exact as ever, wherever it lies."""
+    rng = np.random.default_rng(nodes + at)
+    ctx = 391
+    c = Cache(sb, Q8, 1, nkv, hd, [ctx + nodes], seed=3)
+    masks = sb.tree_masks(random_tree(rng, nodes))
+    q = (rng.normal(0, 1, (nodes, nq, hd)) * hd ** -0.5).astype(np.float32)
+    q[..., 0] = 1.0
+    dim0(c, at, score)
+    set_rows(c, 1, at, size)
+    got = attend(sb, c, 0, [nodes], [ctx], masks, q, 1.0)
+    check(got, *plain(c, 0, [nodes], [ctx], masks, q, 1.0))
+
+
+@pytest.mark.parametrize("nodes,nq,nkv,hd", ROWS)
+@pytest.mark.parametrize("slope", [0.05, -0.05, 0.012, -0.012])
+@pytest.mark.parametrize("level", [False, True])
+def test_v_scales_that_grow_along_the_context(sb, level, slope, nodes, nq, nkv, hd):
+    """8 bits: scales of 2^(slope i); `level`: with scores that fall as they rise, so that every token's
+    part of the sum is alike."""
+    rng = np.random.default_rng(nodes)
+    ctx = 1100
+    c = Cache(sb, Q8, 1, nkv, hd, [ctx + nodes], seed=7)
+    e, s = c.parts()
+    for i in range(ctx + nodes):
+        page, t = c.table[0, i // 16], i % 16
+        up = slope * (i if slope > 0 else i - ctx)          # from 2^0 up, or down to 2^0
+        s[0, page, 1, :, t] *= np.float32(2.0 ** up)
+        if level:
+            e[0, page, 0, :, t, 0] = -100
+            s[0, page, 0, :, t] = np.float32(up * np.log(2.0) / 100 + 1e-3)
+    raw = c.raw().copy()
+    raw[..., 64:], raw[..., :64] = e.view(np.uint8).reshape(raw[..., 64:].shape), s.view(np.uint8)
+    c.pool.copy_(torch.from_numpy(raw.reshape(-1)))
+    masks = sb.tree_masks(random_tree(rng, nodes))
+    q = (rng.normal(0, 1, (nodes, nq, hd)) * (0.001 if level else hd ** -0.5)).astype(np.float32)
+    q[..., 0] = 1.0 if level else q[..., 0]
+    check(attend(sb, c, 0, [nodes], [ctx], masks, q, 1.0), *plain(c, 0, [nodes], [ctx], masks, q, 1.0))
