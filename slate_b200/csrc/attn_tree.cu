@@ -984,9 +984,9 @@ int launch_mma(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int
                int ld_out, const float* q, int ld_q, float scale, float* ws, cudaStream_t st) {
     using S = Shape<KV, HD, MODE>;
     const auto k = attn_tree_mma<KV, HD, MODE>;
-    static const cudaError_t ready =
-        cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-    if (ready != cudaSuccess) return sb_cuda_check(ready, "attention_tree shared memory");
+    static unsigned long long ready = 0;
+    const cudaError_t may = sb_allow_smem((const void*)k, S::SMEM, &ready);
+    if (may != cudaSuccess) return sb_cuda_check(may, "attention_tree shared memory");
     const int rc = sb_cuda_check(sb_launch_pdl(k, dim3(S::CPS * SMS), dim3(32 * MW), S::SMEM, st, c, layer, tr, nq, out,
                                                ld_out, q, ld_q, scale, ws),
                                  "attention_tree");

@@ -915,9 +915,9 @@ template <int KV, int HD, bool SPLIT>
 int launch(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq, float* out, int ld_out,
            const float* q, int ld_q, float scale, float* ws, cudaStream_t st) {
     const auto k = attn_tree_tc<KV, HD, SPLIT>;
-    static const cudaError_t ready =
-        cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, TcShape<KV, HD>::SMEM);
-    if (ready != cudaSuccess) return sb_cuda_check(ready, "attention_tree shared memory");
+    static unsigned long long ready = 0;
+    const cudaError_t may = sb_allow_smem((const void*)k, TcShape<KV, HD>::SMEM, &ready);
+    if (may != cudaSuccess) return sb_cuda_check(may, "attention_tree shared memory");
     return sb_cuda_check(sb_launch_pdl(k, dim3(SMS), dim3(NTHREADS), TcShape<KV, HD>::SMEM, st, c, layer, tr, nq,
                                        out, ld_out, q, ld_q, scale, ws),
                          "attention_tree");

@@ -22,6 +22,19 @@
 __device__ __forceinline__ void sb_grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void sb_grid_release() { asm volatile("griddepcontrol.launch_dependents;"); }
 
+/* Lets a kernel have `bytes` of dynamic shared memory on the current device, for which the limit is kept: it is
+ * set once a device (`ready`: a bit for each ordinal below 64; beyond, every time) and again after a failure. */
+static inline cudaError_t sb_allow_smem(const void* kernel, int bytes, unsigned long long* ready) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+    if (__atomic_load_n(ready, __ATOMIC_RELAXED) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) __atomic_fetch_or(ready, bit, __ATOMIC_RELAXED);
+    return e;
+}
+
 template <typename... KArgs, typename... Args>
 static inline cudaError_t sb_launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block,
                                         size_t smem, cudaStream_t st, Args&&... args) {
