@@ -284,7 +284,11 @@ int slate_tree_masks(uint64_t* mask, const int32_t* parent, int n);
  * q[row] over the sequence's context and the nodes that its mask names, with
  * grouped heads (n_heads % n_kv_heads == 0), scores scaled by `scale`.
  * A row that sees nothing gets zeros; what a row does not see has no influence
- * on it, whatever it holds.  ws: slate_cuda_attention_tree_workspace() bytes of
+ * on it, whatever it holds.  Of what it sees, a key whose score is -infinity is as
+ * if not seen; a score of +infinity or NaN makes the row NaN; an infinity or NaN in
+ * v makes that dim of the row it (NaN where infinities differ in sign), whatever
+ * its weight.  Rows that meet such values are computed apart, at a hundredth of the usual
+ * rate.  out and q do not overlap.  ws: slate_cuda_attention_tree_workspace() bytes of
  * device memory, 16-byte aligned, that calls which may overlap do not share. */
 size_t slate_cuda_attention_tree_workspace(const slate_kv_cache_t* cache, int n_heads, int n_seq,
                                            int rows, int max_nodes);

@@ -32,12 +32,6 @@ using namespace sb_tree;
 
 namespace {
 
-__device__ __forceinline__ float element(const unsigned char* blk, int kv_dtype, int at) {
-    return kv_dtype == SLATE_KV_F32   ? ((const float*)blk)[at]
-           : kv_dtype == SLATE_KV_F16 ? __half2float(((const __half*)blk)[at])
-                                      : (float)((const int8_t*)blk)[SB_Q8_SCALES + at];
-}
-
 // Any head_dim: one CTA per (row, query head), its four warps take pages in
 // turn.  A page's scores are formed first, then its maximum joins the running
 // one and its sum of p v is formed by itself before it joins the running sum,
@@ -45,7 +39,7 @@ __device__ __forceinline__ float element(const unsigned char* blk, int kv_dtype,
 // does not see are skipped, so nothing they hold can reach it.  Each row reads the
 // cache by itself: the head_dims that no common model has.
 constexpr int NW = 4;
-__global__ void __launch_bounds__(32 * NW) attn_tree_rows(
+__global__ void __launch_bounds__(32 * NW, 8) attn_tree_rows(
     const slate_kv_cache_t c, int layer, const slate_tree_t tr, int nq, float* __restrict__ out,
     int ld_out, const float* __restrict__ q, int ld_q, float scale) {
     __shared__ float sm[NW], sl[NW], so[NW][256];
@@ -83,9 +77,9 @@ __global__ void __launch_bounds__(32 * NW) attn_tree_rows(
             float s = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (lane + 32 * i < hd) s = fmaf(qv[i], element(kb, c.kv_dtype, t * hd + lane + 32 * i), s);
+                if (lane + 32 * i < hd) s = fmaf(qv[i], kv_element(kb, c.kv_dtype, t * hd + lane + 32 * i), s);
             for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(FULL, s, x);
-            if (c.kv_dtype == SLATE_KV_Q8) s *= ((const float*)kb)[t];
+            if (c.kv_dtype == SLATE_KV_Q8) s *= no_inf(((const float*)kb)[t]);
             if (lane == t) sc = s;
         }
         float mx = sc;
@@ -107,7 +101,7 @@ __global__ void __launch_bounds__(32 * NW) attn_tree_rows(
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (lane + 32 * i < hd)
-                    po[i] = fmaf(pt, element(vb, c.kv_dtype, t * hd + lane + 32 * i), po[i]);
+                    po[i] = fmaf(pt, kv_element(vb, c.kv_dtype, t * hd + lane + 32 * i), po[i]);
         }
         l = fmaf(l, corr, ps);
         m = mn;
@@ -125,11 +119,17 @@ __global__ void __launch_bounds__(32 * NW) attn_tree_rows(
     for (int w = 0; w < NW; ++w) M = fmaxf(M, sm[w]);
     // a warp that saw no key has l = 0 and o = 0
     for (int w = 0; w < NW; ++w) L += sl[w] * (sm[w] == -INFINITY ? 1.f : expf(sm[w] - M));
+    bool nan = false;
     for (int d = tid; d < hd; d += 32 * NW) {
         float O = 0.f;
         for (int w = 0; w < NW; ++w) O += so[w][d] * (sm[w] == -INFINITY ? 1.f : expf(sm[w] - M));
-        out[(size_t)row * ld_out + (size_t)h * hd + d] = L == 0.f ? 0.f : O / L;
+        O = L == 0.f ? 0.f : O / L;
+        nan |= O != O;
+        out[(size_t)row * ld_out + (size_t)h * hd + d] = O;
     }
+    if (__syncthreads_or(nan) && warp == 0)
+        row_by_formula<8>(row_job(c, layer, kvh, slot, ctx, n, mask), q + (size_t)row * ld_q + (size_t)h * hd, scale,
+                       out + (size_t)row * ld_out + (size_t)h * hd);
 }
 
 // ------------------------------------------------------------ tensor-core path
@@ -191,7 +191,7 @@ struct Shape {
     // CTAs an SM: three where 168 registers a thread do (64 sequences of one node over 4096 tokens 54.9
     // us, with two 60.3; head_dim 128 spills, 93 against 84)
     static constexpr int CPS = KV == SLATE_KV_Q8 && HD == 64 && MODE == 0 ? 3 : 2;
-    static_assert(CPS * MR <= TC_ROWS, "workspace");
+    static_assert(CPS * MR <= TC_ROWS && CPS * SMS <= MAX_CTAS, "workspace");
     static constexpr int NS0 = ((CPS == 3 ? 74 : 112) * 1024 - QB) / (MW * TB);
     static constexpr int NS = NS0 > 6 ? 6 : NS0;
     static constexpr int MERGE = MW * MR * (HD + 2) * 4;
@@ -238,6 +238,7 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
     Start st_;
     int unit = UNIT;
     if (!plan_start(c, tr, G, MR, unit, S::SLACK, gridDim.x, buf, st_)) return;
+    if (tid == 0) nan_words(ws, HD)[blockIdx.x] = 0;
     int64_t at = st_.at, seq_before = st_.seq_before;
     const int64_t stop = st_.stop;
     Seq sq_ = st_.sq;
@@ -560,7 +561,7 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
 #pragma unroll
                 for (int j = 0; j < NTK; ++j) {
                     const float2 x = *(const float2*)(ksc + 8 * j + 2 * t4);
-                    kf[j][0] = x.x, kf[j][1] = x.y;
+                    kf[j][0] = no_inf(x.x), kf[j][1] = no_inf(x.y);
                 }
             float corr[RI];
 #pragma unroll
@@ -634,31 +635,44 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
                 }
             }
             // An infinity or NaN in a v that only some rows see would reach the others as
-            // 0 * inf: such values are taken out of the tile and added for the rows that see them.
-            uint32_t odd = 0;
-            if (KV != SLATE_KV_Q8 && tail) {
-                for (int e = lane; e < KT * S::CPR; e += 32) {
-                    const int r = e / S::CPR;
-                    uint32_t* w = (uint32_t*)(st + KT * RB + swz<KV, RB>(r, e % S::CPR));
-                    if (t0 + r < sq_.ctx) continue;
+            // 0 * inf: such values are taken out of the tile (8 bits: their p is 0 already), and the rows that see
+            // them made NaN, to be computed by the formula.
+            if (tail) {
+                uint32_t odd = 0;
+                if (KV == SLATE_KV_Q8)
+                    odd = __ballot_sync(FULL, t0 + lane >= sq_.ctx && t0 + lane < end && !(fabsf(vsc[lane]) < INFINITY));
+                else {
+                    for (int e = lane; e < KT * S::CPR; e += 32) {
+                        const int r = e / S::CPR;
+                        uint32_t* w = (uint32_t*)(st + KT * RB + swz<KV, RB>(r, e % S::CPR));
+                        if (t0 + r < sq_.ctx) continue;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t x = w[k];
-                        uint32_t keep = 0xffffffffu;
-                        if (KV == SLATE_KV_F32) {
-                            if ((x & 0x7f800000u) == 0x7f800000u) keep = 0;
-                        } else {
-                            if ((x & 0x7c00u) == 0x7c00u) keep &= 0xffff0000u;
-                            if ((x & 0x7c000000u) == 0x7c000000u) keep &= 0x0000ffffu;
-                        }
-                        if (keep != 0xffffffffu) {
-                            w[k] = x & keep;
-                            odd |= 1u << r;
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t x = w[k];
+                            uint32_t keep = 0xffffffffu;
+                            if (KV == SLATE_KV_F32) {
+                                if ((x & 0x7f800000u) == 0x7f800000u) keep = 0;
+                            } else {
+                                if ((x & 0x7c00u) == 0x7c00u) keep &= 0xffff0000u;
+                                if ((x & 0x7c000000u) == 0x7c000000u) keep &= 0x0000ffffu;
+                            }
+                            if (keep != 0xffffffffu) {
+                                w[k] = x & keep;
+                                odd |= 1u << r;
+                            }
                         }
                     }
+                    odd = __reduce_or_sync(FULL, odd);
+                    __syncwarp();                      // other lanes read the words that this one changed
                 }
-                odd = __reduce_or_sync(FULL, odd);
-                __syncwarp();                          // other lanes read the words that this one changed
+                if (odd) {
+                    const int x = t0 - sq_.ctx;        // above -32
+#pragma unroll
+                    for (int ri = 0; ri < RI; ++ri) {
+                        const uint64_t mk = rowmask[8 * ri + g];
+                        if (odd & (uint32_t)(x >= 0 ? mk >> x : mk << -x)) l[ri] = NAN;
+                    }
+                }
             }
             // ---- o = o corr + p v
             if constexpr (KV == SLATE_KV_F32) {
@@ -782,32 +796,6 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
                                 o[a][jd + x][e] = fmaf(o[a][jd + x][e], corr[MODE == 0 ? 0 : (2 * a + (e >> 1)) % RI], d[a][x][e]);
                 }
             }
-            if (KV != SLATE_KV_Q8 && odd) {
-                const float f = KV == SLATE_KV_F16 ? 32768.f : 1.f;
-#pragma unroll
-                for (int j = 0; j < NTK; ++j)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        for (int q4 = 0; q4 < 4; ++q4) {
-                            const int r = 8 * j + 2 * q4 + e;
-                            if (!(odd >> r & 1)) continue;
-                            const int page = sb_kv_page(c, sq_.slot, t0 + r);
-                            if (page < 0) continue;
-                            const unsigned char* v = sb_kv_block(c, layer, page, 1, kvh) + (size_t)((t0 + r) & 15) * RB;
-#pragma unroll
-                            for (int ri = 0; ri < RI; ++ri) {
-                                const float pv = __shfl_sync(FULL, p[ri][j][e], (lane & 28) | q4) * f;
-#pragma unroll
-                                for (int jd = 0; jd < NTD; ++jd)
-#pragma unroll
-                                    for (int x = 0; x < 2; ++x) {
-                                        const int d = 8 * jd + 2 * t4 + x;
-                                        const float y = KV == SLATE_KV_F32 ? ((const float*)v)[d] : __half2float(((const __half*)v)[d]);
-                                        if (pv != 0.f && !(fabsf(y) < INFINITY)) o[ri >> 1][jd][2 * (ri & 1) + x] += pv * y;
-                                    }
-                            }
-                        }
-            }
             __syncwarp();                              // the stage is read: it may be filled again
             issue(i + NS - 1);
         }
@@ -856,8 +844,9 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
             }
             if (whole) {
                 const int row = r_base + r;
-                out[(size_t)(sq_.r0 + row / G) * ld_out + (size_t)(kvh * G + row % G) * HD + d] =
-                    L == 0.f ? 0.f : O / L;
+                O = L == 0.f ? 0.f : O / L;
+                out[(size_t)(sq_.r0 + row / G) * ld_out + (size_t)(kvh * G + row % G) * HD + d] = O;
+                if (O != O) nan_words(ws, HD)[blockIdx.x] = 1;
             } else {
                 float* rec = part + (size_t)r * (HD + 2);
                 if (d == 0) {
@@ -870,14 +859,29 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
     }
 }
 
+// Rows row0 + i of sequence s and a kv head, for each bit i of `which`, by a warp.
+template <int E>
+__device__ __forceinline__ void rows_by_formula(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int s, int kvh, int G, int row0,
+                                                uint32_t which, float* out, int ld_out, const float* q, int ld_q, float scale) {
+    const Seq a = seq_of(c, tr, s, G, 1, 1);             // (read anew: the sums have no registers for it)
+    for (; which; which &= which - 1) {
+        const int row = row0 + __ffs(which) - 1, rr = a.r0 + row / G, hd = c.head_dim;
+        const size_t head = (size_t)(kvh * G + row % G) * hd;
+        row_by_formula<E>(row_job(c, layer, kvh, a.slot, a.ctx, a.n, __ldg(tr.mask + rr)), q + (size_t)rr * ld_q + head, scale,
+                          out + (size_t)rr * ld_out + head);
+    }
+}
+
 // Joins the partials of the cut items: a CTA a (sequence, kv head, `rpc` rows), W warps a row,
 // each with every W-th record: lane i forms the weight of the warp's record i, then the lanes
-// sum their dims over the records, eight records in flight.  The loads' latency is what bounds it.
+// sum their dims over the records, F records in flight.  The loads' latency is what bounds it.
+// A row that comes out as NaN, here or in the CTA that wrote it whole, is computed by the formula.
 template <int HD, int W>
 __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) attn_tree_join(
-    const slate_kv_cache_t c, const slate_tree_t tr, int nq, int MR, int unit, int slack, int ctas, int rpc,
-    float* __restrict__ out, int ld_out, const float* __restrict__ ws) {
+    const slate_kv_cache_t c, int layer, const slate_tree_t tr, int nq, int MR, int unit, int slack, int ctas, int rpc,
+    float* __restrict__ out, int ld_out, const float* __restrict__ qs, int ld_q, float scale, const float* __restrict__ ws) {
     constexpr int E = HD / 32;                           // dims a lane: 2 or 4
+    constexpr int F = W == 1 && HD == 128 ? 6 : 8;       // records in flight; 8 would take more than 72 registers there
     __shared__ PlanBuf buf;
     __shared__ float sm[W], sl[W], so[W][HD];
     const int nkv = c.n_kv_heads, G = nq / nkv, tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
@@ -889,10 +893,20 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) attn_tree_join(
     const Cut cut(total, ctas);
     sb_grid_wait();        // the partials; before any return, so that the chain stays ordered
     const int row0 = blockIdx.x % chunks * rpc, w = W == 1 ? 0 : warp;
+    uint32_t again = 0;                                  // the warp's rows that came out as NaN
     for (int row = row0 + (W == 1 ? warp : 0); row < min(row0 + rpc, q.n * G); row += W == 1 ? 4 : 1) {
         const int64_t first = before + (int64_t)(kvh * q.tiles + row / MR) * q.units;
         const int c0 = cut.owner(first), n = cut.owner(first + q.units - 1) - c0 + 1;
-        if (n == 1) continue;                            // written by its CTA
+        const auto place = [&]() { return out + (size_t)(q.r0 + row / G) * ld_out + (size_t)(kvh * G + row % G) * HD; };
+        bool nan = false;
+        if (n == 1) {                                    // written by its CTA
+            if (nan_words(ws, HD)[c0] && w == 0) {
+                const float* o = place();
+                for (int k = 0; k < E; ++k) nan |= o[E * lane + k] != o[E * lane + k];
+                if (__any_sync(FULL, nan)) again |= 1u << (row - row0);
+            }
+            continue;
+        }
         // an item that begins inside its first CTA's range is that CTA's later segment
         const size_t rec = (size_t)MR * (HD + 2);
         const float* base = ws + (size_t)2 * c0 * rec + (size_t)(row % MR) * (HD + 2);
@@ -910,10 +924,10 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) attn_tree_join(
                 f = ml.x == -INFINITY ? 1.f : ex2(ml.x - M);
                 L = fmaf(ml.y, f, L);
             }
-            for (int j0 = 0; j0 < 32 && i0 + W * j0 < n; j0 += 8) {
-                float2 y[8][E / 2];
+            for (int j0 = 0; j0 < 32 && i0 + W * j0 < n; j0 += F) {
+                float2 y[F][E / 2];
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
+                for (int u = 0; u < F; ++u) {
                     const int i = i0 + W * (j0 + u);
                     if (i >= n) break;
 #pragma unroll
@@ -921,7 +935,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) attn_tree_join(
                         y[u][k] = *(const float2*)(base + 2 * i * rec + (i ? 0 : late) + 2 + E * lane + 2 * k);
                 }
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
+                for (int u = 0; u < F; ++u) {
                     if (i0 + W * (j0 + u) >= n) break;
                     const float v = __shfl_sync(FULL, f, j0 + u);
 #pragma unroll
@@ -933,10 +947,15 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) attn_tree_join(
             }
         }
         for (int x = 16; x; x >>= 1) L += __shfl_xor_sync(FULL, L, x);
-        float* o = out + (size_t)(q.r0 + row / G) * ld_out + (size_t)(kvh * G + row % G) * HD;
+        float* o = place();
         if (W == 1) {
 #pragma unroll
-            for (int k = 0; k < E; ++k) o[E * lane + k] = L == 0.f ? 0.f : O[k] / L;
+            for (int k = 0; k < E; ++k) {
+                const float x = L == 0.f ? 0.f : O[k] / L;
+                o[E * lane + k] = x;
+                nan |= x != x;
+            }
+            if (__any_sync(FULL, nan)) again |= 1u << (row - row0);
             continue;
         }
         // (one row a CTA: nothing of a row before it is still read)
@@ -947,7 +966,6 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) attn_tree_join(
 #pragma unroll
         for (int k = 0; k < E; ++k) so[w][E * lane + k] = O[k];
         __syncthreads();
-        if (tid >= HD) return;
         M = -INFINITY, L = 0.f;
         float x = 0.f;
 #pragma unroll
@@ -956,27 +974,31 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) attn_tree_join(
         for (int i = 0; i < W; ++i) {
             const float f = sm[i] == -INFINITY ? 1.f : ex2(sm[i] - M);
             L = fmaf(sl[i], f, L);
-            x = fmaf(so[i][tid], f, x);
+            if (tid < HD) x = fmaf(so[i][tid], f, x);
         }
-        o[tid] = L == 0.f ? 0.f : x / L;
+        x = L == 0.f ? 0.f : x / L;
+        if (tid < HD) o[tid] = x;
+        if (__syncthreads_or(x != x) && w == 0) again = 1;
     }
+    __syncwarp();                                        // the row's lanes change below
+    if (again) rows_by_formula<E>(c, layer, tr, s, kvh, G, row0, again, out, ld_out, qs, ld_q, scale);
 }
 
 template <int HD>
-int join(const slate_kv_cache_t& c, const slate_tree_t& tr, int nq, int MR, int unit, int slack, int ctas, float* out,
-         int ld_out, const float* ws, cudaStream_t st) {
+int join(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq, int MR, int unit, int slack, int ctas, float* out,
+         int ld_out, const float* q, int ld_q, float scale, float* ws, cudaStream_t st) {
     const int R = tr.max_nodes * (nq / c.n_kv_heads);
     // eight warps a row where an item, if long, is cut into eight records or more: one token over 3000
     // tokens of 8 heads 13.5 us against 18.7 with a warp a row (whole calls); more items than that fill
     // the GPU with a warp a row
     if ((int64_t)tr.n_seq * c.n_kv_heads * ((R + MR - 1) / MR) * 8 <= ctas)
         return sb_cuda_check(sb_launch_pdl(attn_tree_join<HD, 8>, dim3((unsigned)(tr.n_seq * R), (unsigned)c.n_kv_heads), dim3(256), 0,
-                                           st, c, tr, nq, MR, unit, slack, ctas, 1, out, ld_out, ws),
+                                           st, c, layer, tr, nq, MR, unit, slack, ctas, 1, out, ld_out, q, ld_q, scale, ws),
                              "attention_tree join");
     const int rpc = R >= 128 ? 16 : 4;
     const dim3 grid((unsigned)(tr.n_seq * ((R + rpc - 1) / rpc)), (unsigned)c.n_kv_heads);
-    return sb_cuda_check(sb_launch_pdl(attn_tree_join<HD, 1>, grid, dim3(128), 0, st, c, tr, nq, MR, unit, slack, ctas, rpc, out,
-                                       ld_out, ws),
+    return sb_cuda_check(sb_launch_pdl(attn_tree_join<HD, 1>, grid, dim3(128), 0, st, c, layer, tr, nq, MR, unit, slack, ctas, rpc, out,
+                                       ld_out, q, ld_q, scale, ws),
                          "attention_tree join");
 }
 template <int KV, int HD, int MODE>
@@ -990,7 +1012,7 @@ int launch_mma(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int
     const int rc = sb_cuda_check(sb_launch_pdl(k, dim3(S::CPS * SMS), dim3(32 * MW), S::SMEM, st, c, layer, tr, nq, out,
                                                ld_out, q, ld_q, scale, ws),
                                  "attention_tree");
-    return rc ? rc : join<HD>(c, tr, nq, S::MR, UNIT, S::SLACK, S::CPS * SMS, out, ld_out, ws, st);
+    return rc ? rc : join<HD>(c, layer, tr, nq, S::MR, UNIT, S::SLACK, S::CPS * SMS, out, ld_out, q, ld_q, scale, ws, st);
 }
 template <int KV, int HD>
 int launch_mode(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq, float* out,
@@ -1006,7 +1028,7 @@ int launch_mode(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, in
         if (KV == SLATE_KV_F32 || M <= few)
             return launch_mma<KV, HD, 2>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);
     const int rc = attend_tc(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);
-    return rc ? rc : join<HD>(c, tr, nq, TC_ROWS, TC_UNIT, TC_SLACK, SMS, out, ld_out, ws, st);
+    return rc ? rc : join<HD>(c, layer, tr, nq, TC_ROWS, TC_UNIT, TC_SLACK, SMS, out, ld_out, q, ld_q, scale, ws, st);
 }
 bool takes_mma(const slate_kv_cache_t* c) { return c->head_dim == 64 || c->head_dim == 128; }
 
@@ -1015,8 +1037,8 @@ bool takes_mma(const slate_kv_cache_t* c) { return c->head_dim == 64 || c->head_
 extern "C" size_t slate_cuda_attention_tree_workspace(const slate_kv_cache_t* cache, int n_heads,
                                                       int n_seq, int rows, int max_nodes) {
     if (!cache || n_heads < 1 || n_seq < 1 || rows < 0 || max_nodes < 1) return 0;
-    // two partials for each CTA: 148 of 128 rows, or 3 * 148 of 8, 2 * 148 of 32 at most
-    return takes_mma(cache) ? (size_t)2 * SMS * TC_ROWS * (cache->head_dim + 2) * 4 : 16;
+    // two partials for each CTA: 148 of 128 rows, or 3 * 148 of 8, 2 * 148 of 32 at most; a word for each
+    return takes_mma(cache) ? 4 * (partial_floats(cache->head_dim) + MAX_CTAS) : 16;
 }
 
 extern "C" int slate_cuda_attention_tree(const slate_kv_cache_t* cache, int layer,

@@ -232,6 +232,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
     int unit = KT;
     if (!plan_start(c, tr, G, MR, unit, TC_SLACK, gridDim.x, buf, st_)) return;
     if (tid == 0) {
+        nan_words(ws, HD)[blockIdx.x] = 0;
         for (int i = 0; i < NB; ++i) {
             bar_init(&bars.kfull[i], 8);          // pages
             bar_init(&bars.vfull[i], 8);
@@ -570,24 +571,16 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
             if (ok && live) {
                 add_d();
                 // f16: infinities and NaN were taken out of the v that only some rows see (the last 64
-                // tokens at most); the rows that see them get them here
+                // tokens at most); a row that sees one becomes NaN, to be computed by the formula
                 if (!Q8)
                     for (int j = max(nt - 2, 0); j < nt; ++j) {
-                        const int t0 = tok0 + j * KT;
-                        if (t0 + KT <= sq_.ctx) continue;
-                        for (int w = 0; w < 8; ++w)
-                            for (uint32_t rest = odd_s[(tb + j) % SCB][w]; rest; rest &= rest - 1) {
-                                const int t = t0 + 16 * w + __ffs(rest) - 1, x = t - sq_.ctx;
-                                const int page = sb_kv_page(c, sq_.slot, t);
-                                if (page < 0 || x < 0 || x >= sq_.n || !(mk >> x & 1)) continue;
-                                if (SPLIT && (w >> 2) != (r >> 6)) continue;   // the other lane's token
-                                const __half* v = (const __half*)sb_kv_block(c, layer, page, 1, kvh) + (t & 15) * HD + HO * h;
-#pragma unroll
-                                for (int i = 0; i < HO; ++i) {
-                                    const float y = __half2float(v[i]);
-                                    if (!(fabsf(y) < INFINITY)) O[i] += y;
-                                }
-                            }
+                        const int x0 = tok0 + j * KT - sq_.ctx;
+                        if (x0 + KT <= 0) continue;
+                        for (int w = 0; w < 8; ++w) {
+                            const int x = x0 + 16 * w;                 // 16 tokens from node x
+                            if (SPLIT && (w >> 2) != (r >> 6)) continue;       // the other lane's tokens
+                            if (x > -16 && x < sq_.n && (odd_s[(tb + j) % SCB][w] & (uint32_t)(x >= 0 ? mk >> x : mk << -x))) l = NAN;
+                        }
                     }
             }
             tb += nt;
@@ -597,6 +590,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
             }
             if (live) part_max[0][h][r] = l;
             __syncthreads();                           // every product is done: q and the scales are free
+            bool nan = false;
             if constexpr (SPLIT) {
                 const float bad = *fail ? NAN : 0.f;   // a wait ran out: no number may pass for a result
                 if (rq < n_rows) {
@@ -625,7 +619,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                         o[-1] = L;
                     }
 #pragma unroll
-                    for (int k = 0; k < HD / 32; ++k) o[lane + 32 * k] = fmaf(x[32 * k], fa, x[64 * (HD + 1) + 32 * k] * fb);
+                    for (int k = 0; k < HD / 32; ++k) {
+                        const float y = fmaf(x[32 * k], fa, x[64 * (HD + 1) + 32 * k] * fb);
+                        o[lane + 32 * k] = y;
+                        nan |= y != y;
+                    }
                 }
             } else {
                 if (r < n_rows) {
@@ -649,9 +647,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                     float* o = sg.whole ? out + (size_t)(sq_.r0 + rr / G) * ld_out + (size_t)(kvh * G + rr % G) * HD
                                         : ws + ((size_t)(2 * blockIdx.x + (sg.seg ? 1 : 0)) * MR + i) * (HD + 2) + 2;
 #pragma unroll
-                    for (int k = 0; k < HD / 32; ++k) o[lane + 32 * k] = ((const float*)(skv + S::STAGE))[i * (HD + 1) + lane + 32 * k];
+                    for (int k = 0; k < HD / 32; ++k) {
+                        const float y = ((const float*)(skv + S::STAGE))[i * (HD + 1) + lane + 32 * k];
+                        o[lane + 32 * k] = y;
+                        nan |= y != y;
+                    }
                 }
             }
+            if (nan) nan_words(ws, HD)[blockIdx.x] = 1;
             if (*fail) break;
         }
     } else {
@@ -786,7 +789,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                         uint32_t vm = 0, vn = 0;
                         if (lane < 4) {
                             float* sc = ssc + sc_ * 2 * KT + 16 * pg + 4 * lane;
-                            *(float4*)sc = k4;
+                            *(float4*)sc = make_float4(no_inf(k4.x), no_inf(k4.y), no_inf(k4.z), no_inf(k4.w));
                             *(float4*)(sc + KT) = v4;
                             const int t = tok0 + j * KT + 16 * pg + 4 * lane;
                             const float vv[4] = {v4.x, v4.y, v4.z, v4.w};
@@ -898,7 +901,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
     __syncthreads();
     if (*fail) {
         // products and copies in flight end before the CTA does; then, what this CTA owed and
-        // did not do: NaN, whole or in part
+        // did not do: NaN, whole or in part, which attn_tree_join has computed by the formula
+        if (tid == 0) nan_words(ws, HD)[blockIdx.x] = 1;
         for (const uint64_t t0 = gtimer(); gtimer() - t0 < WAIT_NS / 100;) {}
         while (next_segment()) {
             for (int e = tid; e < sg.n_rows * (HD + 2); e += NTHREADS) {

@@ -251,9 +251,98 @@ __device__ __forceinline__ uint32_t i8_f16(uint32_t w) {
     return *(const uint32_t*)&h;
 }
 
+// An 8-bit key's infinite scale as NaN: its row holds infinities and, from zeros, NaN.
+__device__ __forceinline__ float no_inf(float x) { return fmaf(0.f, x, x); }
+
+// ---------------------------------------------------------------- rows by the formula itself
+// Products of halves know no infinities (hi * inf + lo * inf, lo of either sign or 0, is NaN where q * inf is not),
+// and a sum of halves neither.  So whatever gave NaN is computed again here, a warp a row, in f32 with sums in
+// f64: a key of score -inf is as if not seen; one of +inf or NaN makes the row NaN; an infinity or NaN in v of a
+// key that is seen makes that dim it, whatever the key's weight.  Rows without such values never come here.
+struct RowJob {
+    const unsigned char* pool;       // block of (layer, page 0, K, kv head)
+    size_t page_step, kv_step;
+    const int32_t* pages;            // of the slot, `last` of them
+    int last, n_pages, hd, kv_dtype, ctx, n;
+    uint64_t mask;
+};
+__device__ __forceinline__ RowJob row_job(const slate_kv_cache_t& c, int layer, int kvh, int slot, int ctx, int n, uint64_t mask) {
+    RowJob j;
+    j.pool = sb_kv_block(c, layer, 0, 0, kvh);
+    j.kv_step = (size_t)c.n_kv_heads * sb_kv_block_bytes(c.kv_dtype, c.head_dim);
+    j.page_step = 2 * j.kv_step;
+    const bool in = slot >= 0 && slot < c.n_slots;
+    j.pages = c.page_table + (in ? (size_t)slot * c.max_pages : 0);
+    j.last = in ? min(c.max_pages, (ctx + n + SB_PAGE_TOKENS - 1) / SB_PAGE_TOKENS) : 0;
+    j.n_pages = (int)c.n_pages;
+    j.hd = c.head_dim;
+    j.kv_dtype = c.kv_dtype;
+    j.ctx = ctx;
+    j.n = n;
+    j.mask = mask;
+    return j;
+}
+__device__ __forceinline__ float kv_element(const unsigned char* blk, int kv_dtype, int at) {
+    return kv_dtype == SLATE_KV_F32   ? ((const float*)blk)[at]
+           : kv_dtype == SLATE_KV_F16 ? __half2float(((const __half*)blk)[at])
+                                      : (float)((const int8_t*)blk)[SB_Q8_SCALES + at];
+}
+// E: dims a lane, head_dim up to 32 E
+template <int E>
+__device__ __forceinline__ void row_by_formula(const RowJob& j, const float* q, float scale, float* out) {
+    const int lane = threadIdx.x & 31;
+    const bool q8 = j.kv_dtype == SLATE_KV_Q8;
+    float qv[E], top = -INFINITY;
+    double o[E], l = 0.;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        qv[i] = lane + 32 * i < j.hd ? q[lane + 32 * i] * scale : 0.f;
+        o[i] = 0.;
+        nan |= qv[i] != qv[i];
+    }
+    nan = __any_sync(FULL, nan);
+#pragma unroll 1
+    for (uint32_t x = 0, len = 16u * j.last; x < 2 * len && !nan; ++x) {       // the maximum, then the sums
+        const bool sums = x >= len;
+        const int at = sums ? x - len : x, page = __ldg(j.pages + at / 16), node = at - j.ctx;
+        if (page < 0 || page >= j.n_pages || node >= j.n || (node >= 0 && !(j.mask >> node & 1))) continue;
+        const unsigned char *kb = j.pool + page * j.page_step, *vb = kb + j.kv_step;
+        const int t = at % 16;
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (lane + 32 * i < j.hd) s = fmaf(qv[i], kv_element(kb, j.kv_dtype, t * j.hd + lane + 32 * i), s);
+        for (int y = 16; y; y >>= 1) s += __shfl_xor_sync(FULL, s, y);
+        if (q8) s *= no_inf(((const float*)kb)[t]);
+        if (s == -INFINITY) continue;
+        nan = !(s < INFINITY);
+        if (!sums) {
+            top = fmaxf(top, s);
+            continue;
+        }
+        const float p = expf(s - top), vs = q8 ? ((const float*)vb)[t] : 1.f;
+        l += p;
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (lane + 32 * i < j.hd) {
+                const float v = kv_element(vb, j.kv_dtype, t * j.hd + lane + 32 * i) * vs;
+                o[i] += (double)(fabsf(v) < INFINITY ? p : 1.f) * v;   // (an infinity is one whatever its weight)
+            }
+    }
+    const float inv = l == 0. ? 0.f : 1.f / (float)l;
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+        if (lane + 32 * i < j.hd) out[lane + 32 * i] = nan ? NAN : (float)(o[i] * inv);
+}
+
 // attn_tree_tc.cu: rows in tiles of TC_ROWS, units of TC_UNIT tokens, SMS CTAs; two
-// partials of TC_ROWS x (head_dim + 2) floats for each in ws.
-constexpr int TC_ROWS = 128, TC_UNIT = 128, TC_SLACK = 4;
+// partials of TC_ROWS x (head_dim + 2) floats for each in ws.  Behind the partials, a word a CTA: some row that it
+// wrote whole holds NaN (attn_tree_join looks for it).
+constexpr int TC_ROWS = 128, TC_UNIT = 128, TC_SLACK = 4, MAX_CTAS = 3 * SMS;
+__host__ __device__ constexpr size_t partial_floats(int hd) { return (size_t)2 * SMS * TC_ROWS * (hd + 2); }
+__device__ __forceinline__ int* nan_words(float* ws, int hd) { return (int*)(ws + partial_floats(hd)); }
+__device__ __forceinline__ const int* nan_words(const float* ws, int hd) { return (const int*)(ws + partial_floats(hd)); }
 int attend_tc(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq, float* out, int ld_out,
               const float* q, int ld_q, float scale, float* ws, cudaStream_t st);
 

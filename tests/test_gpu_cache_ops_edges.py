@@ -145,3 +145,116 @@ def test_v_scales_that_grow_along_the_context(sb, level, slope, nodes, nq, nkv, 
     q = (rng.normal(0, 1, (nodes, nq, hd)) * (0.001 if level else hd ** -0.5)).astype(np.float32)
     q[..., 0] = 1.0 if level else q[..., 0]
     check(attend(sb, c, 0, [nodes], [ctx], masks, q, 1.0), *plain(c, 0, [nodes], [ctx], masks, q, 1.0))
+
+
+# ------------------------------------------------------------- infinities that a row sees
+def formula(c, nodes, ctx, masks, q, scale):
+    """The formula in f64 with infinities and NaN: a key of score -inf is as if not seen; one of +inf or NaN
+    makes the row NaN; an infinity or NaN in v of a key that is seen makes that dim it (NaN: where signs differ)."""
+    out, r = np.zeros(q.shape), 0
+    values = c.values()
+    with np.errstate(all="ignore"):
+        for s, n in enumerate(nodes):
+            K, V = c.rows(0, s, ctx[s] + n, values)
+            for i in range(n):
+                see = np.r_[np.arange(ctx[s]), ctx[s] + np.array([j for j in range(n) if int(masks[r]) >> j & 1], int)].astype(int)
+                for h in range(q.shape[1]):
+                    k, v = K[see, h // (q.shape[1] // c.nkv)], V[see, h // (q.shape[1] // c.nkv)]
+                    z = (k * q[r, h].astype(np.float64)).sum(-1) * scale
+                    v, z = v[z != -np.inf], z[z != -np.inf]
+                    if not len(z):
+                        continue
+                    p = np.exp(z - z.max())
+                    fin = np.isfinite(v)
+                    out[r, h] = (p @ np.where(fin, v, 0)) / p.sum() + np.where(fin, 0, v).sum(0)
+                r += 1
+    return out
+
+
+def check_values(got, want, size):
+    """The same infinities and NaN, and the numbers beside them within the usual bound."""
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.array_equal(np.isposinf(got), np.isposinf(want)) and np.array_equal(np.isneginf(got), np.isneginf(want))
+    fin = np.isfinite(want)
+    check(np.where(fin, got, 0), np.where(fin, want, 0), size)
+
+
+def edge_case(sb, kv, nodes, nq, nkv, hd, ctx=150):
+    rng = np.random.default_rng(nodes + hd)
+    c = Cache(sb, kv, 1, nkv, hd, [ctx + nodes], seed=3)
+    masks = sb.tree_masks(random_tree(rng, nodes))
+    q = (rng.normal(0, 1, (nodes, nq, hd)) * hd ** -0.5).astype(np.float32)
+    q[..., 0] = 1.0
+    size = plain(c, 0, [nodes], [ctx], masks, q, 1.0)[1]
+    return c, masks, q, size
+
+
+@pytest.mark.parametrize("kv", [F32, F16])
+@pytest.mark.parametrize("nodes,nq,nkv,hd", ROWS)
+@pytest.mark.parametrize("at", [3, 149, 152])
+def test_a_key_of_score_minus_infinity_weighs_nothing(sb, at, nodes, nq, nkv, hd, kv):
+    """In the context and among the nodes; its v, an infinity too, does not count either."""
+    c, masks, q, size = edge_case(sb, kv, nodes, nq, nkv, hd)
+    for inf_v in (False, True):
+        set_rows(c, 0, at, np.where(np.arange(hd) == 0, -np.inf, 1.0))
+        if inf_v:
+            set_rows(c, 1, at, -np.inf)
+        want = formula(c, [nodes], [150], masks, q, 1.0)
+        assert np.isfinite(want).all()
+        check_values(attend(sb, c, 0, [nodes], [150], masks, q, 1.0), want, size)
+
+
+@pytest.mark.parametrize("kv", [F32, F16])
+@pytest.mark.parametrize("nodes,nq,nkv,hd", ROWS)
+def test_infinite_v_that_rows_see(sb, nodes, nq, nkv, hd, kv):
+    """Dims of v that are infinite in the context, in one node, in tokens of opposite signs, in tokens whose weight
+    is too small for f32: each shows where the row sees it, the other dims keep their sums."""
+    c, masks, q, size = edge_case(sb, kv, nodes, nq, nkv, hd)
+    v = np.full(hd, 0.5)
+    v[3], v[5], v[7] = np.inf, -np.inf, np.nan
+    set_rows(c, 1, 20, v)
+    w = np.full(hd, -0.25)
+    w[5], w[9], w[11] = np.inf, np.inf, -np.inf
+    set_rows(c, 1, 140, w)
+    u = np.full(hd, 0.125)
+    u[13], u[9] = -np.inf, np.inf
+    set_rows(c, 1, 152, u)                              # a node
+    dim0(c, 100, -300.0)                                # weights that f32 does not hold, in the context ...
+    set_rows(c, 1, 100, np.where(np.arange(hd) == 15, np.inf, 1.0))
+    dim0(c, 153, -300.0)                                # ... and in a node
+    set_rows(c, 1, 153, np.where(np.arange(hd) == 2, -np.inf, 1.0))
+    check_values(attend(sb, c, 0, [nodes], [150], masks, q, 1.0), formula(c, [nodes], [150], masks, q, 1.0), 2 * size)
+
+
+@pytest.mark.parametrize("kv", [F32, F16, Q8])
+@pytest.mark.parametrize("nodes,nq,nkv,hd", ROWS)
+@pytest.mark.parametrize("x", [np.inf, np.nan])
+def test_scores_that_are_no_numbers(sb, x, nodes, nq, nkv, hd, kv):
+    """A score of +inf or NaN makes the rows that see it NaN and no others."""
+    c, masks, q, size = edge_case(sb, kv, nodes, nq, nkv, hd)
+    set_rows(c, 0, 152, x if kv == Q8 else np.where(np.arange(hd) == 0, x, 1.0))
+    want = formula(c, [nodes], [150], masks, q, 1.0)
+    sees = masks >> np.uint64(2) & np.uint64(1) > 0
+    if kv == Q8:                                        # an infinite scale: infinities of both signs
+        want[sees] = np.nan
+    assert np.isnan(want[sees]).all() and np.isfinite(want[~sees]).all()
+    check_values(attend(sb, c, 0, [nodes], [150], masks, q, 1.0), want, size)
+
+
+@pytest.mark.parametrize("nodes,nq,nkv,hd", ROWS)
+@pytest.mark.parametrize("x", [np.inf, np.nan])
+@pytest.mark.parametrize("score", [0.0, -300.0])
+def test_8_bit_v_that_is_no_number(sb, score, x, nodes, nq, nkv, hd):
+    """A v row that the append wrote from an infinity or NaN (such a scale, integers of 0) makes the rows that see it
+    NaN, whatever their weight."""
+    c, masks, q, size = edge_case(sb, Q8, nodes, nq, nkv, hd)
+    dim0(c, 152, score)
+    dim0(c, 152, 1.0, which=1)
+    e, s = c.parts()
+    e[0, c.table[0, 9], 1, :, 8] = 0
+    raw = c.raw().copy()
+    raw[..., 64:] = e.view(np.uint8).reshape(raw[..., 64:].shape)
+    c.pool.copy_(torch.from_numpy(raw.reshape(-1)))
+    set_rows(c, 1, 152, x)
+    want = formula(c, [nodes], [150], masks, q, 1.0)
+    check_values(attend(sb, c, 0, [nodes], [150], masks, q, 1.0), want, size)
