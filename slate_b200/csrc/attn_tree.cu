@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
             }
             top = __reduce_max_sync(FULL, top);
             // exponent of the maximum, kept where 2^-e and 2^e are normal numbers
-            const int e = min(max((int)(top >> 23) - 127, -100), 100);
+            const int e = min(max((int)(top >> 23) - 127, -126), 126);
             const float inv = __int_as_float((127 - e) << 23);
             if (lane == 0) rowscale[r] = scale * 1.4426950408889634f * __int_as_float((127 + e) << 23);
             if constexpr (S::I8) {
@@ -290,11 +290,11 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
                 // -128 .. 127.  Dims 32 ks + 16 hi + 4 t + b are byte b of register 2 hi (+ 1: row + 8)
                 // of lane (row % 8, t).  Up to 8 rows: operand 0 holds the top digit in its rows 0-7 and
                 // the middle one in rows 8-15, operand 1 the low digit; else an operand a digit.
-                const float f = inv * (0.5f * DIG);
-                if (lane == 0) rowscale[r] = top < 0x7f800000u ? rowscale[r] * (2.f / DIG) : NAN;
+                // (a maximum of 2^127 and more has no digits: by the formula)
+                if (lane == 0) rowscale[r] = top < 0x7f000000u ? rowscale[r] * (2.f / DIG) : NAN;
 #pragma unroll
                 for (int i = 0; i < HD / 32; ++i) {
-                    const int d = lane * (HD / 32) + i, v0 = __float2int_rn(v[i] * f);
+                    const int d = lane * (HD / 32) + i, v0 = __float2int_rn(v[i] * inv * (0.5f * DIG));
                     const int d0 = (int8_t)v0, v1 = (v0 - d0) >> 8, d1 = (int8_t)v1, d2 = (v1 - d1) >> 8;
                     const int reg = (d >> 4 & 1) * 2, at = ((r & 7) * 4 + (d >> 2 & 3)) * 16 + (d & 3);
                     int8_t* f8 = (int8_t*)(sq + (size_t)(d / 32) * S::HL * 32);

@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
             uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < PARTS; ++i) top = max(top, __float_as_uint(part_max[0][i][r]));
-            const int qe = min(max((int)(top >> 23) - 127, -100), 100);
+            const int qe = min(max((int)(top >> 23) - 127, -126), 126);
             const float rs = fabsf(scale) * 1.4426950408889634f * __int_as_float((127 + qe) << 23);
             {
                 const float inv = copysignf(__int_as_float((127 - qe) << 23), scale);

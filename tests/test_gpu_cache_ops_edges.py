@@ -258,3 +258,14 @@ def test_8_bit_v_that_is_no_number(sb, score, x, nodes, nq, nkv, hd):
     set_rows(c, 1, 152, x)
     want = formula(c, [nodes], [150], masks, q, 1.0)
     check_values(attend(sb, c, 0, [nodes], [150], masks, q, 1.0), want, size)
+
+
+# ------------------------------------------------------------- queries
+@pytest.mark.parametrize("kv", [F32, F16, Q8])
+@pytest.mark.parametrize("nodes,nq,nkv,hd", ROWS)
+@pytest.mark.parametrize("e", [-120, -104, 101, 112, 120])
+def test_queries_of_any_exponent(sb, e, nodes, nq, nkv, hd, kv):
+    c, masks, q, size = edge_case(sb, kv, nodes, nq, nkv, hd)
+    s = 0.1 * 2.0 ** -e
+    check(attend(sb, c, 0, [nodes], [150], masks, (q * np.float32(2.0 ** e)).astype(np.float32), s),
+          plain(c, 0, [nodes], [150], masks, q, 0.1)[0], size)
