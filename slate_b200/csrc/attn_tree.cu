@@ -7,15 +7,19 @@
 //
 // The M = nodes * group rows that share a kv head are one matrix product with the
 // cache: attn_tree_mma (head_dim 64 and 128) reads the cache once for up to 32 of
-// them and multiplies on the tensor cores; attn_tree_rows takes any head_dim.
+// them (16 at head_dim 128 on f16 and 8 bits, where attn_tree_tc takes the others) and multiplies on the tensor
+// cores; attn_tree_rows takes any head_dim.
 //
 // f32-level products from 16-bit operands.  f16 and 8-bit cache: k and v are
 // exact in f16 (8 bits: the integer; its scale joins the score, or p).  q and p
-// are split into f16 hi + lo (x = hi + lo to ~22 bits), so two products carry
+// are split into f16 hi + lo, so two products carry
 // what f32 would.  To stay clear of f16's ends each q row is first divided by the
-// power of two below its largest element, and p (at most 1) multiplied by 2^15, so
-// that the lo half of a p of 2^-10 still has its bits.  f32 cache: tf32 hi + lo of
-// both sides, three products.  The running sums stay in f32 registers: every tile's
+// power of two that leaves its largest element at 2^14 or more, and p (at most 1) multiplied by 2^15: an
+// element down to 2^-18 of the largest keeps 22 bits, a smaller one is off by 2^-40 of the largest at most.
+// 8 bits, up to 16 rows: q as integers of four 8-bit digits, each element off by 2^-24 of itself and 2^-31 of the
+// row's largest.  f32 cache: tf32 hi + lo of
+// both sides (22 bits whatever the size), three products, lo lo left out: 2^-22 of a product.  The running sums stay in
+// f32 registers: every tile's
 // product is formed from zero and added by one FMA with the rescale, because a
 // tensor-core accumulator carried over thousands of tokens would truncate each time.
 #include <cuda_runtime.h>
@@ -135,7 +139,7 @@ __global__ void __launch_bounds__(32 * NW, 8) attn_tree_rows(
 // ------------------------------------------------------------ tensor-core path
 constexpr int UNIT = 64;
 constexpr int MW = 4;                       // warps a CTA
-constexpr float DIG = 127.f * 65536.f;      // three digits to base 256 stay within 8 bits each
+constexpr float DIG = 127.f * 0x1p24f;      // four digits to base 256 stay within 8 bits each
 
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -183,10 +187,10 @@ struct Shape {
     static constexpr int TB = 2 * KT * RB + (KV == SLATE_KV_Q8 ? 8 * KT : 0);
     static constexpr int MT = MODE == 2 ? 2 : 1;
     static constexpr int MR = MODE == 0 ? 8 : 16 * MT;              // rows a tile
-    // 8 bits and up to 16 rows: scores from integer products, q in three 8-bit digits
+    // 8 bits and up to 16 rows: scores from integer products, q in four 8-bit digits
     static constexpr bool I8 = KV == SLATE_KV_Q8 && MODE < 2;
     static constexpr int KS = I8 ? HD / 32 : KV == SLATE_KV_F32 ? HD / 8 : HD / 16;    // k steps of a score
-    static constexpr int HL = I8 ? MODE + 2 : MODE == 0 ? 1 : 2;    // A operands a k step
+    static constexpr int HL = I8 ? 2 * MODE + 2 : MODE == 0 ? 1 : 2;    // A operands a k step
     static constexpr int QB = MT * KS * HL * 512;
     // CTAs an SM: three where 168 registers a thread do (64 sequences of one node over 4096 tokens 54.9
     // us, with two 60.3; head_dim 128 spills, 93 against 84)
@@ -260,7 +264,7 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
         const int end = sq_.ctx + sq_.n, tok0 = u0 * unit, tok1 = min(end, u1 * unit);
         at += u1 - u0;
 
-        // ---- q as A fragments, each row divided by the power of two below its maximum
+        // ---- q as A fragments, each row divided by a power of two
         __syncthreads();                               // the last segment's merge is read
         if (tid < MR) rowmask[tid] = tid < n_rows ? __ldg(tr.mask + sq_.r0 + (r_base + tid) / G) : 0;
         float qv[MR / MW][HD / 32];                    // all of the warp's rows before any is used
@@ -282,32 +286,29 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
             }
             top = __reduce_max_sync(FULL, top);
             // exponent of the maximum, kept where 2^-e and 2^e are normal numbers
-            const int e = min(max((int)(top >> 23) - 127, -126), 126);
+            constexpr int UP = KV == SLATE_KV_F32 || S::I8 ? 0 : 14;
+            const int e = min(max((int)(top >> 23) - 127, UP - 126), 126) - UP;
             const float inv = __int_as_float((127 - e) << 23);
             if (lane == 0) rowscale[r] = scale * 1.4426950408889634f * __int_as_float((127 + e) << 23);
             if constexpr (S::I8) {
-                // q / 2^(e + 1) (below 1) times DIG as an integer of three digits to base 256, each in
-                // -128 .. 127.  Dims 32 ks + 16 hi + 4 t + b are byte b of register 2 hi (+ 1: row + 8)
-                // of lane (row % 8, t).  Up to 8 rows: operand 0 holds the top digit in its rows 0-7 and
-                // the middle one in rows 8-15, operand 1 the low digit; else an operand a digit.
+                // q / 2^(e + 1) (below 1) times DIG as an integer of four digits to base 256, each in
+                // -128 .. 127: an element is off by 2^-24 of itself (the factor 127) and 2^-31 of the row's largest.
+                // Dims 32 ks + 16 hi + 4 t + b are byte b of register 2 hi (+ 1: row + 8)
+                // of lane (row % 8, t).  Up to 8 rows: an operand holds a digit in its rows 0-7 and the next lower
+                // one in rows 8-15; else an operand a digit.
                 // (a maximum of 2^127 and more has no digits: by the formula)
                 if (lane == 0) rowscale[r] = top < 0x7f000000u ? rowscale[r] * (2.f / DIG) : NAN;
 #pragma unroll
                 for (int i = 0; i < HD / 32; ++i) {
                     const int d = lane * (HD / 32) + i, v0 = __float2int_rn(v[i] * inv * (0.5f * DIG));
-                    const int d0 = (int8_t)v0, v1 = (v0 - d0) >> 8, d1 = (int8_t)v1, d2 = (v1 - d1) >> 8;
+                    const int d0 = (int8_t)v0, v1 = (v0 - d0) >> 8, d1 = (int8_t)v1, v2 = (v1 - d1) >> 8, d2 = (int8_t)v2;
+                    const int digit[4] = {(v2 - d2) >> 8, d2, d1, d0};
                     const int reg = (d >> 4 & 1) * 2, at = ((r & 7) * 4 + (d >> 2 & 3)) * 16 + (d & 3);
                     int8_t* f8 = (int8_t*)(sq + (size_t)(d / 32) * S::HL * 32);
-                    if (MODE == 0) {
-                        f8[at + 4 * reg] = (int8_t)d2;
-                        f8[at + 4 * (reg + 1)] = (int8_t)d1;
-                        f8[512 + at + 4 * reg] = (int8_t)d0;
-                        f8[512 + at + 4 * (reg + 1)] = 0;
-                    } else {
-                        const int up8 = r >> 3 & 1;
-                        f8[at + 4 * (reg + up8)] = (int8_t)d2;
-                        f8[512 + at + 4 * (reg + up8)] = (int8_t)d1;
-                        f8[1024 + at + 4 * (reg + up8)] = (int8_t)d0;
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        const int op = MODE == 0 ? h / 2 : h, up8 = MODE == 0 ? h % 2 : r >> 3 & 1;
+                        f8[512 * op + at + 4 * (reg + up8)] = (int8_t)digit[h];
                     }
                 }
             } else {
@@ -316,6 +317,8 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
 #pragma unroll
             for (int i = 0; i < HD / 32; ++i) {
                 const int d = lane * (HD / 32) + i;
+                // (f16 halves: y of 2^14 and more for the row's largest, so that the low halves of elements down to
+                // 2^-18 of it have all of their bits)
                 const float y = v[i] * inv;
                 if (KV == SLATE_KV_F32) {
                     // k steps 2j, 2j + 1 hold dims 16j + 4 t4 + {0, 1} and {2, 3}
@@ -505,10 +508,11 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
                 for (int j = 0; j < NTK; ++j)
 #pragma unroll
                     for (int e = 0; e < (MODE == 0 ? 2 : 4); ++e) {
-                        const float d2 = __int_as_float(acc[0][j][e]) - BIAS;
-                        const float d1 = __int_as_float(acc[MODE == 0 ? 0 : 1][j][MODE == 0 ? 2 + e : e]) - BIAS;
-                        const float d0 = __int_as_float(acc[S::HL - 1][j][e]) - BIAS;
-                        sc[0][j][e] = fmaf(fmaf(d2, 256.f, d1), 256.f, d0);
+                        float x = 0.f;
+#pragma unroll
+                        for (int h = 0; h < 4; ++h)
+                            x = fmaf(x, 256.f, __int_as_float(acc[MODE == 0 ? h / 2 : h][j][MODE == 0 ? 2 * (h % 2) + e : e]) - BIAS);
+                        sc[0][j][e] = x;
                     }
             } else {
                 // an ldmatrix.x4 brings two 8-token tiles: f16 of one k step, 8 bits of two

@@ -296,7 +296,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
             const auto toff = [&]() { return TQ * h + (SPLIT ? r & 64 : 0); };     // the thread's first token of a tile
             const bool live = ((warp & 3) * 32 & RMASK) < n_rows;       // of the warp
             const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-            // ---- q, each row divided by the power of two below its maximum; scale's sign joins q
+            // ---- q, each row divided by a power of two, so that its halves have their bits down to 2^-18 of its
+            // ---- maximum; scale's sign joins q
             // ---- (a row at a time through the K and V tiles, which nobody else uses yet: a thread that
             // read its own row would ask for a sector an element)
             float O[HO];
@@ -331,7 +332,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
             uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < PARTS; ++i) top = max(top, __float_as_uint(part_max[0][i][r]));
-            const int qe = min(max((int)(top >> 23) - 127, -126), 126);
+            const int qe = min(max((int)(top >> 23) - 127, -112), 126) - 14;   // the largest becomes 2^14 to 2^15
             const float rs = fabsf(scale) * 1.4426950408889634f * __int_as_float((127 + qe) << 23);
             {
                 const float inv = copysignf(__int_as_float((127 - qe) << 23), scale);

@@ -269,3 +269,25 @@ def test_queries_of_any_exponent(sb, e, nodes, nq, nkv, hd, kv):
     s = 0.1 * 2.0 ** -e
     check(attend(sb, c, 0, [nodes], [150], masks, (q * np.float32(2.0 ** e)).astype(np.float32), s),
           plain(c, 0, [nodes], [150], masks, q, 0.1)[0], size)
+
+
+@pytest.mark.parametrize("kv", [F32, F16, Q8])
+@pytest.mark.parametrize("nodes,nq,nkv,hd", ROWS)
+@pytest.mark.parametrize("outlier", [1e3, 2e4])
+def test_queries_with_one_large_dim(sb, outlier, nodes, nq, nkv, hd, kv):
+    """A dim that is `outlier` times the others and meets keys of 0 there: the others' products keep f32's exactness."""
+    rng = np.random.default_rng(nodes)
+    ctx = 600
+    c = Cache(sb, kv, 1, nkv, hd, [ctx + nodes], seed=3)
+    e, s = c.parts()
+    e[:, :, 0, :, :, 5] = 0
+    raw = c.raw().copy()
+    if kv == Q8:
+        raw[..., 64:] = e.view(np.uint8).reshape(raw[..., 64:].shape)
+    else:
+        raw = np.ascontiguousarray(e).view(np.uint8).reshape(raw.shape)
+    c.pool.copy_(torch.from_numpy(raw.reshape(-1)))
+    masks = sb.tree_masks(random_tree(rng, nodes))
+    q = rng.normal(0, 1, (nodes, nq, hd)).astype(np.float32)
+    q[..., 5] = outlier
+    check(attend(sb, c, 0, [nodes], [ctx], masks, q, hd ** -0.5), *plain(c, 0, [nodes], [ctx], masks, q, hd ** -0.5))
