@@ -269,7 +269,8 @@ int slate_cuda_kv_read(const slate_kv_cache_t* cache, int layer0, int n_layers, 
 #define SLATE_TREE_MAX_NODES 64
 typedef struct slate_tree {
     int n_seq, rows;             /* rows = row_off[n_seq] */
-    int max_nodes;               /* of a sequence, 1..64; picks the kernel. Attention leaves out nodes beyond */
+    int max_nodes;               /* of a sequence, 1..64; picks the kernel. Nodes beyond are left out: their rows
+                                    of out stay as they are, and they are not accepted */
     const int32_t* row_off;      /* [n_seq + 1] */
     const int32_t* slot;         /* [n_seq] */
     const int32_t* ctx;          /* [n_seq] */

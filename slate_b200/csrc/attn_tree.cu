@@ -59,9 +59,9 @@ __global__ void __launch_bounds__(32 * NW, 8) attn_tree_rows(
     const int r0 = max(tr.row_off[lo], 0), slot = tr.slot[lo];
     const int ctx = min(max(tr.ctx[lo], 0), c.max_pages * SB_PAGE_TOKENS);
     const int n = min(max(min(tr.row_off[lo + 1], tr.rows) - r0, 0), tr.max_nodes);
-    const bool in = row >= r0 && row < r0 + n;
-    const uint64_t mask = in ? tr.mask[row] : 0;
-    const int end = in ? ctx + n : 0;
+    if (row < r0 || row >= r0 + n) return;               // of no sequence, or beyond max_nodes: left as it is
+    const uint64_t mask = tr.mask[row];
+    const int end = ctx + n;
     float qv[8], o[8], m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {

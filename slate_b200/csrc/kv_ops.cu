@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(AT) tree_accept_kernel(
     __shared__ int src_page[64], src_t[64], dst_page[64], dst_t[64];
     const int s = blockIdx.x, layer = blockIdx.y, tid = threadIdx.x;
     const int r0 = max(tr.row_off[s], 0), r1 = min(tr.row_off[s + 1], tr.rows);
-    const int n = min(max(r1 - r0, 0), SLATE_TREE_MAX_NODES);
+    const int n = min(max(r1 - r0, 0), tr.max_nodes);    // as the attention
     const uint64_t live = n == 64 ? ~0ull : (1ull << n) - 1;
     const int slot = tr.slot[s], ctx = min(max(tr.ctx[s], 0), c.max_pages * SB_PAGE_TOKENS);
     uint64_t m = 0;

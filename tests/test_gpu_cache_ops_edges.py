@@ -291,3 +291,37 @@ def test_queries_with_one_large_dim(sb, outlier, nodes, nq, nkv, hd, kv):
     q = rng.normal(0, 1, (nodes, nq, hd)).astype(np.float32)
     q[..., 5] = outlier
     check(attend(sb, c, 0, [nodes], [ctx], masks, q, hd ** -0.5), *plain(c, 0, [nodes], [ctx], masks, q, hd ** -0.5))
+
+
+# ------------------------------------------------------------- nodes and masks beyond what a step names
+@pytest.mark.parametrize("kv", [F32, F16, Q8])
+@pytest.mark.parametrize("hd,nq", [(64, 2), (128, 16), (64, 32), (24, 4)])
+def test_rows_of_nodes_beyond_max_nodes_stay_as_they_are(sb, hd, nq, kv):
+    rng = np.random.default_rng(1)
+    c = Cache(sb, kv, 1, 2, hd, [60, 60], seed=1)
+    masks = np.concatenate([sb.tree_masks(random_tree(rng, n)) for n in (9, 1)])
+    q = rng.normal(0, 1, (10, nq, hd)).astype(np.float32)
+    got = attend(sb, c, 0, [9, 1], [40, 50], masks, q, 0.1, max_nodes=5)
+    assert (got[5:9] == 9).all() and (got[:5] != 9).all() and (got[9] != 9).all()
+
+
+def accept(sb, c, nodes, ctx, masks, parents, tokens, targets, max_nodes):
+    off = np.concatenate([[0], np.cumsum(nodes)]).astype(np.int32)
+    keep = [dev(off), dev(np.arange(len(nodes), dtype=np.int32)), dev(np.array(ctx, np.int32)), dev(np.asarray(masks, np.uint64).view(np.int64)),
+            *(dev(np.asarray(x, np.int32)) for x in (parents, tokens, targets))]
+    tree = sb.TreeBatch(n_seq=len(nodes), rows=int(off[-1]), max_nodes=max_nodes, row_off=keep[0].data_ptr(), slot=keep[1].data_ptr(),
+                        ctx=keep[2].data_ptr(), mask=keep[3].data_ptr())
+    cnt = torch.full((len(nodes),), -7, dtype=torch.int32, device="cuda")
+    node, tok = (torch.full((len(nodes), 64), -7, dtype=torch.int32, device="cuda") for _ in range(2))
+    sb.tree_accept(c.desc, tree, *(k.data_ptr() for k in keep[4:]), cnt.data_ptr(), node.data_ptr(), tok.data_ptr())
+    return cnt.tolist(), node.cpu().numpy(), tok.cpu().numpy()
+
+
+def test_accept_leaves_out_nodes_beyond_max_nodes(sb):
+    """A chain of seven nodes that all match, of which the step names four (one more sequence keeps
+    rows within n_seq * max_nodes)."""
+    c = Cache(sb, F16, 2, 1, 64, [40, 40])
+    parents = np.arange(7) - 1
+    cnt, node, tok = accept(sb, c, [7, 1], [20, 30], np.r_[sb.tree_masks(parents), [np.uint64(1)]], np.r_[parents, -1], np.r_[np.arange(7), 3],
+                            np.r_[np.arange(1, 8), 4], 4)
+    assert cnt == [4, 1] and node[0, :5].tolist() == [0, 1, 2, 3, -1] and tok[0, :5].tolist() == [1, 2, 3, 4, -1]
