@@ -302,9 +302,10 @@ int slate_cuda_attention_tree(const slate_kv_cache_t* cache, int layer, const sl
  * sequence (-1: none, the node is taken as given).  A node is accepted when it
  * and all nodes of its mask are given or equal their parents' target; the
  * deepest accepted node (most mask bits; ties to the lowest index) ends the
- * path.  For sequence s: out_count[s] = nodes of the path, out_node[s][64] their
- * indexes and out_token[s][64] their targets (the new tokens), -1 beyond; the
- * path's K/V rows of every layer are moved to places ctx[s], ctx[s] + 1, ...
+ * path, which is the nodes of its mask.  For sequence s: out_count[s] = nodes of
+ * the path, out_node[s][64] their indexes and out_token[s][64] their targets (the
+ * new tokens), -1 beyond; the path's K/V rows of every layer are moved to places
+ * ctx[s], ctx[s] + 1, ...
  * (ctx itself is not changed). */
 int slate_cuda_tree_accept(const slate_kv_cache_t* cache, const slate_tree_t* tree,
                            const int32_t* parent, const int32_t* token, const int32_t* target,

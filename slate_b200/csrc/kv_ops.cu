@@ -397,8 +397,8 @@ __global__ void __launch_bounds__(AT) tree_accept_kernel(
     __syncthreads();
     if (tid < 64) {
         const uint64_t ok = ok_s[0] | (uint64_t)ok_s[1] << 32;
-        // deepest first, then the lowest index
-        const int score = tid < n && !(m & ~ok) ? __popcll(m) * 64 + 63 - tid : 0;
+        // the node itself and all of its mask; deepest first, then the lowest index
+        const int score = tid < n && !((m | 1ull << tid) & ~ok) ? __popcll(m) * 64 + 63 - tid : 0;
         const int b = (int)__reduce_max_sync(FULL, (unsigned)score);
         if ((tid & 31) == 0) best_s[tid >> 5] = b;
     }

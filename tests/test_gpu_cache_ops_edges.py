@@ -325,3 +325,17 @@ def test_accept_leaves_out_nodes_beyond_max_nodes(sb):
     cnt, node, tok = accept(sb, c, [7, 1], [20, 30], np.r_[sb.tree_masks(parents), [np.uint64(1)]], np.r_[parents, -1], np.r_[np.arange(7), 3],
                             np.r_[np.arange(1, 8), 4], 4)
     assert cnt == [4, 1] and node[0, :5].tolist() == [0, 1, 2, 3, -1] and tok[0, :5].tolist() == [1, 2, 3, 4, -1]
+
+
+def test_accept_of_a_node_whose_mask_does_not_name_it(sb):
+    """The node itself has to match too, whether or not its mask has its own bit."""
+    c = Cache(sb, F16, 1, 1, 64, [40])
+    masks = np.array([0b1, 0b11, 0b011, 0b011], np.uint64)               # nodes 2 and 3: their ancestors alone
+    parents, targets = [-1, 0, 1, 1], [5, 6, 7, 8]
+    cnt, node, _ = accept(sb, c, [4], [20], masks, parents, [1, 9, 6, 4], targets, 4)      # node 1 fails: the root alone
+    assert cnt == [1] and node[0, 0] == 0
+    cnt, node, _ = accept(sb, c, [4], [20], np.array([0b1, 0b10, 0b1, 0b1], np.uint64), [-1, 0, 0, 0], [1, 9, 4, 3], targets, 4)
+    assert cnt == [1] and node[0, 0] == 0
+    masks = np.array([0b1, 0b11, 0b1011, 0b0011], np.uint64)             # the deepest by its mask does not match itself
+    cnt, node, _ = accept(sb, c, [4], [20], masks, [-1, 0, 1, 1], [1, 5, 4, 6], targets, 4)
+    assert cnt == [2] and node[0, :2].tolist() == [0, 1]
