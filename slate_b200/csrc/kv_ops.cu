@@ -30,7 +30,7 @@ constexpr unsigned FULL = 0xffffffffu;
 // on the side that the plain f32 formula gives.
 __global__ void __launch_bounds__(256) rope_append_kernel(
     const slate_kv_cache_t c, int layer, const slate_rope_t rope, int rows, int nq,
-    float* __restrict__ q_out, int ld_qo, const float* q, int ld_q, const float* __restrict__ k,
+    float* q_out, int ld_qo, const float* q, int ld_q, const float* __restrict__ k,
     int ld_k, const float* __restrict__ v, int ld_v, const int32_t* __restrict__ row_slot,
     const int32_t* __restrict__ row_index, const int32_t* __restrict__ row_pos) {
     chain();

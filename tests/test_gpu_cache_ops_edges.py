@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_cache_ops import F16, F32, NP, Q8, Cache, attend, check, dev, plain, random_tree
+from test_gpu_cache_ops import F16, F32, NP, Q8, Cache, attend, check, dev, f32_rotate, plain, random_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -339,3 +339,26 @@ def test_accept_of_a_node_whose_mask_does_not_name_it(sb):
     masks = np.array([0b1, 0b11, 0b1011, 0b0011], np.uint64)             # the deepest by its mask does not match itself
     cnt, node, _ = accept(sb, c, [4], [20], masks, [-1, 0, 1, 1], [1, 5, 4, 6], targets, 4)
     assert cnt == [2] and node[0, :2].tolist() == [0, 1]
+
+
+# ------------------------------------------------------------- buffers, graphs, streams
+@pytest.mark.parametrize("kv", [F32, F16, Q8])
+@pytest.mark.parametrize("hd,rot,layout,odd", [(64, 64, 0, 1), (128, 64, 1, 1), (256, 256, 0, 0), (20, 14, 1, 3), (128, 128, 0, 0)])
+def test_rope_append_in_place(sb, hd, rot, layout, odd, kv):
+    """q_out = q, a part of the row that k and v come from, on strides that vectors take and on others."""
+    nq, nkv, rows = 6, 2, 37
+    c = Cache(sb, kv, 1, nkv, hd, [rows], seed=3, fill=False)
+    rng = np.random.default_rng(hd)
+    ld = (nq + 2 * nkv) * hd + odd
+    x = rng.normal(0, 1, (rows, ld)).astype(np.float32)
+    cos, sin = sb.rope_tables(500, rot, 1e4)
+    pos = rng.integers(0, 500, rows).astype(np.int32)
+    d, dc, ds, dp, i = dev(x), dev(cos), dev(sin), dev(pos), dev(np.arange(rows, dtype=np.int32))
+    z = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    rope = sb.Rope(cos=dc.data_ptr(), sin=ds.data_ptr(), n_pos=500, rot_dim=rot, layout=layout)
+    p = d.data_ptr()
+    sb.rope_append(c.desc, 0, rope, rows, nq, p, ld, p, ld, p + 4 * nq * hd, ld, p + 4 * (nq + nkv) * hd, ld, z.data_ptr(), i.data_ptr(),
+                   dp.data_ptr())
+    want = x.copy()
+    want[:, :nq * hd] = f32_rotate(x[:, :nq * hd].reshape(rows, nq, hd), cos[pos], sin[pos], rot, layout).reshape(rows, -1)
+    assert np.array_equal(d.cpu().numpy(), want)
