@@ -362,3 +362,114 @@ def test_rope_append_in_place(sb, hd, rot, layout, odd, kv):
     want = x.copy()
     want[:, :nq * hd] = f32_rotate(x[:, :nq * hd].reshape(rows, nq, hd), cos[pos], sin[pos], rot, layout).reshape(rows, -1)
     assert np.array_equal(d.cpu().numpy(), want)
+
+
+class Step:
+    """A layer's calls over device buffers that a graph can hold: append the nodes, attend, accept, read back."""
+
+    def __init__(self, sb, kv, hd, nq, nodes, ctx, seed):
+        rng = np.random.default_rng(seed)
+        self.sb, self.nq, self.hd, self.nkv = sb, nq, hd, 2
+        self.rows = sum(nodes)
+        self.c = Cache(sb, kv, 1, 2, hd, [x + n + 40 for x, n in zip(ctx, nodes)], seed=seed)
+        parents = [random_tree(rng, n) for n in nodes]
+        cos, sin = sb.rope_tables(3000, hd, 1e4)
+        i32 = lambda a: dev(np.asarray(a, np.int32))  # noqa: E731
+        self.off, self.slot, self.ctx = i32(np.concatenate([[0], np.cumsum(nodes)])), i32(np.arange(len(nodes))), i32(ctx)
+        self.mask = dev(np.concatenate([sb.tree_masks(p) for p in parents]).view(np.int64))
+        self.parent, self.token, self.target = i32(np.concatenate(parents)), i32(rng.integers(0, 3, self.rows)), i32(rng.integers(0, 3, self.rows))
+        self.row_slot = i32(np.repeat(np.arange(len(nodes)), nodes))
+        self.index = i32(np.concatenate([x + np.arange(n) for x, n in zip(ctx, nodes)]))
+        self.cos, self.sin = dev(cos), dev(sin)
+        self.qkv = dev(rng.normal(0, 1, (self.rows, (nq + 4) * hd)).astype(np.float32))
+        self.q, self.out = (torch.zeros(self.rows, nq * hd, device="cuda") for _ in range(2))
+        self.K, self.V = (torch.zeros(self.rows, 2 * hd, device="cuda") for _ in range(2))
+        self.cnt = torch.zeros(len(nodes), dtype=torch.int32, device="cuda")
+        self.node, self.new = (torch.zeros(len(nodes), 64, dtype=torch.int32, device="cuda") for _ in range(2))
+        self.rope = sb.Rope(cos=self.cos.data_ptr(), sin=self.sin.data_ptr(), n_pos=3000, rot_dim=hd, layout=0)
+        self.tree = sb.TreeBatch(n_seq=len(nodes), rows=self.rows, max_nodes=max(nodes), row_off=self.off.data_ptr(), slot=self.slot.data_ptr(),
+                                 ctx=self.ctx.data_ptr(), mask=self.mask.data_ptr())
+        self.ws = torch.empty(sb.attention_tree_workspace(self.c.desc, nq, len(nodes), self.rows, max(nodes)), dtype=torch.uint8, device="cuda")
+        self.pool0 = self.c.pool.clone()
+        torch.cuda.synchronize()
+
+    def reset(self):
+        self.c.pool.copy_(self.pool0)
+        for x in (self.q, self.out, self.K, self.V, self.cnt, self.node, self.new):
+            x.zero_()
+
+    def run(self, stream):
+        sb, p, ld, nq, hd = self.sb, self.qkv.data_ptr(), (self.nq + 4) * self.hd, self.nq, self.hd
+        sb.rope_append(self.c.desc, 0, self.rope, self.rows, nq, self.q.data_ptr(), nq * hd, p, ld, p + 4 * nq * hd, ld, p + 4 * (nq + 2) * hd,
+                       ld, self.row_slot.data_ptr(), self.index.data_ptr(), self.index.data_ptr(), stream)
+        sb.attention_tree(self.c.desc, 0, self.tree, nq, self.out.data_ptr(), nq * hd, self.q.data_ptr(), nq * hd, hd ** -0.5,
+                          self.ws.data_ptr(), self.ws.numel(), stream)
+        sb.tree_accept(self.c.desc, self.tree, self.parent.data_ptr(), self.token.data_ptr(), self.target.data_ptr(), self.cnt.data_ptr(),
+                       self.node.data_ptr(), self.new.data_ptr(), stream)
+        sb.kv_read(self.c.desc, 0, 1, self.rows, self.row_slot.data_ptr(), self.index.data_ptr(), self.K.data_ptr(), self.V.data_ptr(), F32,
+                   stream)
+
+    def results(self):
+        torch.cuda.synchronize()
+        return [x.cpu().numpy() for x in (self.q, self.out, self.K, self.V, self.cnt, self.node, self.new, self.c.pool)]
+
+
+def same(a, b):
+    return all(np.array_equal(x, y) for x, y in zip(a, b))
+
+
+STEPS = [(64, 4, [1, 1, 1], [700, 3, 90]), (128, 8, [5, 2], [333, 0]), (64, 8, [16, 9], [1200, 31]), (128, 16, [40, 13], [260, 1001]),
+         (80, 4, [6], [100])]
+
+
+@pytest.mark.parametrize("kv", [F32, F16, Q8])
+@pytest.mark.parametrize("hd,nq,nodes,ctx", STEPS)
+def test_a_captured_step(sb, hd, nq, nodes, ctx, kv):
+    """A graph of all four operators gives what the calls give, and reads lengths, places, masks and
+    inputs anew at every replay."""
+    s = Step(sb, kv, hd, nq, nodes, ctx, 5)
+    s.run(torch.cuda.current_stream().cuda_stream)
+    first = s.results()
+    s.reset()
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        s.run(torch.cuda.current_stream().cuda_stream)
+    s.reset()
+    graph.replay()
+    assert same(first, s.results())
+    # longer contexts, other masks and values, in the same buffers
+    s.ctx += 17
+    s.index += 17
+    s.qkv.mul_(-0.5)
+    s.token.copy_(s.token.flip(0))
+    s.mask.copy_(s.mask & -2 | 1)
+    s.reset()
+    s.run(torch.cuda.current_stream().cuda_stream)
+    second = s.results()
+    assert not same(first, second)
+    s.reset()
+    graph.replay()
+    assert same(second, s.results())
+    del graph
+
+
+@pytest.mark.parametrize("kv", [F32, F16, Q8])
+@pytest.mark.parametrize("hd,nq,nodes,ctx", STEPS[:4])
+def test_steps_on_two_streams(sb, hd, nq, nodes, ctx, kv):
+    """Two sequences of calls at the same time, with a cache and a workspace each, give the bits of either alone."""
+    steps = [Step(sb, kv, hd, nq, nodes, ctx, 5), Step(sb, kv, hd, nq, nodes[::-1], ctx[::-1], 6)]
+    alone = []
+    for s in steps:
+        s.run(torch.cuda.current_stream().cuda_stream)
+        alone.append(s.results())
+    streams = [torch.cuda.Stream() for _ in steps]
+    for _ in range(8):
+        for s in steps:
+            s.reset()
+        torch.cuda.synchronize()
+        for s, st in zip(steps, streams):
+            s.run(st.cuda_stream)
+        for s, a in zip(steps, alone):
+            assert same(a, s.results())
