@@ -47,6 +47,7 @@ __global__ void __launch_bounds__(32 * NW, 8) attn_tree_rows(
     const slate_kv_cache_t c, int layer, const slate_tree_t tr, int nq, float* __restrict__ out,
     int ld_out, const float* __restrict__ q, int ld_q, float scale) {
     __shared__ float sm[NW], sl[NW], so[NW][256];
+    sb_grid_wait();
     const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, hd = c.head_dim;
     const int row = blockIdx.x, h = blockIdx.y, kvh = h / (nq / c.n_kv_heads);
     // the row's sequence: the last s with row_off[s] <= row
@@ -1075,7 +1076,7 @@ extern "C" int slate_cuda_attention_tree(const slate_kv_cache_t* cache, int laye
         return f(*cache, layer, *tree, n_heads, out, ld_out, q, ld_q, scale, (float*)ws,
                  (cudaStream_t)stream);
     }
-    attn_tree_rows<<<dim3((unsigned)tree->rows, (unsigned)n_heads), 32 * NW, 0,
-                     (cudaStream_t)stream>>>(*cache, layer, *tree, n_heads, out, ld_out, q, ld_q, scale);
-    return sb_cuda_check(cudaGetLastError(), "attention_tree");
+    return sb_cuda_check(sb_launch_pdl(attn_tree_rows, dim3((unsigned)tree->rows, (unsigned)n_heads), dim3(32 * NW), 0, (cudaStream_t)stream,
+                                       *cache, layer, *tree, n_heads, out, ld_out, q, ld_q, scale),
+                         "attention_tree");
 }

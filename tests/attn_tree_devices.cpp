@@ -10,6 +10,7 @@
 #include "slate_cuda.h"
 
 static int device = 0, set_calls = 0, fail_sets = 0, launches = 0;
+static cudaError_t pending = cudaSuccess;       // of some call before, of another library say
 static std::map<std::pair<int, const void*>, size_t> allowed;
 
 extern "C" {
@@ -20,7 +21,7 @@ void __cudaRegisterFunction(void**, const char*, char*, const char*, int, uint3*
 unsigned __cudaPushCallConfiguration(dim3, dim3, size_t, void*) { return 0; }
 cudaError_t __cudaPopCallConfiguration(dim3*, dim3*, size_t*, void*) { return cudaSuccess; }
 cudaError_t cudaGetDevice(int* d) { *d = device; return cudaSuccess; }
-cudaError_t cudaGetLastError(void) { return cudaSuccess; }
+cudaError_t cudaGetLastError(void) { const cudaError_t e = pending; pending = cudaSuccess; return e; }
 cudaError_t cudaLaunchKernel(const void*, dim3, dim3, void**, size_t, cudaStream_t) { ++launches; return cudaSuccess; }
 cudaError_t cudaFuncSetAttribute(const void* f, cudaFuncAttribute a, int v) {
     ++set_calls;
@@ -68,5 +69,11 @@ int main() {
     device = 70;                                  // an ordinal beyond the ones whose state is kept
     const int a = call(40, 1, 128), b = call(40, 1, 128);
     printf("device 70: %d %d\n", a, b);
+    device = 0;
+    pending = cudaErrorInvalidValue;
+    const int c = call(3, 1, 64);
+    pending = cudaErrorInvalidValue;
+    const int d = call(3, 1, 24);
+    printf("after an error of another call: %d %d\n", c, d);
     return 0;
 }

@@ -36,3 +36,7 @@ def test_a_failure_is_not_remembered(lines):
 
 def test_a_device_beyond_the_known_ordinals(lines):
     assert lines[5] == "device 70: 0 0"
+
+
+def test_an_error_of_another_call_is_not_this_ones(lines):
+    assert lines[6] == "after an error of another call: 0 0"
