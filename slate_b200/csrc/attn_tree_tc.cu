@@ -218,8 +218,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
     __shared__ uint32_t tmem_s;
     __shared__ __align__(8) uint8_t gone_s[SCB][8];                // per page: the table has none
     __shared__ uint16_t odd_s[SCB][8];                             // per page: tokens whose v is not finite
-    __shared__ uint4 vexp_s[SCB][2];                               // per page, 16 bits: exponent of its largest v scale; 255 - that
-                                                                   // of the smallest (0: it has none)
+    __shared__ uint2 vends_s[SCB];                                 // bits of the tile's largest v scale; 0 - those of the
+                                                                   // smallest (0: it has none)
     __shared__ float part_max[2][PARTS][MR];      // [tile parity][part][row]
     __shared__ float part_top[Q8 ? 2 : 1][PARTS][Q8 ? MR : 1];     // alike, of score + exponent of the v scale
     __shared__ int need_s[4];                     // tile % 4: some row's maximum grew beyond LAG
@@ -245,6 +245,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
             bar_init(&bars.dfull[i], 1);
         }
         for (int i = 0; i < 4; ++i) need_s[i] = 0;
+        for (int i = 0; i < SCB; ++i) vends_s[i] = make_uint2(0, 0);
         fail_s = 0;
         sg.at = st_.at;
         sg.stop = st_.stop;
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
             // 8 bits: O is in units of 2^(m + a - (15 - LAG)); 2^a is above every v scale so far, and l's units are
             // the same; once `wide`, a is the row's own and l's units are 2^(m - (15 - LAG))
             float a = -80.f;
-            int vlow = 0;                              // 255 - the smallest v scale's exponent so far
+            uint32_t vlow = 0u - 0x7f7fffffu;          // 0 - the bits of the smallest v scale so far
             bool wide = false;
             bool ok = true;
             const auto scales = [&](int j) { return ssc + (tb + j) % SCB * (2 * KT) + toff(); };
@@ -483,11 +484,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                 }
                 return sum.x + sum.y;
             };
-            const auto of_pages = [&](int j, int k) {
-                const uint4 x = vexp_s[(tb + j) % SCB][k];
-                const uint32_t y = __vmaxu2(__vmaxu2(x.x, x.y), __vmaxu2(x.z, x.w));
-                return (int)max(y & 0xffffu, y >> 16);
-            };
             // the part's maximum of tile j for the row's other threads, and whether anything has to be
             // rescaled for it; a barrier
             const auto publish = [&](int j, float mx, float top, float high) {
@@ -498,7 +494,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                     if (mx * rs > m + (float)LAG || (Q8 && (wide ? top > m + a + (float)LAG : high > a))) need_s[t & 3] = 1;
                 }
                 softmax_sync();
-                if (tid == 0) need_s[(t + 2) & 3] = 0;
+                if (tid == 0) {
+                    need_s[(t + 2) & 3] = 0;
+                    // (before the producers come to that tile, whose K follows the scores of tile t + 2)
+                    if (Q8) vends_s[(t + 4) % SCB] = make_uint2(0, 0);
+                }
             };
             const auto add_d = [&]() {                 // O += D
 #pragma unroll
@@ -515,9 +515,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                 wait_s(j);
                 float high = a;
                 if (Q8 && !wide) {                     // (alike in every thread)
-                    vlow = max(vlow, of_pages(j, 1));
-                    high = fmaxf(a, (float)(of_pages(j, 0) - 126));
-                    if (high > (float)TALL || high + (float)vlow > (float)(SPAN + 129)) {
+                    const uint2 v = vends_s[t % SCB];
+                    vlow = max(vlow, v.y);
+                    high = fmaxf(a, (float)((int)(v.x >> 23) - 126));
+                    if (high > (float)TALL || high - (float)(int)((0u - vlow) >> 23) > (float)(SPAN - 126)) {
                         wide = true;
                         l *= ex2(a);
                     }
@@ -787,25 +788,20 @@ __global__ void __launch_bounds__(NTHREADS, 1) attn_tree_tc(
                         *(uint4*)(dst + (to[i & 1] ^ 16) + TS * i * 128) = z;
                     }
                     if (!(n & 8)) {                    // before kfull: the softmax reads them after the scores
-                        uint32_t vm = 0, vn = 0;
                         if (lane < 4) {
                             float* sc = ssc + sc_ * 2 * KT + 16 * pg + 4 * lane;
                             *(float4*)sc = make_float4(no_inf(k4.x), no_inf(k4.y), no_inf(k4.z), no_inf(k4.w));
                             *(float4*)(sc + KT) = v4;
+                            uint32_t b[4] = {__float_as_uint(v4.x), __float_as_uint(v4.y), __float_as_uint(v4.z), __float_as_uint(v4.w)};
                             const int t = tok0 + j * KT + 16 * pg + 4 * lane;
-                            const float vv[4] = {v4.x, v4.y, v4.z, v4.w};
+                            if (t + 4 > ctx)           // what only some rows see, or none, and is no number: not looked at
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (const uint32_t e = __float_as_uint(vv[i]) >> 23 & 255; t + i < end && vv[i] != 0.f && e < 255) {
-                                    vm = max(vm, e);
-                                    vn = max(vn, 255 - e);
-                                }
+                                for (int i = 0; i < 4; ++i)
+                                    if (t + i >= end || (t + i >= ctx && b[i] >= 0x7f800000u)) b[i] = 0;
+                            atomicMax(&vends_s[sc_].x, max(max(b[0], b[1]), max(b[2], b[3])));
+                            atomicMax(&vends_s[sc_].y, max(max(0u - b[0], 0u - b[1]), max(0u - b[2], 0u - b[3])));
                         }
-                        vm = __reduce_max_sync(FULL, vm);
-                        vn = __reduce_max_sync(FULL, vn);
                         if (lane == 0) {
-                            ((uint16_t*)&vexp_s[sc_][0])[pg] = (uint16_t)vm;
-                            ((uint16_t*)&vexp_s[sc_][1])[pg] = (uint16_t)vn;
                             gone_s[sc_][pg] = r.page < 0;
                         }
                     }
