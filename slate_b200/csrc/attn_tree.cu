@@ -596,8 +596,7 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
                 for (int j = 0; j < NTK; ++j) mx = fmaxf(mx, fmaxf(p[ri][j][0], p[ri][j][1]));
                 mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 2));
-                // (8 bits: to the integer above it, so that o's units, powers of two, can be set against it)
-                const float mn = fmaxf(m[ri], KV == SLATE_KV_Q8 ? ceilf(mx) : mx), base = mn == -INFINITY ? 0.f : mn;
+                const float mn = fmaxf(m[ri], mx), base = mn == -INFINITY ? 0.f : mn;
                 corr[ri] = ex2(m[ri] - base);
                 m[ri] = mn;
                 l[ri] *= corr[ri];
@@ -611,7 +610,7 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
             }
             // ---- weights of v: 8 bits: p vscale against the row's largest so far: that of the tokens which it
             // sees, with their p, so that no scale that weighs nothing in a row takes the others' bits in f16.
-            // vtop = m + its exponent only grows: o is rescaled by a power of two.  0 stays 0 whatever the scale
+            // vtop = m + its log2 only grows.  0 stays 0 whatever the scale
             if (KV == SLATE_KV_Q8) {
                 float vf[NTK][2];
 #pragma unroll
@@ -631,10 +630,10 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
                         }
                     top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
-                    const float grown = fmaxf(vtop[ri], m[ri] + (float)max((int)(__float_as_uint(top) >> 23) - 126, -100));
-                    corr[ri] = __int_as_float((127 + max((int)(vtop[ri] - grown), -126)) << 23);
+                    const float grown = fmaxf(vtop[ri], m[ri] + fmaxf(lg2(top), -100.f));
+                    corr[ri] = ex2(vtop[ri] - grown);
                     vtop[ri] = grown;
-                    const float f = __int_as_float((142 + min(max((int)(m[ri] - grown), -129), 100)) << 23);
+                    const float f = ex2(m[ri] - grown + 15.f);
 #pragma unroll
                     for (int j = 0; j < NTK; ++j) p[ri][j][0] *= f, p[ri][j][1] *= f;
                 }
@@ -812,7 +811,7 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
 #pragma unroll
         for (int ri = 0; ri < RI; ++ri) {
             float* rec = mg + ((size_t)warp * MR + 8 * ri + g) * (HD + 2);
-            const float of = KV == SLATE_KV_Q8    ? __int_as_float((112 + min(max((int)(vtop[ri] - m[ri]), -111), 130)) << 23)
+            const float of = KV == SLATE_KV_Q8    ? ex2(fminf(vtop[ri] - m[ri] - 15.f, 120.f))
                              : KV == SLATE_KV_F16 ? 0x1p-15f
                                                   : 1.f;
             float ls = l[ri];
