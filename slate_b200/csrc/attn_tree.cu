@@ -863,16 +863,17 @@ __global__ void __launch_bounds__(32 * MW, Shape<KV, HD, MODE>::CPS) attn_tree_m
     }
 }
 
-// Rows row0 + i of sequence s and a kv head, for each bit i of `which`, by a warp.
+// Rows row0 + i of sequence s and a kv head, for each bit i of `which`, by a warp (of their dims, `blocks`).
 template <int E>
 __device__ __forceinline__ void rows_by_formula(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int s, int kvh, int G, int row0,
-                                                uint32_t which, float* out, int ld_out, const float* q, int ld_q, float scale) {
+                                                uint32_t which, uint32_t blocks, float* out, int ld_out, const float* q, int ld_q,
+                                                float scale) {
     const Seq a = seq_of(c, tr, s, G, 1, 1);             // (read anew: the sums have no registers for it)
     for (; which; which &= which - 1) {
         const int row = row0 + __ffs(which) - 1, rr = a.r0 + row / G, hd = c.head_dim;
         const size_t head = (size_t)(kvh * G + row % G) * hd;
         row_by_formula<E>(row_job(c, layer, kvh, a.slot, a.ctx, a.n, __ldg(tr.mask + rr)), q + (size_t)rr * ld_q + head, scale,
-                          out + (size_t)rr * ld_out + head);
+                          out + (size_t)rr * ld_out + head, blocks);
     }
 }
 
@@ -904,9 +905,12 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) attn_tree_join(
         const auto place = [&]() { return out + (size_t)(q.r0 + row / G) * ld_out + (size_t)(kvh * G + row % G) * HD; };
         bool nan = false;
         if (n == 1) {                                    // written by its CTA
-            if (nan_words(ws, HD)[c0] && w == 0) {
+            if (nan_words(ws, HD)[c0] && w < E) {
                 const float* o = place();
-                for (int k = 0; k < E; ++k) nan |= o[E * lane + k] != o[E * lane + k];
+                if (W == 1)
+                    for (int k = 0; k < E; ++k) nan |= o[32 * k + lane] != o[32 * k + lane];
+                else
+                    nan = o[32 * w + lane] != o[32 * w + lane];
                 if (__any_sync(FULL, nan)) again |= 1u << (row - row0);
             }
             continue;
@@ -970,6 +974,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) attn_tree_join(
 #pragma unroll
         for (int k = 0; k < E; ++k) so[w][E * lane + k] = O[k];
         __syncthreads();
+        if (tid >= HD) return;
         M = -INFINITY, L = 0.f;
         float x = 0.f;
 #pragma unroll
@@ -978,14 +983,14 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) attn_tree_join(
         for (int i = 0; i < W; ++i) {
             const float f = sm[i] == -INFINITY ? 1.f : ex2(sm[i] - M);
             L = fmaf(sl[i], f, L);
-            if (tid < HD) x = fmaf(so[i][tid], f, x);
+            x = fmaf(so[i][tid], f, x);
         }
         x = L == 0.f ? 0.f : x / L;
-        if (tid < HD) o[tid] = x;
-        if (__syncthreads_or(x != x) && w == 0) again = 1;
+        o[tid] = x;
+        if (__any_sync(FULL, x != x)) again = 1;         // (a warp: the dims that it wrote)
     }
     __syncwarp();                                        // the row's lanes change below
-    if (again) rows_by_formula<E>(c, layer, tr, s, kvh, G, row0, again, out, ld_out, qs, ld_q, scale);
+    if (again) rows_by_formula<E>(c, layer, tr, s, kvh, G, row0, again, W == 1 ? ~0u : 1u << warp, out, ld_out, qs, ld_q, scale);
 }
 
 template <int HD>

@@ -292,9 +292,9 @@ __device__ __forceinline__ float kv_element(const unsigned char* blk, int kv_dty
            : kv_dtype == SLATE_KV_F16 ? __half2float(((const __half*)blk)[at])
                                       : (float)((const int8_t*)blk)[SB_Q8_SCALES + at];
 }
-// E: dims a lane, head_dim up to 32 E
+// E: dims a lane, head_dim up to 32 E; writes the blocks of 32 dims that `blocks` has bits for
 template <int E>
-__device__ __forceinline__ void row_by_formula(const RowJob& j, const float* q, float scale, float* out) {
+__device__ __forceinline__ void row_by_formula(const RowJob& j, const float* q, float scale, float* out, uint32_t blocks = ~0u) {
     const int lane = threadIdx.x & 31;
     const bool q8 = j.kv_dtype == SLATE_KV_Q8;
     float qv[E], top = -INFINITY;
@@ -338,7 +338,7 @@ __device__ __forceinline__ void row_by_formula(const RowJob& j, const float* q, 
     const float inv = l == 0. ? 0.f : 1.f / (float)l;
 #pragma unroll
     for (int i = 0; i < E; ++i)
-        if (lane + 32 * i < j.hd) out[lane + 32 * i] = nan ? NAN : (float)(o[i] * inv);
+        if (lane + 32 * i < j.hd && blocks >> i & 1) out[lane + 32 * i] = nan ? NAN : (float)(o[i] * inv);
 }
 
 // attn_tree_tc.cu: rows in tiles of TC_ROWS, units of TC_UNIT tokens, SMS CTAs; two
