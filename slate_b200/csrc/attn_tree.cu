@@ -179,8 +179,9 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
 // chunk each) nor the f32 reads (4 or 8 rows) meet in a bank.
 template <int KV, int HD, int MODE>
 struct Shape {
-    // (f32: a unit's arithmetic takes longer than what a second range costs; 16 x 7 nodes over 1501
-    // tokens 43.2 us, with 2 45.4)
+    // (f32: a unit's arithmetic takes longer than what a second range costs; with 0, 1 and 4: 16 x 7 nodes over 700
+    // tokens 31.2, 29.0 and 28.9 us, over 1501 42.6, 42.6 and 44.4, over 3000 64.3, 64.4 and 71.2, 5 x 1 over 6000
+    // at head_dim 128 41.8, 39.8 and 39.8)
     static constexpr int SLACK = KV == SLATE_KV_F32 ? 1 : 4;
     static constexpr int RB = KV == SLATE_KV_F32 ? 4 * HD : KV == SLATE_KV_F16 ? 2 * HD : HD;
     static constexpr int KT = RB == 512 ? 8 : RB == 256 ? 16 : 32;
@@ -193,8 +194,8 @@ struct Shape {
     static constexpr int KS = I8 ? HD / 32 : KV == SLATE_KV_F32 ? HD / 8 : HD / 16;    // k steps of a score
     static constexpr int HL = I8 ? 2 * MODE + 2 : MODE == 0 ? 1 : 2;    // A operands a k step
     static constexpr int QB = MT * KS * HL * 512;
-    // CTAs an SM: three where 168 registers a thread do (64 sequences of one node over 4096 tokens 54.9
-    // us, with two 60.3; head_dim 128 spills, 93 against 84)
+    // CTAs an SM: three where 168 registers a thread do (64 sequences of one node over 4096 tokens 57
+    // us, with two 62; head_dim 128 spilled with three, 93 against 84)
     static constexpr int CPS = KV == SLATE_KV_Q8 && HD == 64 && MODE == 0 ? 3 : 2;
     static_assert(CPS * MR <= TC_ROWS && CPS * SMS <= MAX_CTAS, "workspace");
     static constexpr int NS0 = ((CPS == 3 ? 74 : 112) * 1024 - QB) / (MW * TB);
@@ -214,11 +215,13 @@ __device__ __forceinline__ uint32_t swz(int row, int chunk) {
     return row * RB + ((chunk ^ (row & 7)) << 4);
 }
 
-// A CTA of four warps, each with its own ring of tiles.  Bound by HBM for up to 16 rows: 64
-// sequences of one node over 4096 tokens, 32 heads over 8 of 128, 8 bits: 84 us, 5.0 TB/s.  f32 with 32
-// rows is bound by the three tf32 products and the latency between them (two warps a scheduler, 255
-// registers each): 16 x 7 nodes over 1501 tokens, 32 heads over 8 of 64: 42.6 us, 1.8 TB/s (12000
-// tokens: 177 us, 3.3 TB/s).  One node over 700 tokens: 8.7 us, two launches and five dependent
+// A CTA of four warps, each with its own ring of tiles.  What bounds it: HBM for up to 8 rows of f16 and f32 (64
+// sequences of one node over 4096 tokens, 32 heads over 8 of 128: 129 and 243 us, 6.2 and 6.6 TB/s).  8 bits: neither
+// HBM (60 % busy) nor the issue slots (54 %), but the latency between a warp's own instructions, two warps a
+// scheduler at 253 registers (the same call: 85 us, 4.9 TB/s).  f32 with 32
+// rows: the three tf32 products and the latency between them, again two warps a scheduler:
+// 16 x 7 nodes over 1501 tokens, 32 heads over 8 of 64: 42.5 us, 1.8 TB/s (12000
+// tokens: 179 us, 3.3 TB/s).  One node over 700 tokens: 8.9 us, two launches and five dependent
 // reads.
 // Partial of one cut item: [MR][HD + 2]: (max in log2 units, sum, o) rows.
 template <int KV, int HD, int MODE>
@@ -886,7 +889,9 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) attn_tree_join(
     const slate_kv_cache_t c, int layer, const slate_tree_t tr, int nq, int MR, int unit, int slack, int ctas, int rpc,
     float* __restrict__ out, int ld_out, const float* __restrict__ qs, int ld_q, float scale, const float* __restrict__ ws) {
     constexpr int E = HD / 32;                           // dims a lane: 2 or 4
-    constexpr int F = W == 1 && HD == 128 ? 6 : 8;       // records in flight; 8 would take more than 72 registers there
+    // records in flight: at head_dim 128 eight take more than the 72 registers (of a warp a row) that seven CTAs an SM
+    // leave, and an eighth of the threads an SM with eight warps a row
+    constexpr int F = HD == 128 ? 6 : 8;
     __shared__ PlanBuf buf;
     __shared__ float sm[W], sl[W], so[W][HD];
     const int nkv = c.n_kv_heads, G = nq / nkv, tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
@@ -998,7 +1003,8 @@ int join(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, int nq, i
          int ld_out, const float* q, int ld_q, float scale, float* ws, cudaStream_t st) {
     const int R = tr.max_nodes * (nq / c.n_kv_heads);
     // eight warps a row where an item, if long, is cut into eight records or more: one token over 3000
-    // tokens of 8 heads 13.5 us against 18.7 with a warp a row (whole calls); more items than that fill
+    // tokens of 8 heads 10.2 us against 12.9 with a warp a row, over 700 9.1 against 9.6 (whole calls; 16 nodes over
+    // 100 tokens, which are not cut, 16.0 against 14.0); more items than that fill
     // the GPU with a warp a row
     if ((int64_t)tr.n_seq * c.n_kv_heads * ((R + MR - 1) / MR) * 8 <= ctas)
         return sb_cuda_check(sb_launch_pdl(attn_tree_join<HD, 8>, dim3((unsigned)(tr.n_seq * R), (unsigned)c.n_kv_heads), dim3(256), 0,
@@ -1028,8 +1034,8 @@ int launch_mode(const slate_kv_cache_t& c, int layer, const slate_tree_t& tr, in
                 int ld_out, const float* q, int ld_q, float scale, float* ws, cudaStream_t st) {
     const int M = tr.max_nodes * (nq / c.n_kv_heads);
     // attn_tree_mma with 32 rows against attn_tree_tc, 16 sequences of 8 nodes x 4 heads: head_dim 128 over
-    // 1000 tokens of 8 bits 36 and 31 us, over 8000 103 and 103, of f16 113 and 87; head_dim 64 over 8000 of
-    // f16 63 and 69, of 8 bits 61 and 91
+    // 1000 tokens of 8 bits 37.5 and 32.3 us, over 8000 110 and 103, of f16 103 and 86; head_dim 64 over 8000 of
+    // f16 59.6 and 69.7, of 8 bits 62 and 89
     constexpr int few = KV != SLATE_KV_F32 && HD == 128 ? 16 : 32;
     if (M <= 8) return launch_mma<KV, HD, 0>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);
     if (M <= 16) return launch_mma<KV, HD, 1>(c, layer, tr, nq, out, ld_out, q, ld_q, scale, ws, st);

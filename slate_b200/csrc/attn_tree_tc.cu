@@ -19,14 +19,15 @@
 // its own row moved a sector an element: 15.5 us for one tile a CTA against 21.8).
 // SPLIT, up to 64 rows: lanes 64-127 would idle, and the softmax of a tile is what the next waits for;
 // so they hold the rows again, each lane takes half of a tile's tokens (P is 0 for the others), and
-// a row's two lanes are joined like two CTAs' parts (8 x 16 nodes of f16: 50.5 us against 52.3, at
-// head_dim 64 42.8 against 47.0).
+// a row's two lanes are joined like two CTAs' parts (8 x 16 nodes of f16: 51 us against 54, at
+// head_dim 64 44 against 47.5, of 8 bits 60 against 64).
 // What bounds it.  256 rows and more over long contexts (4 sequences of 64 nodes, 64 heads over
-// 8, 32000 tokens of 8 bits: 436 us, 415 TFLOP/s of the formula, 830 with both halves): the softmax's
-// issue slots, two passes over S with an exponential and a split a score, next to tensor cores that
+// 8, 32000 tokens of 8 bits: 438 us, 413 TFLOP/s of the formula, 827 with both halves): the softmax's
+// issue slots (59 % busy), two passes over S with an exponential and a split a score, next to tensor cores that
 // are busy about half of the time.  Few rows (8 sequences of 16 nodes, 32 heads over 8, 8000 tokens
-// of f16: 50.6 us, 3.2 TB/s): the loads within the tiles, then what a CTA does before the first tile
-// and after the last, some 20 us of the call.
+// of f16: 51 us, 3.1 TB/s): the loads within the tiles, then what a CTA does before the first tile
+// and after the last, some 20 us of the call.  8 bits with as few rows (60 us, 1.4 TB/s): widening K and V to f16
+// through registers, with two buffers, for products of which half are padding.
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -54,7 +55,8 @@ constexpr int LAG = 8;
 // 8 bits: as long as a range's v scales lie within 2^SPAN (and below 2^TALL), p v's factor in f16 is set
 // by the largest of them, for all rows alike: a row's top token then keeps 31 - SPAN bits, and the sum l takes the
 // same factor.  From the first tile on where they do not, each row has its own, by the tokens that it sees and
-// their p, and l none (see `wide`).  Weights and activations leave scales within 2^7 or so.
+// their p, and l none (see `wide`): 4 x 64 nodes over 32000 tokens 774 us instead of 438, 8 x 16 over 8000 75 instead
+// of 60.  Scales that spread like exp(normal / 2) stay within 2^7.
 constexpr int SPAN = 10, TALL = 40;
 // Tiles that D may add up before it is drained (a power of two).  The tensor cores cut each
 // step's sum off: 8 tiles, 128 steps, cost 1e-6 of the output at worst, one tile 1e-7.
@@ -63,8 +65,8 @@ constexpr int RUN = 8;
 template <int KV, int HD>
 struct TcShape {
     // K and V tiles in shared memory, of each: the 8-bit producers go through registers and
-    // the first-level cache, which a third pair would leave little of (490 against 550 us at 256
-    // rows over 32000 tokens); f16 keeps more copies in flight with three (76 against 66 us, 64 rows)
+    // the first-level cache, which a third pair would leave little of (256 rows over 32000 tokens took 550 us with
+    // three, 490 with two, when this was chosen); f16 keeps more copies in flight with three (64 rows 66 us, with two 76)
     static constexpr int NB = KV == SLATE_KV_Q8 ? 2 : 3;
     static constexpr int TB = KT * HD * 2;                 // a K or V tile in f16
     static constexpr int SC = SCB * 2 * KT * 4;

@@ -1,7 +1,7 @@
 /*
  * sb_tree.h -- what the tree-attention kernels share (attn_tree.cu,
- * attn_tree_tc.cu; internal, CUDA C++ only): the cut of the work over the CTAs
- * and the splitting of operands.
+ * attn_tree_tc.cu; internal, CUDA C++ only): the cut of the work over the CTAs,
+ * the splitting of operands and the rows that halves cannot form.
  */
 #ifndef SB_TREE_H
 #define SB_TREE_H
@@ -138,8 +138,8 @@ __device__ __forceinline__ Seq seq_from(const Seq& q, int lane) {
 }
 // A second range costs a CTA about `slack` units (q, the first tile's latency, O): a unit of T
 // units, T up to `slack` more than the even share, is taken if that leaves a CTA one range.
-// 8 x 16 nodes over 8000 tokens of f16: 54 us against 60 with even ranges (slack 4; 16 made 20000
-// tokens slower, 140 against 131); one token over 3000 of 8 bits: 9.9 against 13.6.
+// 8 x 16 nodes over 8000 tokens of f16: 51 us against 58 with slack 0, of 8 bits 60 against 68 (slack 4; 16 makes 20000
+// tokens slower, 136 against 127).
 __device__ __forceinline__ int64_t plan_warp(const slate_kv_cache_t& c, const slate_tree_t& tr, int G, int MR,
                                              int& unit, int slack, int ctas, Seq& q, int64_t& before) {
     const int lane = threadIdx.x & 31;

@@ -147,6 +147,31 @@ def test_v_scales_that_grow_along_the_context(sb, level, slope, nodes, nq, nkv, 
     check(attend(sb, c, 0, [nodes], [ctx], masks, q, 1.0), *plain(c, 0, [nodes], [ctx], masks, q, 1.0))
 
 
+@pytest.mark.parametrize("nodes,nq,nkv,hd", [(1, 4, 1, 128), (4, 4, 1, 64), (8, 4, 1, 64), (5, 4, 1, 128), (16, 4, 1, 128), (11, 4, 1, 64), (30, 4, 1, 64)])
+def test_v_scales_of_many_sequences(sb, nodes, nq, nkv, hd):
+    """8 bits: sequences of even scales beside others whose scales spread over 2^20, more of them than workers: what
+    one leaves in a worker does not reach the next."""
+    rng = np.random.default_rng(nodes)
+    n = 170
+    counts = [nodes - s % 2 * (nodes // 2) for s in range(n)]
+    ctx = [int(x) for x in rng.integers(100, 420, n)]
+    c = Cache(sb, Q8, 1, nkv, hd, [x + k for x, k in zip(ctx, counts)], seed=8)
+    e, s = c.parts()
+    for i in range(0, n, 3):
+        for page in c.table[i, :-(-(ctx[i] + counts[i]) // 16)]:
+            s[0, page, 1] *= np.exp2(rng.uniform(0, 20, 16)).astype(np.float32)
+    raw = c.raw().copy()
+    raw[..., :64] = s.view(np.uint8)
+    c.pool.copy_(torch.from_numpy(raw.reshape(-1)))
+    masks = np.concatenate([sb.tree_masks(random_tree(rng, k)) for k in counts])
+    q = rng.normal(0, 1, (sum(counts), nq, hd)).astype(np.float32)
+    got = attend(sb, c, 0, counts, ctx, masks, q, hd ** -0.5)
+    want, size = plain(c, 0, counts, ctx, masks, q, hd ** -0.5)
+    at = np.repeat(np.arange(n) % 3 == 0, counts)                # apart: their outputs differ in size
+    check(got[at], want[at], size)
+    check(got[~at], want[~at], size)
+
+
 # ------------------------------------------------------------- infinities that a row sees
 def formula(c, nodes, ctx, masks, q, scale):
     """The formula in f64 with infinities and NaN: a key of score -inf is as if not seen; one of +inf or NaN
