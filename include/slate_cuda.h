@@ -242,10 +242,10 @@ int slate_rope_tables(float* cos, float* sin, int n_pos, int rot_dim, float thet
 /* For each of `rows` tokens r: q_out[r] = q[r] (n_heads heads, f32, row strides
  * ld_q / ld_q_out in floats) turned to position row_pos[r]; k[r] turned and
  * v[r] (n_kv_heads heads) written to place row_index[r] of slot row_slot[r] in
- * `layer`, rounded to f16 or quantised to 8 bits as they are written.  q_out
- * may be q; q, k and v may be parts of one row (one ld).  A row with a negative
- * row_index or a row_pos outside the tables is skipped; two rows of a call must
- * not name the same place. */
+ * `layer`, rounded to f16 (an infinity from 65520 on) or quantised to 8 bits as
+ * they are written.  q_out may be q; q, k and v may be parts of one row (one ld).
+ * A row with a negative row_index or a row_pos outside the tables is skipped; two
+ * rows of a call must not name the same place. */
 int slate_cuda_rope_append(const slate_kv_cache_t* cache, int layer, const slate_rope_t* rope,
                            int rows, int n_heads, float* q_out, int ld_q_out, const float* q,
                            int ld_q, const float* k, int ld_k, const float* v, int ld_v,
